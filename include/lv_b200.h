@@ -47,7 +47,9 @@ enum { LV_TYPE_F32 = 0, LV_TYPE_F16 = 1, LV_TYPE_Q4_0 = 2, LV_TYPE_Q8_0 = 8,
         * matmul_silu_ff.comp without the _fp16 suffix).  Not a GGML code: such files say "q4_0" too. */
        LV_TYPE_Q4_0_V1 = 258,
        /* bfloat16 and 32-bit integers of safetensors files, under GGML's codes */
-       LV_TYPE_I32 = 26, LV_TYPE_BF16 = 30 };
+       LV_TYPE_I32 = 26, LV_TYPE_BF16 = 30,
+       /* 8-bit values of paged caches: int8 (GGML's code) and the 8-bit floating type with 4 exponent and 3 fraction bits and no infinities (no GGML code) */
+       LV_TYPE_I8 = 24, LV_TYPE_E4M3 = 259 };
 
 typedef struct lv_ctx lv_ctx;
 typedef struct lv_graph lv_graph;
@@ -636,6 +638,116 @@ typedef struct lv_ssm_args {
 uint32_t lv_ssm_state_rows(uint32_t state);
 size_t lv_ssm_scratch_bytes(const lv_ssm_args* a, uint32_t batch);
 int lv_ssm(lv_ctx* ctx, const lv_ssm_args* a, void* scratch, size_t scratch_bytes, uint32_t batch);
+
+/* ---- a cache in pages, shared by sequences of different lengths (no counterpart in the reference, whose sessions hold one
+ *      contiguous cache each) --------------------------------------------------------------------------------------------
+ *
+ * A step takes the new tokens of every sequence: one each when they decode, several with drafted tokens, thousands of a prompt, in any mix.
+ * Its calls are lv_paged_append and lv_paged_attention for every layer, lv_probabilities and lv_verify_drafts behind the output head.
+ *
+ * Sequence s has lens[s] positions, the new ones among them; its new tokens are the rows starts[s] .. starts[s + 1] - 1 of the step's rows
+ * (starts[0] is the first row; starts do not decrease), which are its last positions.  Rows from starts[seqs] on belong to nobody and stay as they
+ * are.  Position i lies in row i mod page_rows of page table[s * table_ld + i / page_rows].  Two sequences may share a page that neither appends to.
+ * lens, starts and the table are device memory, so that a recorded step serves every token.  What they say is checked on the device: a length beyond
+ * table_ld * page_rows, new tokens beyond the step's rows, beyond the stated upper bounds or before position 0, and pages beyond `pages` set the error word
+ * (lv_stream_sync); such a sequence is left out, and positions of a page that is not there count as masked.
+ *
+ * 8-bit types hold one f32 scale per row and head: value = code * scale, scale = a / top and code = round(x * (top / a)) to the nearest (ties to
+ * even), a = max |x| of the row, top = 127 (LV_TYPE_I8) or 448 (LV_TYPE_E4M3).  A row with a < 2^-100 is stored as zeros, one that is not finite with
+ * a NaN as its scale.
+ *
+ * The argument checks come before the context's: a call without a context says what else is wrong with it. */
+typedef struct lv_paged_cache {
+    void* k;                        /* [pages][kv_heads][page_rows][dim] of `type`, 16-byte aligned */
+    void* v;
+    float* k_scale;                 /* 8-bit types: f32 [pages][kv_heads][page_rows]; else unused */
+    float* v_scale;
+    int type;                       /* LV_TYPE_F16, LV_TYPE_BF16, LV_TYPE_I8 or LV_TYPE_E4M3 */
+    uint32_t pages, page_rows, kv_heads;
+    uint32_t dim;                   /* of a head: a multiple of 16, at most 256 */
+    const uint32_t* table;          /* [seqs][table_ld] */
+    uint32_t table_ld;
+    const uint32_t* lens;           /* [seqs] */
+    const uint32_t* starts;         /* [seqs + 1] */
+    uint32_t seqs;
+} lv_paged_cache;
+
+/* Where row `position` of head `head` of a sequence begins in k and v, in values (in k_scale and v_scale: / dim), for a host that has a
+ * copy of the sequence's table row: pages that are moved, saved or shared.  The kernels place rows by the same rule. */
+int lv_paged_locate(const lv_paged_cache* cache, const uint32_t* table_row, uint32_t position, uint32_t head, uint64_t* value_index);
+
+/* Keys and values of the new tokens (k, v: [tokens][ld] of in_type f32, f16 or bf16, kv_heads * dim values a row, rows 16-byte aligned) to their
+ * places.  Keys are rotated on the way: the pair (2 i, 2 i + 1) of every head turns by angles[t * angle_ld + 2 i] = {cos, sin} for
+ * i < angle_pairs, t the token's row (lv_rotary_table makes such rows); products and sums of the rotation are rounded to f32 one by one.  angles null:
+ * none.  tokens: rows of k and v. */
+int lv_paged_append(lv_ctx* ctx, const lv_paged_cache* cache, const void* k, const void* v, int in_type, uint32_t ld, const float* angles, uint32_t angle_ld,
+                    uint32_t angle_pairs, uint32_t tokens);
+
+/* Positions first .. first + rows - 1 of every sequence back as f32, f16 or bf16 values: head h of position first + i of sequence s to
+ * k_out[s * seq_stride + h * head_stride + i * row_stride] (values; multiples of 16 bytes), the same for v.  What lies behind a sequence's length stays as it is.
+ * A code times its scale is rounded to f32, then to out_type. */
+int lv_paged_read(lv_ctx* ctx, const lv_paged_cache* cache, void* k_out, void* v_out, int out_type, size_t seq_stride, size_t head_stride, size_t row_stride,
+                  uint32_t first, uint32_t rows);
+
+/* Attention of the new tokens over their sequences' pages (appended before): query head h of a token at position i looks at the key/value head
+ * h / (heads / kv_heads) of the positions max(0, i + 1 - window) <= j <= i (window 0: from 0 on),
+ *   s_j = scale * (q . k_j),   out = sum_j e^(s_j) v_j / (e^(sink_h) + sum_j e^(s_j)).
+ * A row that sees nothing gets zeros.  q [tokens][q_ld] and out [tokens][out_ld]: heads * dim values a row, rows 16-byte aligned; q is rotated like the
+ * keys of lv_paged_append.  max_new and max_len: upper bounds of the new tokens and of the length of a sequence; they size the launch.
+ * Sums, maxima and the softmax are f32.  Output in 16 bits: queries and probabilities enter the matrix products in 16 bits (bf16 for a bf16 cache, else f16).
+ * Output in f32: as the sums of two 16-bit numbers each.  Places that no new token sees are not looked at, whatever they hold; a value that is not finite reaches the
+ * tokens that see it, and may reach others of the same sequence and step.
+ * scratch: 16-byte aligned, lv_paged_attention_scratch_bytes; calls that run at the same time need their own. */
+typedef struct lv_paged_attention_args {
+    lv_paged_cache cache;
+    const void* q;
+    int q_type;                     /* f32, f16 or bf16 */
+    uint32_t q_ld, heads, tokens, max_new, max_len;
+    float scale;
+    uint32_t window;
+    const float* sink;              /* [heads]; null: none */
+    const float* angles;
+    uint32_t angle_ld, angle_pairs;
+    void* out;
+    int out_type;                   /* f32, f16 or bf16 */
+    uint32_t out_ld;
+} lv_paged_attention_args;
+/* 0 for arguments that lv_paged_attention refuses */
+size_t lv_paged_attention_scratch_bytes(lv_ctx* ctx, const lv_paged_attention_args* a);
+int lv_paged_attention(lv_ctx* ctx, const lv_paged_attention_args* a, void* scratch, size_t scratch_bytes);
+
+/* out[r] = softmax(logits[r] / temperature[r]) over vocab values, f32 [rows][out_ld] and [rows][ld]; temperature f32 [rows] (device), null: 1
+ * everywhere.  Temperature 0: one at the first index of the maximum, zero elsewhere (NaN never is the maximum; a row of nothing else: index 0).  A row of
+ * nothing but -infinity gets zeros at any other temperature.
+ * out may be logits (with the same stride). */
+int lv_probabilities(lv_ctx* ctx, float* out, uint32_t out_ld, const float* logits, uint32_t ld, uint32_t vocab, uint32_t rows, const float* temperature);
+
+/* Drafted tokens against the target's probabilities, from given random numbers (speculative sampling: what comes out is distributed as if drawn from the
+ * target alone).  The rows of sequence s are starts[s] .. starts[s + 1] - 1 as above: target[r] f32 [vocab] holds the target's probabilities behind
+ * row r, and drafted[r] the token that the draft model chose there, with its probabilities draft[r] -- in every row but the sequence's last, which
+ * has no draft behind it.  draft null: the drafts were certain (probability 1).
+ *   draft i of s is accepted while all before it were and accept[r] * draft[r][d] < target[r][d],  r = starts[s] + i, d = drafted[r]
+ *   then one token is drawn from row starts[s] + (number accepted): from max(target - draft, 0) behind a rejected draft (from target where that leaves
+ *   nothing), from target behind the last one: the first index whose cumulative weight is above pick[s] * the whole weight
+ * accepted[s]: number of drafts accepted; tokens[starts[s] ..]: the accepted drafts, the drawn token, then 0xFFFFFFFF.  A sequence without rows accepts 0 and draws nothing;
+ * a draft >= vocab is reported through the error word and rejected, a row without weight reported, its token 0xFFFFFFFF.
+ * lens (may be null): lens[s] -= number of rejected drafts, whose rows in a paged cache are overwritten by the next step.
+ * accept, pick: in [0, 1).  Weights are summed in f64. */
+typedef struct lv_verify_args {
+    const float* target;
+    uint32_t target_ld;
+    const float* draft;
+    uint32_t draft_ld, vocab;
+    const uint32_t* drafted;        /* [rows] */
+    const uint32_t* starts;         /* [seqs + 1] */
+    uint32_t seqs, rows;            /* rows: of target, drafted, accept and tokens */
+    const float* accept;            /* [rows] */
+    const float* pick;              /* [seqs] */
+    uint32_t* tokens;               /* [rows] */
+    uint32_t* accepted;             /* [seqs] */
+    uint32_t* lens;
+} lv_verify_args;
+int lv_verify_drafts(lv_ctx* ctx, const lv_verify_args* a);
 
 /* ---- multi-GPU: one process per GPU, one communicator per context.  The
  *      reference is single-device (llava_context.cpp:264-279 takes one queue of

@@ -26,6 +26,7 @@ LV_ERR_COMM = 103
 TYPE_F32, TYPE_F16, TYPE_Q4_0, TYPE_Q8_0 = 0, 1, 2, 8
 TYPE_Q4_0_V1 = 258
 TYPE_I32, TYPE_BF16 = 26, 30
+TYPE_I8, TYPE_E4M3 = 24, 259
 
 _p = C.c_void_p
 _u32 = C.c_uint32
@@ -71,6 +72,25 @@ class SsmArgs(C.Structure):
                 ("out_type", _int), ("out_ld", _u32), ("form", _int)]
 
 
+class PagedCache(C.Structure):
+    """lv_paged_cache"""
+    _fields_ = [("k", _p), ("v", _p), ("k_scale", _p), ("v_scale", _p), ("type", _int), ("pages", _u32), ("page_rows", _u32), ("kv_heads", _u32), ("dim", _u32),
+                ("table", _p), ("table_ld", _u32), ("lens", _p), ("starts", _p), ("seqs", _u32)]
+
+
+class PagedAttentionArgs(C.Structure):
+    """lv_paged_attention_args"""
+    _fields_ = [("cache", PagedCache), ("q", _p), ("q_type", _int), ("q_ld", _u32), ("heads", _u32), ("tokens", _u32), ("max_new", _u32), ("max_len", _u32),
+                ("scale", _f32), ("window", _u32), ("sink", _p), ("angles", _p), ("angle_ld", _u32), ("angle_pairs", _u32), ("out", _p), ("out_type", _int),
+                ("out_ld", _u32)]
+
+
+class VerifyArgs(C.Structure):
+    """lv_verify_args"""
+    _fields_ = [("target", _p), ("target_ld", _u32), ("draft", _p), ("draft_ld", _u32), ("vocab", _u32), ("drafted", _p), ("starts", _p), ("seqs", _u32),
+                ("rows", _u32), ("accept", _p), ("pick", _p), ("tokens", _p), ("accepted", _p), ("lens", _p)]
+
+
 # name -> (restype, argtypes); mirrors include/lv_b200.h
 KERNEL_API = {
     "lv_device_count": (_int, [C.POINTER(_int)]),
@@ -112,6 +132,13 @@ KERNEL_API = {
     "lv_tp_arm_pull": (_int, [_p, _int, _u32, _u32, _p]),
     "lv_argmax_advance": (_int, [_p, _p, _u32, _p, _p, _u32, _u32, _p, _p]),
     "lv_norm_qkv_kvappend": (_int, [_p, _p, _p, _p, _p, _p, _p, _int, _p, _p, _p, _u32, _u32, _u32, _u32]),
+    "lv_paged_locate": (_int, [_p, _p, _u32, _u32, _p]),
+    "lv_paged_append": (_int, [_p, _p, _p, _p, _int, _u32, _p, _u32, _u32, _u32]),
+    "lv_paged_read": (_int, [_p, _p, _p, _p, _int, _sz, _sz, _sz, _u32, _u32]),
+    "lv_paged_attention_scratch_bytes": (_sz, [_p, _p]),
+    "lv_paged_attention": (_int, [_p, _p, _p, _sz]),
+    "lv_probabilities": (_int, [_p, _p, _u32, _p, _u32, _u32, _u32, _p]),
+    "lv_verify_drafts": (_int, [_p, _p]),
     "lv_comm_unique_id": (_int, [_p]),
     "lv_comm_init_rank": (_int, [_p, _p, _int, _int]),
     "lv_allreduce_f32": (_int, [_p, _p, _sz]),

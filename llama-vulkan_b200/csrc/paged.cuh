@@ -1,0 +1,130 @@
+// What the kernels of a paged cache share: where a row lies, which sequence a token belongs to, and the types that values come in.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <math.h>
+
+#include "../../include/lv_b200.h"
+#include "common.cuh"
+#include "ctx.h"
+
+namespace lv {
+
+constexpr float kPagedTiny = 0x1p-100f;          // rows whose largest magnitude is below are stored as zeros
+
+// Row (of k or v, and of the scales) of a head's position; false: the table names no page of the cache.  64 bits: a cache has more than 2^32 values.
+__host__ __device__ __forceinline__ bool paged_row(const lv_paged_cache& c, const uint32_t* table_row, uint32_t position, uint32_t head, uint64_t* row) {
+    const uint32_t slot = position / c.page_rows, page = slot < c.table_ld ? table_row[slot] : c.pages;
+    *row = (uint64_t(page) * c.kv_heads + head) * c.page_rows + (position - slot * c.page_rows);
+    return page < c.pages;
+}
+
+// New rows and length of a sequence; false: they contradict each other, the step's rows or the table.
+struct PagedSeq {
+    uint32_t row0, n, len;
+};
+__device__ __forceinline__ bool paged_seq(const lv_paged_cache& c, uint32_t s, uint32_t tokens, PagedSeq* out) {
+    const uint32_t a = c.starts[s], b = c.starts[s + 1], len = c.lens[s];
+    out->row0 = a;
+    out->n = b - a;
+    out->len = len;
+    return a <= b && b <= tokens && b - a <= len && len <= uint64_t(c.table_ld) * c.page_rows;
+}
+
+// The sequence of row t: the last s with starts[s] <= t (seqs: t belongs to nobody).  Ends for any contents of starts.
+__device__ __forceinline__ uint32_t paged_owner(const lv_paged_cache& c, uint32_t t) {
+    if (t < c.starts[0]) return c.seqs;
+    uint32_t lo = 0, hi = c.seqs;                // starts[lo] <= t < starts[hi], were starts[seqs + 1] infinite
+    if (t >= c.starts[hi]) return c.seqs;
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) / 2;
+        if (c.starts[mid] <= t) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+__host__ __device__ __forceinline__ bool paged_is8(int type) { return type == LV_TYPE_I8 || type == LV_TYPE_E4M3; }
+__host__ __device__ __forceinline__ uint32_t paged_bytes(int type) { return type == LV_TYPE_F32 ? 4u : paged_is8(type) ? 1u : 2u; }
+inline bool paged_value_type(int type) { return type == LV_TYPE_F32 || type == LV_TYPE_F16 || type == LV_TYPE_BF16; }
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// Four consecutive values of type f32, f16 or bf16 (the type is the same for a whole launch)
+__device__ __forceinline__ float4 load_values4(const void* p, size_t at, int type) {
+    if (type == LV_TYPE_F32) return *reinterpret_cast<const float4*>(static_cast<const float*>(p) + at);
+    const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + at);
+    float2 a, b;
+    if (type == LV_TYPE_BF16) {
+        a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.x));
+        b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.y));
+    } else {
+        a = __half22float2(*reinterpret_cast<const __half2*>(&u.x));
+        b = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
+    }
+    return make_float4(a.x, a.y, b.x, b.y);
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint2 pack_values4(const float4& v, int type) {
+    return type == LV_TYPE_BF16 ? make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w)) : make_uint2(pack_f16(v.x, v.y), pack_f16(v.z, v.w));
+}
+__device__ __forceinline__ void store_values4(void* p, size_t at, int type, const float4& v) {
+    if (type == LV_TYPE_F32) *reinterpret_cast<float4*>(static_cast<float*>(p) + at) = v;
+    else *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p) + at) = pack_values4(v, type);
+}
+
+// Four values of a cache row; 8-bit codes come as whole numbers or e4m3 values, without their scale
+__device__ __forceinline__ float4 load_cached4(const void* p, size_t at, int type) {
+    if (!paged_is8(type)) return load_values4(p, at, type);
+    const uint32_t u = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(p) + at);
+    if (type == LV_TYPE_I8)
+        return make_float4(float(int8_t(u & 0xffu)), float(int8_t((u >> 8) & 0xffu)), float(int8_t((u >> 16) & 0xffu)), float(int8_t(u >> 24)));
+    const float2 a = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(u & 0xffffu), __NV_E4M3)));
+    const float2 b = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(u >> 16), __NV_E4M3)));
+    return make_float4(a.x, a.y, b.x, b.y);
+}
+
+// Values c .. c + 3 of a head's vector turned by a token's angles: the pairs (2 i, 2 i + 1), every product and sum rounded by itself, so that the
+// codes that a rotated key is stored as are the same wherever it is rotated
+__device__ __forceinline__ float4 rotate4(float4 v, const float* angles, uint32_t c, uint32_t pairs) {
+    if (c < 2 * pairs) {
+        const float2 t = *reinterpret_cast<const float2*>(angles + c);
+        const float x = v.x;
+        v.x = __fsub_rn(__fmul_rn(x, t.x), __fmul_rn(v.y, t.y));
+        v.y = __fadd_rn(__fmul_rn(v.y, t.x), __fmul_rn(x, t.y));
+    }
+    if (c + 2 < 2 * pairs) {
+        const float2 t = *reinterpret_cast<const float2*>(angles + c + 2);
+        const float z = v.z;
+        v.z = __fsub_rn(__fmul_rn(z, t.x), __fmul_rn(v.w, t.y));
+        v.w = __fadd_rn(__fmul_rn(v.w, t.x), __fmul_rn(z, t.y));
+    }
+    return v;
+}
+
+// What is wrong with a cache's description (LV_OK: nothing)
+inline int paged_check(const lv_paged_cache* c) {
+    LV_REQUIRE(c && c->k && c->v && c->table && c->lens && c->starts, "paged cache: null argument");
+    LV_REQUIRE(c->type == LV_TYPE_F16 || c->type == LV_TYPE_BF16 || paged_is8(c->type), "paged cache: unsupported type");
+    LV_REQUIRE(!paged_is8(c->type) || (c->k_scale && c->v_scale), "paged cache: 8-bit values need scales");
+    LV_REQUIRE(c->dim && c->dim % 16 == 0 && c->dim <= 256, "paged cache: head size");
+    LV_REQUIRE(c->pages && c->page_rows && c->kv_heads && c->kv_heads <= 65535 && c->table_ld && c->seqs && c->seqs <= 65535, "paged cache: bad sizes");
+    LV_REQUIRE(uint64_t(c->table_ld) * c->page_rows <= 0x7fffffffull && c->pages < 0xffffffffu, "paged cache: positions of a sequence are below 2^31");
+    LV_REQUIRE(aligned16(c->k) && aligned16(c->v), "paged cache: k and v are 16-byte aligned");
+    return LV_OK;
+}
+inline int paged_check_rotation(const float* angles, uint32_t angle_ld, uint32_t angle_pairs, uint32_t dim) {
+    LV_REQUIRE(!angles || (angle_pairs <= dim / 2 && angle_ld >= 2 * angle_pairs && angle_ld % 2 == 0 && (reinterpret_cast<uintptr_t>(angles) & 7u) == 0), "paged cache: bad angles");
+    return LV_OK;
+}
+
+}  // namespace lv
