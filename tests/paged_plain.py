@@ -147,7 +147,9 @@ def attend(cache, starts, q, heads, scale, window=0, sink=None, angles=None, out
     bound: how far a result may be off.  With u the relative error of an operand of the products (queries, probabilities), a score is off by at most
     d = (u + (dim + 3) 2^-24 + 4 2^-24) scale sum |q| |k| (the rounding of q, f32 sums in any order, the factors), a weight by 2 d + 2 u relative to
     itself, its own and the normaliser's (plus 2^-22 |s| + 2^-20 for the exponentials), the sums over n keys by (log2-like chains of at most n) 2^-24 each; all
-    together times sum p |v|, and the rounding of the output."""
+    together times sum p |v|, and the rounding of the output.  Weights in f16 (all caches but bf16) are whole multiples of 2^-24, while the largest of a row
+    is at least 2^10: each is off by up to 2^-25, which is 2^-35 of the largest one and so of the normaliser; with |v| <= max |v| that is n 2^-35 max |v|
+    at most over n keys (a value that the visible keys of large weight do not have at all is left to weights that small)."""
     u16 = HALF_STEP[BF16 if cache.kind == BF16 else F16]
     u = 2.0 * u16 * u16 if out_kind == F32 else u16
     tokens, dim, G = q.shape[0], cache.dim, heads // cache.H
@@ -171,7 +173,8 @@ def attend(cache, starts, q, heads, scale, window=0, sink=None, angles=None, out
                 out[t, h] = w @ vv / total
                 size = scale * (np.abs(kk) @ np.abs(x[t, h]))
                 d = (u + (dim + 7) * 2.0 ** -24) * size.max()
-                bound[t, h] = (np.expm1(2 * d) + 2 * u + 2.0 ** -19 + 2.0 ** -22 * size.max() + len(z) * 2.0 ** -24) * (w @ np.abs(vv) / total)
+                floor = 0.0 if cache.kind == BF16 else len(z) * 2.0 ** -35 * np.abs(vv).max()
+                bound[t, h] = floor + (np.expm1(2 * d) + 2 * u + 2.0 ** -19 + 2.0 ** -22 * size.max() + len(z) * 2.0 ** -24) * (w @ np.abs(vv) / total)
     bound += HALF_STEP[out_kind] * (np.abs(out) + bound) + 1e-30 + (2.0 ** -25 if out_kind == F16 else 0)
     return out, bound
 
