@@ -691,7 +691,7 @@ int lv_paged_read(lv_ctx* ctx, const lv_paged_cache* cache, void* k_out, void* v
 
 /* Attention of the new tokens over their sequences' pages (appended before): query head h of a token at position i looks at the key/value head
  * h / (heads / kv_heads) of the positions max(0, i + 1 - window) <= j <= i (window 0: from 0 on),
- *   s_j = scale * (q . k_j),   out = sum_j e^(s_j) v_j / (e^(sink_h) + sum_j e^(s_j)).
+ *   s_j = scale * (q . k_j) (scale > 0),   out = sum_j e^(s_j) v_j / (e^(sink_h) + sum_j e^(s_j)).
  * A row that sees nothing gets zeros.  q [tokens][q_ld] and out [tokens][out_ld]: heads * dim values a row, rows 16-byte aligned; q is rotated like the
  * keys of lv_paged_append.  max_new and max_len: upper bounds of the new tokens and of the length of a sequence; they size the launch.
  * Sums, maxima and the softmax are f32.  Output in 16 bits: queries and probabilities enter the matrix products in 16 bits (bf16 for a bf16 cache, else f16).

@@ -35,10 +35,6 @@ __device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uin
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-template <bool BF16>
-__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
-    return BF16 ? pack_bf16(lo, hi) : pack_f16(lo, hi);
-}
 // what the rounding to 16 bits has left of two values, rounded in its turn
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack16_rest(float lo, float hi, uint32_t rounded) {
@@ -46,33 +42,6 @@ __device__ __forceinline__ uint32_t pack16_rest(float lo, float hi, uint32_t rou
     if constexpr (BF16) r = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&rounded));
     else r = __half22float2(*reinterpret_cast<const __half2*>(&rounded));
     return pack16<BF16>(lo - r.x, hi - r.y);
-}
-
-// Two codes (the low or the high half of a word) as f16
-template <int KIND>
-__device__ __forceinline__ uint32_t codes_f16(uint32_t w, bool high) {
-    if constexpr (KIND == LV_TYPE_I8) {
-        // 0x64xx is 1024 + xx in f16; the codes' sign bits are flipped before (128 + code)
-        const uint32_t u = __byte_perm(w, 0x64646464u, high ? 0x4342u : 0x4140u);
-        const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&u), __floats2half2_rn(1152.f, 1152.f));
-        return *reinterpret_cast<const uint32_t*>(&v);
-    } else {
-        uint32_t v;
-        asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(v) : "r"(high ? w >> 16 : w));
-        return v;
-    }
-}
-
-__device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, bool there) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16u : 0u) : "memory");
-}
-__device__ __forceinline__ void cp_async4_zfill(uint32_t dst, const void* src, bool there) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(there ? 4u : 0u) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 // KIND: type of the cache; D: head size rounded up to 64, 128 or 256; EXACT: two 16-bit numbers per query value and weight; MT: blocks of 16 rows
@@ -184,8 +153,7 @@ __global__ void __launch_bounds__(32 * kPrWarps) paged_rows_kernel(const PagedAt
         float f = 1.f;                                                   // 2^-e of the largest value (f16 operands)
         if constexpr (!S::kBf16) {
             top = warp_max(top);
-            const uint32_t e = min(max(__float_as_uint(top) >> 23, 1u), 253u);
-            f = __uint_as_float((254u - e) << 23);
+            f = paged_row_unit(top);
         }
         if (lane == 0) s_factor[r] = a.scale * kPaLog2e / f;
 #pragma unroll
@@ -330,10 +298,10 @@ __global__ void __launch_bounds__(32 * kPrWarps) paged_rows_kernel(const PagedAt
         float keep[MT][2];
         bool moved = false;
         if constexpr (S::kEight) {
-            const uint32_t mine = (__float_as_uint(reinterpret_cast<const float*>(here + 2 * S::kHalf)[S::kKeys + lane]) >> 23) & 255u;
-            const uint32_t top = min(max(__reduce_max_sync(0xffffffffu, mine == 255u ? 0u : mine), 1u), 253u);     // (a NaN scale is its key's own matter)
+            const uint32_t mine = paged_scale_exponent(reinterpret_cast<const float*>(here + 2 * S::kHalf)[S::kKeys + lane]);
+            const uint32_t top = min(max(__reduce_max_sync(0xffffffffu, mine), 1u), 253u);
             if (top > unit) {                                            // (unit 0: nothing yet, all outputs are zero)
-                const float f = unit == 0 ? 1.f : __uint_as_float((127u - min(top - unit, 126u)) << 23);
+                const float f = paged_unit_step(unit, top);
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) keep[mt][0] = keep[mt][1] = f;
                 unit = top;
@@ -583,18 +551,21 @@ struct PagedPlan {
     uint32_t rows, blocks;       // rows of a block, blocks of the longest chunk of new tokens
     uint32_t chunk, splits;
     size_t bytes;
+    bool many;
 };
 
 static PagedPlan paged_plan(const lv_ctx* ctx, const lv_paged_attention_args& a) {
     PagedPlan plan{};
     const uint32_t group = a.heads / a.cache.kv_heads, rows = a.max_new * group;
-    plan.rows = rows <= 16 || a.cache.dim > 128 ? 16 : 32;
+    // 16-bit outputs of more than 32 rows that share their keys: a tile of the tensor cores
+    plan.many = a.out_type != LV_TYPE_F32 && a.cache.dim <= 128 && rows > 32;
+    plan.rows = plan.many ? kPtRows : rows <= 16 || a.cache.dim > 128 ? 16 : 32;
     plan.blocks = (rows + plan.rows - 1) / plan.rows;
     const uint64_t seen = a.window ? std::min<uint64_t>(a.max_len, uint64_t(a.window) + std::min(a.max_new, plan.rows)) : a.max_len;
-    const uint32_t unit = kPrWarps * (paged_is8(a.cache.type) ? 32 : 16);
+    const uint32_t unit = plan.many ? kPtKeys : kPrWarps * (paged_is8(a.cache.type) ? 32 : 16);
     const uint64_t ctas = uint64_t(a.cache.seqs) * a.cache.kv_heads * plan.blocks;
     // CTAs for two per SM; with fewer than eight rounds of them the long sequences would end alone
-    const uint64_t want = 2ull * ctx->sm_count * (ctas > uint64_t(ctx->sm_count) ? 8 : 1);
+    const uint64_t want = plan.many ? uint64_t(ctx->sm_count) * (ctas > uint64_t(ctx->sm_count) ? 6 : 1) : 2ull * ctx->sm_count * (ctas > uint64_t(ctx->sm_count) ? 8 : 1);
     uint64_t splits = std::max<uint64_t>(1, std::min<uint64_t>((want + ctas - 1) / ctas, (seen + unit - 1) / unit));
     uint64_t chunk = ((seen + splits - 1) / splits + unit - 1) / unit * unit;
     plan.chunk = uint32_t(std::max<uint64_t>(chunk, unit));
@@ -636,7 +607,7 @@ static int paged_attention_check(const lv_paged_attention_args* a) {
                "paged attention: rows of q and out are 16-byte aligned");
     LV_REQUIRE(a->max_new <= a->tokens && a->max_new <= a->max_len && a->max_len <= uint64_t(a->cache.table_ld) * a->cache.page_rows, "paged attention: bad upper bounds");
     LV_REQUIRE(uint64_t(a->tokens) * a->heads < (uint64_t(1) << 31), "paged attention: too many tokens");
-    LV_REQUIRE(isfinite(a->scale), "paged attention: scale");
+    LV_REQUIRE(a->scale > 0.f && isfinite(a->scale), "paged attention: scale");
     return paged_check_rotation(a->angles, a->angle_ld, a->angle_pairs, a->cache.dim);
 }
 
@@ -665,7 +636,8 @@ extern "C" int lv_paged_attention(lv_ctx* ctx, const lv_paged_attention_args* a,
     p.part_o = static_cast<float*>(scratch) + (size_t(a->tokens) * a->heads * plan.splits * 2 + 3) / 4 * 4;
     p.err = ctx->d_err;
     int rc = LV_OK;
-    switch (a->cache.type) {
+    if (plan.many) rc = paged_tc_launch(ctx, p, plan.blocks);
+    else switch (a->cache.type) {
         case LV_TYPE_BF16: rc = rows_launch_kind<LV_TYPE_BF16>(ctx, p, plan); break;
         case LV_TYPE_F16: rc = rows_launch_kind<LV_TYPE_F16>(ctx, p, plan); break;
         case LV_TYPE_I8: rc = rows_launch_kind<LV_TYPE_I8>(ctx, p, plan); break;

@@ -12,6 +12,8 @@ constexpr float kPaLift = 10.f;
 // A new maximum becomes the reference when it is above the old one by more than this (log2): then weights stay below 2^(kPaLift + kPaStep + 1) < 65504
 constexpr float kPaStep = 4.f;
 
+constexpr int kPtRows = 256, kPtKeys = 128;      // rows of a block and keys of a step of the kernel for many rows
+
 struct PagedAttn {
     lv_paged_attention_args a;
     uint32_t group;              // query heads of a key/value head
@@ -47,5 +49,48 @@ __device__ __forceinline__ float exp2_fast(float x) {
 // the weight of a head's sink, and the least reference that it fits under
 __device__ __forceinline__ float paged_sink(const PagedAttn& p, uint32_t head) { return p.a.sink ? p.a.sink[head] * kPaLog2e : -INFINITY; }
 __device__ __forceinline__ float paged_sink_weight(float sink, float ref) { return sink == -INFINITY ? 0.f : exp2_fast(sink - ref); }
+
+// paged_attention_tc.cu: blocks of kPtRows rows, 16-bit outputs, heads of up to 128 values
+int paged_tc_launch(lv_ctx* ctx, const PagedAttn& p, uint32_t blocks);
+
+// Value pairs as 16-bit operands, and two codes (the low or the high half of a word) as f16
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+    return BF16 ? pack_bf16(lo, hi) : pack_f16(lo, hi);
+}
+template <int KIND>
+__device__ __forceinline__ uint32_t codes_f16(uint32_t w, bool high) {
+    if constexpr (KIND == LV_TYPE_I8) {
+        // 0x64xx is 1024 + xx in f16; the codes' sign bits are flipped before (128 + code)
+        const uint32_t u = __byte_perm(w, 0x64646464u, high ? 0x4342u : 0x4140u);
+        const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&u), __floats2half2_rn(1152.f, 1152.f));
+        return *reinterpret_cast<const uint32_t*>(&v);
+    } else {
+        uint32_t v;
+        asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(v) : "r"(high ? w >> 16 : w));
+        return v;
+    }
+}
+
+__device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16u : 0u) : "memory");
+}
+__device__ __forceinline__ void cp_async4_zfill(uint32_t dst, const void* src, bool there) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(there ? 4u : 0u) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// 2^-e of a row's largest magnitude (f16 queries are divided by 2^e; rows below 2^-63 have no scores to speak of), and the exponent field of a value's scale (0 for one that is not finite)
+__device__ __forceinline__ float paged_row_unit(float top) { return __uint_as_float((254u - min(max(__float_as_uint(top) >> 23, 64u), 253u)) << 23); }
+__device__ __forceinline__ uint32_t paged_scale_exponent(float scale) {
+    const uint32_t e = (__float_as_uint(scale) >> 23) & 255u;
+    return e == 255u ? 0u : e;
+}
+// what outputs in units of 2^(from - 127) are multiplied by when the unit becomes 2^(to - 127); from 0: there are none yet
+__device__ __forceinline__ float paged_unit_step(uint32_t from, uint32_t to) { return from == 0 ? 1.f : __uint_as_float((127u - min(to - from, 126u)) << 23); }
 
 }  // namespace lv

@@ -72,11 +72,11 @@ def test_reads_that_cannot_be(args, text):
 
 BAD_ATTENTION = [(dict(q=None), "null"), (dict(out=None), "null"), (dict(heads=0), "heads"), (dict(heads=6), "heads"), (dict(q_type=pkg.TYPE_I8), "type"), (dict(out_type=pkg.TYPE_E4M3), "type"),
                  (dict(q_ld=511), "strides"), (dict(out_ld=508), "strides"), (dict(q_ld=514), "16-byte"), (dict(out_ld=516), "16-byte"), (dict(q=P + 4), "16-byte"), (dict(out=P + 2), "16-byte"),
-                 (dict(max_new=7), "bounds"), (dict(max_len=2), "bounds"), (dict(max_len=81), "bounds"), (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"),
+                 (dict(max_new=7), "bounds"), (dict(max_len=2), "bounds"), (dict(max_len=81), "bounds"), (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"), (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"),
                  (dict(tokens=(1 << 31) - 1), "too many"), (dict(angles=P, angle_ld=64, angle_pairs=33), "angles")]
 
 
-@pytest.mark.parametrize("more,text", BAD_ATTENTION, ids=[f"{list(m)[0]}-{t}" for m, t in BAD_ATTENTION])
+@pytest.mark.parametrize("more,text", BAD_ATTENTION, ids=[f"{i}-{t}" for i, (m, t) in enumerate(BAD_ATTENTION)])
 def test_attentions_that_cannot_be(more, text):
     lib, a = pkg.load_kernels(), attention(**more)
     refused(lib.lv_paged_attention(None, C.byref(a), P, 1 << 30), text)
