@@ -52,9 +52,7 @@ inline bool paged_value_type(int type) { return type == LV_TYPE_F32 || type == L
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // Four consecutive values of type f32, f16 or bf16 (the type is the same for a whole launch)
-__device__ __forceinline__ float4 load_values4(const void* p, size_t at, int type) {
-    if (type == LV_TYPE_F32) return *reinterpret_cast<const float4*>(static_cast<const float*>(p) + at);
-    const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + at);
+__device__ __forceinline__ float4 unpack_values4(uint2 u, int type) {
     float2 a, b;
     if (type == LV_TYPE_BF16) {
         a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.x));
@@ -64,6 +62,10 @@ __device__ __forceinline__ float4 load_values4(const void* p, size_t at, int typ
         b = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
     }
     return make_float4(a.x, a.y, b.x, b.y);
+}
+__device__ __forceinline__ float4 load_values4(const void* p, size_t at, int type) {
+    if (type == LV_TYPE_F32) return *reinterpret_cast<const float4*>(static_cast<const float*>(p) + at);
+    return unpack_values4(*reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + at), type);
 }
 
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
@@ -82,15 +84,18 @@ __device__ __forceinline__ void store_values4(void* p, size_t at, int type, cons
     else *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p) + at) = pack_values4(v, type);
 }
 
-// Four values of a cache row; 8-bit codes come as whole numbers or e4m3 values, without their scale
-__device__ __forceinline__ float4 load_cached4(const void* p, size_t at, int type) {
-    if (!paged_is8(type)) return load_values4(p, at, type);
-    const uint32_t u = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(p) + at);
+// Values of a cache row; 8-bit codes come as whole numbers or e4m3 values, without their scale
+__device__ __forceinline__ float4 code_values4(uint32_t u, int type) {
     if (type == LV_TYPE_I8)
         return make_float4(float(int8_t(u & 0xffu)), float(int8_t((u >> 8) & 0xffu)), float(int8_t((u >> 16) & 0xffu)), float(int8_t(u >> 24)));
     const float2 a = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(u & 0xffffu), __NV_E4M3)));
     const float2 b = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(u >> 16), __NV_E4M3)));
     return make_float4(a.x, a.y, b.x, b.y);
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 
 // Values c .. c + 3 of a head's vector turned by a token's angles: the pairs (2 i, 2 i + 1), every product and sum rounded by itself, so that the

@@ -40,12 +40,6 @@ __device__ __forceinline__ bool paged_attention_seq(const PagedAttn& p, uint32_t
     return false;
 }
 
-__device__ __forceinline__ float exp2_fast(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 // the weight of a head's sink, and the least reference that it fits under
 __device__ __forceinline__ float paged_sink(const PagedAttn& p, uint32_t head) { return p.a.sink ? p.a.sink[head] * kPaLog2e : -INFINITY; }
 __device__ __forceinline__ float paged_sink_weight(float sink, float ref) { return sink == -INFINITY ? 0.f : exp2_fast(sink - ref); }

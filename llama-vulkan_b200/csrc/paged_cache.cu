@@ -17,74 +17,95 @@ struct PagedAppend {
     uint32_t* err;
 };
 
-// A warp per row (token, head, key or value).  The values are asked for before the places are looked up, which is a chain of four dependent loads.
+// A warp takes the keys or the values of four (L = 16: eight) heads of a token: L lanes a head, four values a lane and part.  All values are asked for before the
+// places are looked up, which is a chain of four dependent loads, once for the heads of a warp.
+// FIGURES_APPEND
+constexpr int kAppendRows = 4;
+template <int L, int PARTS>
 __global__ void __launch_bounds__(256) paged_append_kernel(const PagedAppend p) {
     pdl_launch_dependents();
     pdl_wait();
     const lv_paged_cache& c = p.c;
-    const uint32_t lane = threadIdx.x & 31u, H = c.kv_heads;
+    constexpr uint32_t kHeads = kAppendRows * (32 / L);
+    const uint32_t lane = threadIdx.x & 31u, H = c.kv_heads, groups = (H + kHeads - 1) / kHeads;
     const uint64_t job = uint64_t(blockIdx.x) * (blockDim.x / 32) + threadIdx.x / 32;
-    if (job >= uint64_t(p.tokens) * H * 2) return;
-    const uint32_t t = uint32_t(job / (2 * H)), which = uint32_t(job - uint64_t(t) * 2 * H) / H, h = uint32_t(job - uint64_t(t) * 2 * H) - which * H;
-    constexpr int kParts = 2;                    // of 128 values
-    float4 v[kParts];
+    const uint32_t t = uint32_t(job / (2 * groups)), in_t = uint32_t(job - uint64_t(t) * 2 * groups), which = in_t / groups, h0 = (in_t - which * groups) * kHeads + lane / L;
+    if (t >= p.tokens) return;
+    const uint32_t at0 = 4 * (lane % L);
+    float4 v[kAppendRows][PARTS];
 #pragma unroll
-    for (int i = 0; i < kParts; ++i) {
-        const uint32_t at = 4 * (lane + 32 * i);
-        v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (at < c.dim) v[i] = load_values4(p.in[which], size_t(t) * p.ld + h * c.dim + at, p.in_type);
-    }
-    if (which == 0 && p.angles != nullptr) {
+    for (int k = 0; k < kAppendRows; ++k)
 #pragma unroll
-        for (int i = 0; i < kParts; ++i) {
-            const uint32_t at = 4 * (lane + 32 * i);
-            if (at < c.dim) v[i] = rotate4(v[i], p.angles + size_t(t) * p.angle_ld, at, p.angle_pairs);
+        for (int i = 0; i < PARTS; ++i) {
+            const uint32_t at = at0 + 4 * L * i, h = h0 + k * (32 / L);
+            v[k][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (at < c.dim && h < H) v[k][i] = load_values4(p.in[which], size_t(t) * p.ld + size_t(h) * c.dim + at, p.in_type);
         }
-    }
     const uint32_t s = paged_owner(c, t);
     PagedSeq q;
     if (s == c.seqs) return;
-    uint64_t row;
-    if (!paged_seq(c, s, p.tokens, &q) || !paged_row(c, c.table + size_t(s) * c.table_ld, q.len - q.n + (t - q.row0), h, &row)) {
+    uint64_t row0;                                                       // of head 0
+    if (!paged_seq(c, s, p.tokens, &q) || !paged_row(c, c.table + size_t(s) * c.table_ld, q.len - q.n + (t - q.row0), 0, &row0)) {
         if (lane == 0) atomicOr(p.err, ERR_BAD_INDEX);
         return;
     }
+    if (which == 0 && p.angles != nullptr) {
+#pragma unroll
+        for (int i = 0; i < PARTS; ++i) {
+            const uint32_t at = at0 + 4 * L * i;
+            if (at >= c.dim) continue;
+#pragma unroll
+            for (int k = 0; k < kAppendRows; ++k) v[k][i] = rotate4(v[k][i], p.angles + size_t(t) * p.angle_ld, at, p.angle_pairs);
+        }
+    }
     void* out = which ? c.v : c.k;
-    if (!paged_is8(c.type)) {
-#pragma unroll
-        for (int i = 0; i < kParts; ++i) {
-            const uint32_t at = 4 * (lane + 32 * i);
-            if (at < c.dim) store_values4(out, row * c.dim + at, c.type, v[i]);
-        }
-        return;
-    }
-    float a = 0.f;
-    bool fine = true;
-#pragma unroll
-    for (int i = 0; i < kParts; ++i) {
-        a = fmaxf(fmaxf(a, fmaxf(fabsf(v[i].x), fabsf(v[i].y))), fmaxf(fabsf(v[i].z), fabsf(v[i].w)));
-        fine = fine && fabsf(v[i].x) < INFINITY && fabsf(v[i].y) < INFINITY && fabsf(v[i].z) < INFINITY && fabsf(v[i].w) < INFINITY;
-    }
-    a = warp_max(a);
-    fine = __all_sync(0xffffffffu, fine);
     const float top = c.type == LV_TYPE_I8 ? 127.f : 448.f;
-    const bool live = fine && a >= kPagedTiny;
-    const float f = live ? top / a : 0.f;
-    if (lane == 0) (which ? c.v_scale : c.k_scale)[row] = live ? a / top : fine ? 0.f : NAN;
 #pragma unroll
-    for (int i = 0; i < kParts; ++i) {
-        const uint32_t at = 4 * (lane + 32 * i);
-        if (at >= c.dim) continue;
-        const float x = live ? v[i].x * f : 0.f, y = live ? v[i].y * f : 0.f, z = live ? v[i].z * f : 0.f, w = live ? v[i].w * f : 0.f;
-        uint32_t u;
-        if (c.type == LV_TYPE_I8) {
-            u = (uint32_t(__float2int_rn(x)) & 0xffu) | ((uint32_t(__float2int_rn(y)) & 0xffu) << 8) | ((uint32_t(__float2int_rn(z)) & 0xffu) << 16) |
-                (uint32_t(__float2int_rn(w)) << 24);
-        } else {
-            u = uint32_t(__nv_cvt_float2_to_fp8x2(make_float2(x, y), __NV_SATFINITE, __NV_E4M3)) |
-                (uint32_t(__nv_cvt_float2_to_fp8x2(make_float2(z, w), __NV_SATFINITE, __NV_E4M3)) << 16);
+    for (int k = 0; k < kAppendRows; ++k) {
+        const uint32_t h = h0 + k * (32 / L);
+        const uint64_t row = row0 + uint64_t(h) * c.page_rows;
+        if (!paged_is8(c.type)) {
+#pragma unroll
+            for (int i = 0; i < PARTS; ++i) {
+                const uint32_t at = at0 + 4 * L * i;
+                if (at < c.dim && h < H) store_values4(out, row * c.dim + at, c.type, v[k][i]);
+            }
+            continue;
         }
-        *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(out) + row * c.dim + at) = u;
+        // the largest magnitude by its bits, which are in the order of the numbers; infinities and NaN are above all numbers
+        uint32_t most = 0;
+#pragma unroll
+        for (int i = 0; i < PARTS; ++i) {
+            const float4 x = v[k][i];
+            most = max(most, max(max(__float_as_uint(x.x) & 0x7fffffffu, __float_as_uint(x.y) & 0x7fffffffu), max(__float_as_uint(x.z) & 0x7fffffffu, __float_as_uint(x.w) & 0x7fffffffu)));
+        }
+        if constexpr (L == 32) {
+            most = __reduce_max_sync(0xffffffffu, most);
+        } else {
+#pragma unroll
+            for (int o = L / 2; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+        }
+        const float a = __uint_as_float(most);
+        const bool fine = most < 0x7f800000u, live = fine && a >= kPagedTiny;
+        const float f = live ? top / a : 0.f;
+        if (h >= H) continue;
+        if (lane % L == 0) (which ? c.v_scale : c.k_scale)[row] = live ? a / top : fine ? 0.f : NAN;
+#pragma unroll
+        for (int i = 0; i < PARTS; ++i) {
+            const uint32_t at = at0 + 4 * L * i;
+            if (at >= c.dim) continue;
+            const float4 x = v[k][i];
+            const float4 y = live ? make_float4(x.x * f, x.y * f, x.z * f, x.w * f) : make_float4(0.f, 0.f, 0.f, 0.f);
+            uint32_t u;
+            if (c.type == LV_TYPE_I8) {
+                u = (uint32_t(__float2int_rn(y.x)) & 0xffu) | ((uint32_t(__float2int_rn(y.y)) & 0xffu) << 8) | ((uint32_t(__float2int_rn(y.z)) & 0xffu) << 16) |
+                    (uint32_t(__float2int_rn(y.w)) << 24);
+            } else {
+                u = uint32_t(__nv_cvt_float2_to_fp8x2(make_float2(y.x, y.y), __NV_SATFINITE, __NV_E4M3)) |
+                    (uint32_t(__nv_cvt_float2_to_fp8x2(make_float2(y.z, y.w), __NV_SATFINITE, __NV_E4M3)) << 16);
+            }
+            *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(out) + row * c.dim + at) = u;
+        }
     }
 }
 
@@ -97,33 +118,71 @@ struct PagedRead {
     uint32_t* err;
 };
 
-// A thread per 16 values of a row: a 16-byte load of codes, 32 or 64 bytes out.  Grid: (units of the rows of one head, heads x {k, v}, sequences).
+// A thread takes eight neighbouring values of four rows: 8 or 16 bytes in, 16 (f32: 32) out, in step with its neighbours.  Grid: (rows of one head, heads x {keys, values},
+// sequences).
+// FIGURES_READ
+constexpr int kReadRows = 4;
 __global__ void __launch_bounds__(256) paged_read_kernel(const PagedRead p) {
     pdl_launch_dependents();
     pdl_wait();
     const lv_paged_cache& c = p.c;
-    const uint32_t units = c.dim / 16, H = c.kv_heads, s = blockIdx.z, which = blockIdx.y / H, h = blockIdx.y - which * H;
-    const uint32_t len = c.lens[s];
-    const uint64_t job = uint64_t(blockIdx.x) * blockDim.x + threadIdx.x;
-    const uint32_t i = uint32_t(job / units), u = uint32_t(job - uint64_t(i) * units);
+    const uint32_t units = c.dim / 8, each = blockDim.x / units, H = c.kv_heads, s = blockIdx.z, which = blockIdx.y / H, h = blockIdx.y - which * H;
+    const uint32_t len = c.lens[s], i0 = threadIdx.x / units, u = threadIdx.x - i0 * units;
     if (len > uint64_t(c.table_ld) * c.page_rows) {
         if (threadIdx.x == 0) atomicOr(p.err, ERR_BAD_INDEX);
         return;
     }
-    if (i >= p.rows || p.first >= len || i >= len - p.first) return;
-    uint64_t row;
-    if (!paged_row(c, c.table + size_t(s) * c.table_ld, p.first + i, h, &row)) {
-        atomicOr(p.err, ERR_BAD_INDEX);
-        return;
-    }
+    if (p.first >= len || i0 >= each) return;
+    const uint32_t rows = min(p.rows, len - p.first);
+    const uint64_t base = uint64_t(blockIdx.x) * each * kReadRows + i0;
     const void* in = which ? c.v : c.k;
-    const float f = paged_is8(c.type) ? (which ? c.v_scale : c.k_scale)[row] : 1.f;
-    const size_t to = s * p.seq_stride + h * p.head_stride + i * p.row_stride + 16 * u;
+    const float* scales = which ? c.v_scale : c.k_scale;
+    uint64_t row[kReadRows];
+    bool here[kReadRows];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        float4 v = load_cached4(in, row * c.dim + 16 * u + 4 * k, c.type);
-        if (paged_is8(c.type)) v = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
-        store_values4(p.out[which], to + 4 * k, p.out_type, v);
+    for (int k = 0; k < kReadRows; ++k) {
+        const uint64_t i = base + k * each;
+        here[k] = i < rows;
+        if (here[k] && !paged_row(c, c.table + size_t(s) * c.table_ld, p.first + uint32_t(i), h, &row[k])) {
+            atomicOr(p.err, ERR_BAD_INDEX);
+            here[k] = false;
+        }
+    }
+    uint4 v[kReadRows];                                                  // eight values, or (the first two words) codes
+    float f[kReadRows];
+#pragma unroll
+    for (int k = 0; k < kReadRows; ++k) {
+        if (!here[k]) continue;
+        const size_t at = row[k] * c.dim + 8 * u;
+        if (paged_is8(c.type)) {
+            const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(in) + at);
+            v[k] = make_uint4(w.x, w.y, 0u, 0u);
+            f[k] = scales[row[k]];
+        } else {
+            v[k] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(in) + at);
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < kReadRows; ++k) {
+        if (!here[k]) continue;
+        float4 x, y;
+        if (paged_is8(c.type)) {
+            x = code_values4(v[k].x, c.type);
+            y = code_values4(v[k].y, c.type);
+            x = make_float4(x.x * f[k], x.y * f[k], x.z * f[k], x.w * f[k]);
+            y = make_float4(y.x * f[k], y.y * f[k], y.z * f[k], y.w * f[k]);
+        } else {
+            x = unpack_values4(make_uint2(v[k].x, v[k].y), c.type);
+            y = unpack_values4(make_uint2(v[k].z, v[k].w), c.type);
+        }
+        const size_t to = s * p.seq_stride + h * p.head_stride + (base + k * each) * p.row_stride + 8 * u;
+        if (p.out_type == LV_TYPE_F32) {
+            store_values4(p.out[which], to, LV_TYPE_F32, x);
+            store_values4(p.out[which], to + 4, LV_TYPE_F32, y);
+        } else {
+            const uint2 a = pack_values4(x, p.out_type), b = pack_values4(y, p.out_type);
+            *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out[which]) + to) = make_uint4(a.x, a.y, b.x, b.y);
+        }
     }
 }
 
@@ -147,7 +206,8 @@ extern "C" int lv_paged_append(lv_ctx* ctx, const lv_paged_cache* cache, const v
     LV_REQUIRE(k && v && paged_value_type(in_type), "paged append: bad input");
     LV_REQUIRE(ld >= uint64_t(cache->kv_heads) * cache->dim && uint64_t(ld) * paged_bytes(in_type) % 16 == 0 && aligned16(k) && aligned16(v), "paged append: rows of k and v are 16-byte aligned");
     if (const int rc = paged_check_rotation(angles, angle_ld, angle_pairs, cache->dim)) return rc;
-    const uint64_t warps = uint64_t(tokens) * cache->kv_heads * 2;
+    const uint32_t heads = kAppendRows * (cache->dim <= 64 ? 2 : 1);
+    const uint64_t warps = uint64_t(tokens) * 2 * ((cache->kv_heads + heads - 1) / heads);
     LV_REQUIRE(warps < (uint64_t(1) << 31), "paged append: too many tokens");
     LV_ENTER(ctx);
     if (!tokens) return LV_OK;
@@ -162,7 +222,10 @@ extern "C" int lv_paged_append(lv_ctx* ctx, const lv_paged_cache* cache, const v
     p.tokens = tokens;
     p.in_type = in_type;
     p.err = ctx->d_err;
-    LV_CUDA(launch_pdl(ctx, paged_append_kernel, dim3(uint32_t((warps + 7) / 8)), dim3(256), 0, p));
+    const dim3 grid(uint32_t((warps + 7) / 8));
+    if (cache->dim <= 64) LV_CUDA(launch_pdl(ctx, paged_append_kernel<16, 1>, grid, dim3(256), 0, p));
+    else if (cache->dim <= 128) LV_CUDA(launch_pdl(ctx, paged_append_kernel<32, 1>, grid, dim3(256), 0, p));
+    else LV_CUDA(launch_pdl(ctx, paged_append_kernel<32, 2>, grid, dim3(256), 0, p));
     return LV_OK;
 }
 
@@ -172,7 +235,8 @@ extern "C" int lv_paged_read(lv_ctx* ctx, const lv_paged_cache* cache, void* k_o
     LV_REQUIRE(k_out && v_out && paged_value_type(out_type), "paged read: bad output");
     const size_t unit = 16 / paged_bytes(out_type);
     LV_REQUIRE(seq_stride % unit == 0 && head_stride % unit == 0 && row_stride % unit == 0 && aligned16(k_out) && aligned16(v_out), "paged read: rows are 16-byte aligned");
-    const uint64_t blocks = (uint64_t(rows) * (cache->dim / 16) + 255) / 256;
+    const uint32_t block_rows = 256 / (cache->dim / 8) * kReadRows;
+    const uint64_t blocks = (uint64_t(rows) + block_rows - 1) / block_rows;
     LV_REQUIRE(cache->kv_heads <= 32767 && blocks < (uint64_t(1) << 31), "paged read: too many heads or rows");
     LV_ENTER(ctx);
     if (!rows) return LV_OK;

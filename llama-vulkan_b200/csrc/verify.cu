@@ -1,15 +1,44 @@
 // Probabilities from logits, and drafted tokens against them.
+#include "attention_gqa.cuh"
 #include "paged.cuh"
 
 namespace lv {
 
-constexpr int kProbThreads = 1024;
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+    uint32_t n;
+    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(n));
+    return n;
+}
+// a word (two words) into the shared memory of another CTA of the cluster
+__device__ __forceinline__ void cluster_store(void* local, uint32_t rank, uint2 v) {
+    uint32_t at;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(local)), "r"(rank));
+    asm volatile("st.shared::cluster.v2.u32 [%0], {%1, %2};" ::"r"(at), "r"(v.x), "r"(v.y) : "memory");
+}
+
+// Before the first store into another CTA's memory it has to be there: arrive first thing, wait behind the earlier launch.
+__device__ __forceinline__ void cluster_here() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_all_here() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+// ---- probabilities --------------------------------------------------------------------------------
+
+// out = e^((x - m) / T) / sum: a cluster of up to 16 CTAs takes a row, so that all of it lies in registers between the read and the write; the CTAs tell one another
+// their maximum and sum once.  A value is read, raised and written once; longer rows than 16 x 16384 are read and raised a second time.
+// FIGURES_PROBS
+constexpr int kProbThreads = 512, kProbGroups = 8;                       // groups of four values that a thread holds
+constexpr uint32_t kProbHeld = kProbThreads * 4 * kProbGroups;           // of a CTA: 16384
+constexpr int kProbCluster = 16;
 
 struct Probabilities {
     float* out;
     const float* logits;
     const float* temperature;
-    uint32_t out_ld, ld, vocab;
+    uint32_t out_ld, ld, vocab, each;                                    // each: values of a CTA, a multiple of 4
 };
 
 // the first index of the larger value (NaN is smaller than all)
@@ -17,148 +46,286 @@ __device__ __forceinline__ void first_max(float& v, uint32_t& i, float w, uint32
     if (w > v || (w == v && j < i)) { v = w; i = j; }
 }
 
-// A CTA per row
-__global__ void __launch_bounds__(kProbThreads) probabilities_kernel(const Probabilities p) {
+// VEC: rows are 16-byte aligned; HELD: a CTA's values fit its registers
+template <bool VEC, bool HELD>
+__global__ void __launch_bounds__(kProbThreads, 2) probabilities_kernel(const Probabilities p) {
     pdl_launch_dependents();
+    cluster_here();
     pdl_wait();
-    __shared__ float s_f[64];
-    __shared__ uint32_t s_i[32];
-    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x / 32;
-    const float* x = p.logits + size_t(blockIdx.x) * p.ld;
-    float* y = p.out + size_t(blockIdx.x) * p.out_ld;
-    const float T = p.temperature ? p.temperature[blockIdx.x] : 1.f;
+    cluster_all_here();
+    __shared__ float s_top[kProbThreads / 32], s_sum[kProbThreads / 32];
+    __shared__ uint32_t s_at[kProbThreads / 32];
+    __shared__ __align__(8) uint2 s_all[2][kProbCluster];                 // {maximum, its index}, {sum}
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x / 32, rank = cluster_rank(), n = cluster_size(), row = blockIdx.x / n;
+    const float* x = p.logits + size_t(row) * p.ld;
+    float* y = p.out + size_t(row) * p.out_ld;
+    const float T = p.temperature ? p.temperature[row] : 1.f;
+    const float f = T == 0.f ? 1.f : 1.4426950408889634f / T;            // e^(z / T) as a power of two
+    const uint32_t lo = min(p.vocab, rank * p.each), hi = min(p.vocab, lo + p.each);
+    // values i .. i + 3; those behind the end count as -inf
+    auto load4 = [&](uint32_t i) {
+        float4 v = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        if (VEC && i + 3 < hi) return *reinterpret_cast<const float4*>(x + i);
+        if (i < hi) v.x = x[i];
+        if (i + 1 < hi) v.y = x[i + 1];
+        if (i + 2 < hi) v.z = x[i + 2];
+        if (i + 3 < hi) v.w = x[i + 3];
+        return v;
+    };
+    auto store4 = [&](uint32_t i, const float4& v) {
+        if (VEC && i + 3 < hi) {
+            *reinterpret_cast<float4*>(y + i) = v;
+            return;
+        }
+        if (i < hi) y[i] = v.x;
+        if (i + 1 < hi) y[i + 1] = v.y;
+        if (i + 2 < hi) y[i + 2] = v.z;
+        if (i + 3 < hi) y[i + 3] = v.w;
+    };
+    constexpr uint32_t kStep = kProbThreads * 4;
+    float4 v[HELD ? kProbGroups : 1];
     float top = -INFINITY;
     uint32_t at = 0xffffffffu;
-    bool odd = false;
-    for (uint32_t i = threadIdx.x; i < p.vocab; i += blockDim.x) {
-        const float v = x[i];
-        odd = odd || v != v;
-        first_max(top, at, v, i);
+    auto look = [&](const float4& w, uint32_t i) {
+        // (in the order of the indexes: a later value has to be larger)
+        if (w.x > top) { top = w.x; at = i; }
+        if (w.y > top) { top = w.y; at = i + 1; }
+        if (w.z > top) { top = w.z; at = i + 2; }
+        if (w.w > top) { top = w.w; at = i + 3; }
+    };
+    if constexpr (HELD) {
+#pragma unroll
+        for (int k = 0; k < kProbGroups; ++k) v[k] = load4(lo + 4 * threadIdx.x + k * kStep);
+#pragma unroll
+        for (int k = 0; k < kProbGroups; ++k) look(v[k], lo + 4 * threadIdx.x + k * kStep);
+    } else {
+        for (uint32_t i = lo + 4 * threadIdx.x; i < hi; i += kStep) look(load4(i), i);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-        const float v = __shfl_xor_sync(0xffffffffu, top, o);
+        const float w = __shfl_xor_sync(0xffffffffu, top, o);
         const uint32_t j = __shfl_xor_sync(0xffffffffu, at, o);
-        first_max(top, at, v, j);
+        first_max(top, at, w, j);
     }
-    if (lane == 0) { s_f[warp] = top; s_i[warp] = at; }
-    odd = __syncthreads_or(odd);
-    for (int w = 0; w < kProbThreads / 32; ++w) first_max(top, at, s_f[w], s_i[w]);
+    if (lane == 0) { s_top[warp] = top; s_at[warp] = at; }
     __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kProbThreads / 32; ++w) first_max(top, at, s_top[w], s_at[w]);
+    const float base = top == -INFINITY ? 0.f : top;
+    float sum = 0.f;
+    auto raise4 = [&](const float4& w) { return make_float4(exp2_fast((w.x - base) * f), exp2_fast((w.y - base) * f), exp2_fast((w.z - base) * f), exp2_fast((w.w - base) * f)); };
+    if (T != 0.f) {
+        if constexpr (HELD) {
+#pragma unroll
+            for (int k = 0; k < kProbGroups; ++k) {
+                if (lo + k * kStep >= hi) continue;
+                v[k] = raise4(v[k]);
+                sum += (v[k].x + v[k].y) + (v[k].z + v[k].w);
+            }
+        } else {
+            for (uint32_t i = lo + 4 * threadIdx.x; i < hi; i += kStep) {
+                const float4 w = raise4(load4(i));
+                sum += (w.x + w.y) + (w.z + w.w);
+            }
+        }
+        sum = warp_sum(sum);
+        if (lane == 0) s_sum[warp] = sum;
+        __syncthreads();
+        sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < kProbThreads / 32; ++w) sum += s_sum[w];
+    }
+    float whole = top, total = 0.f;
+    if (threadIdx.x < n) {
+        cluster_store(&s_all[0][rank], threadIdx.x, make_uint2(__float_as_uint(top), at));
+        cluster_store(&s_all[1][rank], threadIdx.x, make_uint2(__float_as_uint(sum), 0u));
+    }
+    cluster_sync();
+    for (uint32_t r = 0; r < n; ++r) first_max(whole, at, __uint_as_float(s_all[0][r].x), s_all[0][r].y);
+    for (uint32_t r = 0; r < n; ++r) {
+        const float m = __uint_as_float(s_all[0][r].x), part = __uint_as_float(s_all[1][r].x);
+        total += m == -INFINITY ? part : part * exp2_fast((m - whole) * f);   // (without a maximum there is nothing, or NaN)
+    }
     if (T == 0.f) {
         if (at == 0xffffffffu) at = 0;
-        for (uint32_t i = threadIdx.x; i < p.vocab; i += blockDim.x) y[i] = i == at ? 1.f : 0.f;
+        for (uint32_t i = lo + 4 * threadIdx.x; i < hi; i += kStep) store4(i, make_float4(i == at, i + 1 == at, i + 2 == at, i + 3 == at));
         return;
     }
-    const float f = 1.f / T;
-    float sum = 0.f;
-    for (uint32_t i = threadIdx.x; i < p.vocab; i += blockDim.x) sum += expf((x[i] - top) * f);
-    sum = block_sum(sum, s_f);
-    const float g = odd ? NAN : top == -INFINITY ? 0.f : 1.f / sum;
-    for (uint32_t i = threadIdx.x; i < p.vocab; i += blockDim.x) y[i] = g == 0.f ? 0.f : expf((x[i] - top) * f) * g;
+    const float g = total == 0.f ? 0.f : (top == -INFINITY ? 1.f : exp2_fast((top - whole) * f)) / total;
+    if constexpr (HELD) {
+#pragma unroll
+        for (int k = 0; k < kProbGroups; ++k) store4(lo + 4 * threadIdx.x + k * kStep, make_float4(v[k].x * g, v[k].y * g, v[k].z * g, v[k].w * g));
+    } else {
+        for (uint32_t i = lo + 4 * threadIdx.x; i < hi; i += kStep) {
+            const float4 w = raise4(load4(i));
+            store4(i, make_float4(w.x * g, w.y * g, w.z * g, w.w * g));
+        }
+    }
 }
 
-constexpr int kVerifyThreads = 1024;
+// ---- verification ---------------------------------------------------------------------------------
+
+// A cluster of eight CTAs takes a sequence.  Every CTA finds the first rejected draft by itself (two values a draft), then they sum the weights of the one row that
+// a token is drawn from, each an eighth of it and every warp a run of neighbours, and tell one another their sums.  The bounds between runs are the same numbers
+// for both neighbours, so that exactly one run holds the target; its warp looks through it again.  Sums are f64: the first index whose cumulative weight is above
+// the target does not depend on the order of the sums but where the two agree to 2^-52.
+// FIGURES_VERIFY
+constexpr int kVerifyThreads = 512, kVerifyWarps = kVerifyThreads / 32, kVerifyCluster = 8;
 constexpr uint32_t kNobody = 0xffffffffu;
 
-__device__ __forceinline__ double rest_of(const float* p, const float* q, uint32_t drafted, bool rejected, uint32_t i) {
-    double w = p[i];
-    if (rejected) w -= q ? double(q[i]) : i == drafted ? 1.0 : 0.0;
-    return w > 0.0 ? w : 0.0;
-}
-
-// A CTA per sequence
+template <bool VEC>
 __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const lv_verify_args a, uint32_t* err) {
     pdl_launch_dependents();
+    cluster_here();
     pdl_wait();
-    __shared__ double s_sum[33];
-    __shared__ uint32_t s_accepted, s_pick, s_last;
-    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x / 32, s = blockIdx.x;
+    cluster_all_here();
+    __shared__ double s_before[kVerifyWarps + 1];
+    __shared__ __align__(8) uint2 s_all[2][kVerifyCluster];              // the CTAs' sums (of the first and of the second attempt)
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x / 32, rank = cluster_rank(), s = blockIdx.x / kVerifyCluster;
     const uint32_t row0 = a.starts[s], row1 = a.starts[s + 1];
+    const float pick = a.pick[s];
     if (row0 > row1 || row1 > a.rows) {
-        if (threadIdx.x == 0) atomicOr(err, ERR_BAD_INDEX);
+        if (rank == 0 && threadIdx.x == 0) atomicOr(err, ERR_BAD_INDEX);
         return;
     }
     if (row0 == row1) {
-        if (threadIdx.x == 0) a.accepted[s] = 0;
+        if (rank == 0 && threadIdx.x == 0) a.accepted[s] = 0;
         return;
     }
+    // every warp looks at the drafts: no barrier
     const uint32_t n = row1 - row0 - 1;
-    if (warp == 0) {
-        uint32_t good = n;
-        for (uint32_t b = 0; b < n; b += 32) {
-            bool bad = false;
-            if (b + lane < n) {
-                const uint32_t r = row0 + b + lane, d = a.drafted[r];
-                if (d >= a.vocab) {
-                    atomicOr(err, ERR_BAD_INDEX);
-                    bad = true;
-                } else {
-                    const double q = a.draft ? double(a.draft[size_t(r) * a.draft_ld + d]) : 1.0;
-                    bad = !(double(a.accept[r]) * q < double(a.target[size_t(r) * a.target_ld + d]));
-                }
-            }
-            const uint32_t first = __ballot_sync(0xffffffffu, bad);
-            if (first != 0) {
-                good = b + uint32_t(__ffs(int(first))) - 1;
-                break;
+    uint32_t accepted = n, drafted = kNobody;
+    for (uint32_t b = 0; b < n; b += 32) {
+        bool bad = false;
+        uint32_t d = kNobody;
+        if (b + lane < n) {
+            const uint32_t r = row0 + b + lane;
+            d = a.drafted[r];
+            bad = d >= a.vocab;
+            if (!bad) {
+                const double q = a.draft ? double(a.draft[size_t(r) * a.draft_ld + d]) : 1.0;
+                bad = !(double(a.accept[r]) * q < double(a.target[size_t(r) * a.target_ld + d]));
             }
         }
-        if (lane == 0) { s_accepted = good; s_pick = kNobody; s_last = 0; }
+        const uint32_t first = __ballot_sync(0xffffffffu, bad);
+        if (first != 0) {
+            const int l = __ffs(int(first)) - 1;
+            accepted = b + uint32_t(l);
+            drafted = __shfl_sync(0xffffffffu, d, l);
+            break;
+        }
     }
-    __syncthreads();
-    const uint32_t accepted = s_accepted, r = row0 + accepted;
+    if (accepted < n && drafted >= a.vocab && rank == 0 && threadIdx.x == 0) atomicOr(err, ERR_BAD_INDEX);
+    const uint32_t r = row0 + accepted;
     const float *p = a.target + size_t(r) * a.target_ld, *q = a.draft ? a.draft + size_t(r) * a.draft_ld : nullptr;
-    const uint32_t drafted = accepted < n ? a.drafted[r] : kNobody;
-    bool rejected = accepted < n;
-    const uint32_t each = (a.vocab + kVerifyThreads - 1) / kVerifyThreads, lo = min(a.vocab, threadIdx.x * each), hi = min(a.vocab, lo + each);
-    double mine = 0.0, before = 0.0, total = 0.0;
-    for (;;) {
+    // runs of 128 values: those of this warp
+    const uint32_t each = (a.vocab + 128 * kVerifyCluster * kVerifyWarps - 1) / (128 * kVerifyCluster * kVerifyWarps);
+    const uint64_t lo = uint64_t(rank * kVerifyWarps + warp) * each * 128;
+    auto load4 = [&](const float* x, uint64_t i) {
+        if (VEC && i + 3 < a.vocab) return *reinterpret_cast<const float4*>(x + i);
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (i < a.vocab) v.x = x[i];
+        if (i + 1 < a.vocab) v.y = x[i + 1];
+        if (i + 2 < a.vocab) v.z = x[i + 2];
+        if (i + 3 < a.vocab) v.w = x[i + 3];
+        return v;
+    };
+    struct Four { double w[4]; };
+    auto weights = [&](uint64_t i, bool rest) {
+        const float4 x = load4(p, i);
+        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (rest) y = q ? load4(q, i) : make_float4(i == drafted, i + 1 == drafted, i + 2 == drafted, i + 3 == drafted);
+        Four f = {{double(x.x) - double(y.x), double(x.y) - double(y.y), double(x.z) - double(y.z), double(x.w) - double(y.w)}};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) f.w[k] = f.w[k] > 0.0 ? f.w[k] : 0.0;
+        return f;
+    };
+    bool rest = accepted < n;
+    double mine = 0.0, total = 0.0, cta0 = 0.0, cta1 = 0.0;
+    for (int attempt = 0;; ++attempt) {
         mine = 0.0;
-        for (uint32_t i = lo; i < hi; ++i) mine += rest_of(p, q, drafted, rejected, i);
-        double incl = mine;
+#pragma unroll 4
+        for (uint32_t k = 0; k < each; ++k) {
+            const Four f = weights(lo + 128 * k + 4 * lane, rest);
+            mine += (f.w[0] + f.w[1]) + (f.w[2] + f.w[3]);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+        if (attempt != 0) __syncthreads();
+        if (lane == 0) s_before[warp + 1] = mine;
+        __syncthreads();
+        if (warp == 0) {
+            double run = lane < kVerifyWarps ? s_before[lane + 1] : 0.0;
+#pragma unroll
+            for (int o = 1; o < kVerifyWarps; o <<= 1) {
+                const double up = __shfl_up_sync(0xffffffffu, run, o);
+                if (lane >= uint32_t(o)) run += up;
+            }
+            __syncwarp();
+            if (lane < kVerifyWarps) s_before[lane + 1] = run;
+            if (lane == 0) s_before[0] = 0.0;
+            const double sum = __shfl_sync(0xffffffffu, run, kVerifyWarps - 1);
+            if (lane < kVerifyCluster) cluster_store(&s_all[attempt][rank], lane, make_uint2(uint32_t(__double2loint(sum)), uint32_t(__double2hiint(sum))));
+        }
+        cluster_sync();
+        total = 0.0;
+#pragma unroll
+        for (uint32_t c = 0; c < kVerifyCluster; ++c) {
+            const uint2 u = s_all[attempt][c];
+            if (c == rank) cta0 = total;
+            total += __hiloint2double(int(u.y), int(u.x));
+            if (c == rank) cta1 = total;
+        }
+        if (total > 0.0 || !rest) break;
+        rest = false;                                                    // nothing is left behind the draft: from the target itself
+    }
+    if (rank == 0) {
+        for (uint32_t i = threadIdx.x; i <= n; i += kVerifyThreads)
+            if (i != accepted) a.tokens[row0 + i] = i < accepted ? a.drafted[row0 + i] : kNobody;
+        if (threadIdx.x == 0) {
+            a.accepted[s] = accepted;
+            if (a.lens) a.lens[s] -= n - accepted;
+            if (!(total > 0.0)) {
+                a.tokens[r] = kNobody;
+                atomicOr(err, ERR_BAD_INDEX);
+            }
+        }
+    }
+    // the run that holds the target: bounds are sums in a fixed order, the last one of a CTA is the first one of the next
+    const double target = double(pick) * total;
+    const double from = cta0 + s_before[warp], to = warp + 1 == kVerifyWarps ? cta1 : cta0 + s_before[warp + 1];
+    const bool last = rank + 1 == kVerifyCluster && warp + 1 == kVerifyWarps;
+    if (!(total > 0.0) || !(from <= target || (rank == 0 && warp == 0)) || !(target < to || last)) return;
+    double run = from;
+    uint32_t found = kNobody, fallback = kNobody;
+    for (uint32_t k = 0; k < each && found == kNobody; ++k) {
+        const uint64_t i = lo + 128 * k + 4 * lane;
+        const Four f = weights(i, rest);
+        const double sum = (f.w[0] + f.w[1]) + (f.w[2] + f.w[3]);
+        double incl = sum;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const double up = __shfl_up_sync(0xffffffffu, incl, o);
             if (lane >= uint32_t(o)) incl += up;
         }
-        __syncthreads();
-        if (lane == 31) s_sum[warp] = incl;
-        __syncthreads();
-        before = total = 0.0;
-        for (uint32_t w = 0; w < kVerifyThreads / 32; ++w) {
-            if (w == warp) before = total;
-            total += s_sum[w];
-        }
-        before += incl - mine;
-        if (total > 0.0 || !rejected) break;
-        rejected = false;
-    }
-    const double target = double(a.pick[s]) * total;
-    if (mine > 0.0) {
-        double cum = before;
-        uint32_t last = 0;
-        bool found = false;
-        for (uint32_t i = lo; i < hi; ++i) {
-            const double w = rest_of(p, q, drafted, rejected, i);
-            if (w > 0.0) last = i + 1;
-            cum += w;
-            if (cum > target && !found) {
-                found = true;
-                atomicMin(&s_pick, i);
+        double cum = run + (incl - sum);
+        uint32_t at = kNobody, end = kNobody;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            cum += f.w[j];
+            if (f.w[j] > 0.0) {
+                end = uint32_t(i) + j;
+                if (at == kNobody && cum > target) at = end;
             }
         }
-        atomicMax(&s_last, last);
+        found = __reduce_min_sync(0xffffffffu, at);
+        const uint32_t any = __reduce_max_sync(0xffffffffu, end + 1u);   // (kNobody + 1 is 0)
+        if (any != 0) fallback = any - 1u;
+        run += __shfl_sync(0xffffffffu, incl, 31);
     }
-    __syncthreads();
-    uint32_t pick = s_pick;
-    if (pick == kNobody && s_last != 0) pick = s_last - 1;
-    for (uint32_t i = threadIdx.x; i <= n; i += kVerifyThreads) a.tokens[row0 + i] = i < accepted ? a.drafted[row0 + i] : i == accepted ? pick : kNobody;
-    if (threadIdx.x == 0) {
-        a.accepted[s] = accepted;
-        if (pick == kNobody) atomicOr(err, ERR_BAD_INDEX);
-        if (a.lens) a.lens[s] -= n - accepted;
-    }
+    // (rounding may leave the target at the very end of the run)
+    if (found == kNobody) found = fallback;
+    if (lane == 0 && found != kNobody) a.tokens[r] = found;
 }
 
 }  // namespace lv
@@ -167,20 +334,28 @@ using namespace lv;
 
 extern "C" int lv_probabilities(lv_ctx* ctx, float* out, uint32_t out_ld, const float* logits, uint32_t ld, uint32_t vocab, uint32_t rows, const float* temperature) {
     LV_REQUIRE(out && logits && vocab && out_ld >= vocab && ld >= vocab, "probabilities: bad arguments");
-    LV_REQUIRE(vocab <= (1u << 24) && rows < (1u << 31), "probabilities: vocabulary larger than 16777216 or too many rows");
+    LV_REQUIRE(vocab <= (1u << 24) && rows < (1u << 27), "probabilities: vocabulary larger than 16777216 or too many rows");
     LV_REQUIRE(out != logits || out_ld == ld, "probabilities: in place, the strides are the same");
     LV_ENTER(ctx);
     if (!rows) return LV_OK;
-    Probabilities p{out, logits, temperature, out_ld, ld, vocab};
-    LV_CUDA(launch_pdl(ctx, probabilities_kernel, dim3(rows), dim3(kProbThreads), 0, p));
+    Probabilities p{out, logits, temperature, out_ld, ld, vocab, 0};
+    // as many CTAs as hold the row; with few rows more of them, down to 2048 values each (FIGURES_SPLIT)
+    uint32_t n = 1;
+    while (n < uint32_t(kProbCluster) && (uint64_t(n) * kProbHeld < vocab || (uint64_t(rows) * n * 2 <= uint64_t(ctx->sm_count) && n < 8 && vocab / (2 * n) >= 2048))) n *= 2;
+    p.each = ((vocab + n - 1) / n + 3) / 4 * 4;
+    const bool vec = aligned16(out) && aligned16(logits) && out_ld % 4 == 0 && ld % 4 == 0, held = p.each <= kProbHeld;
+    auto* kernel = vec ? (held ? probabilities_kernel<true, true> : probabilities_kernel<true, false>) : (held ? probabilities_kernel<false, true> : probabilities_kernel<false, false>);
+    if (n > 8) LV_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    LV_CUDA(launch_pdl_cluster(ctx, kernel, dim3(rows * n), dim3(kProbThreads), dim3(n), 0, p));
     return LV_OK;
 }
 
 extern "C" int lv_verify_drafts(lv_ctx* ctx, const lv_verify_args* a) {
     LV_REQUIRE(a && a->target && a->drafted && a->starts && a->accept && a->pick && a->tokens && a->accepted, "verification of drafts: null argument");
     LV_REQUIRE(a->vocab && a->vocab <= (1u << 24) && a->target_ld >= a->vocab && (!a->draft || a->draft_ld >= a->vocab), "verification of drafts: bad sizes");
-    LV_REQUIRE(a->seqs && a->rows < (1u << 31), "verification of drafts: too many rows");
+    LV_REQUIRE(a->seqs && a->seqs < (1u << 28) && a->rows < (1u << 31), "verification of drafts: too many rows");
     LV_ENTER(ctx);
-    LV_CUDA(launch_pdl(ctx, verify_kernel, dim3(a->seqs), dim3(kVerifyThreads), 0, *a, ctx->d_err));
+    const bool vec = aligned16(a->target) && a->target_ld % 4 == 0 && aligned16(a->draft) && (!a->draft || a->draft_ld % 4 == 0);
+    LV_CUDA(launch_pdl_cluster(ctx, vec ? verify_kernel<true> : verify_kernel<false>, dim3(a->seqs * kVerifyCluster), dim3(kVerifyThreads), dim3(kVerifyCluster), 0, *a, ctx->d_err));
     return LV_OK;
 }
