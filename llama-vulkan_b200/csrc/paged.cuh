@@ -14,9 +14,31 @@ namespace lv {
 
 constexpr float kPagedTiny = 0x1p-100f;          // rows whose largest magnitude is below are stored as zeros
 
+// n / d for n < 2^31: (n * mul) >> (31 + shift) with shift = ceil(log2 d) and mul = ceil(2^(31 + shift) / d), which has 32 bits.  Exact: mul * d exceeds
+// 2^(31 + shift) by less than d, so that n * mul / 2^(31 + shift) exceeds n / d by less than n / 2^(31 + shift) < 2^-shift <= 1 / d.
+struct PagedDiv {
+    uint32_t mul, shift;
+};
+inline PagedDiv paged_div(uint32_t d) {
+    uint32_t shift = 0;
+    while ((uint64_t(1) << shift) < d) ++shift;
+    return {uint32_t(((uint64_t(1) << (31 + shift)) + d - 1) / d), shift};
+}
+
+// A cache as the kernels get it
+struct PagedCache : lv_paged_cache {
+    PagedDiv by_rows;                            // a position's page
+};
+inline PagedCache paged_cache(const lv_paged_cache& c) {
+    PagedCache p{};
+    static_cast<lv_paged_cache&>(p) = c;
+    p.by_rows = paged_div(c.page_rows);
+    return p;
+}
+
 // Row (of k or v, and of the scales) of a head's position; false: the table names no page of the cache.  64 bits: a cache has more than 2^32 values.
-__host__ __device__ __forceinline__ bool paged_row(const lv_paged_cache& c, const uint32_t* table_row, uint32_t position, uint32_t head, uint64_t* row) {
-    const uint32_t slot = position / c.page_rows, page = slot < c.table_ld ? table_row[slot] : c.pages;
+__host__ __device__ __forceinline__ bool paged_row(const PagedCache& c, const uint32_t* table_row, uint32_t position, uint32_t head, uint64_t* row) {
+    const uint32_t slot = uint32_t((uint64_t(position) * c.by_rows.mul) >> (31 + c.by_rows.shift)), page = slot < c.table_ld ? table_row[slot] : c.pages;
     *row = (uint64_t(page) * c.kv_heads + head) * c.page_rows + (position - slot * c.page_rows);
     return page < c.pages;
 }
@@ -33,17 +55,20 @@ __device__ __forceinline__ bool paged_seq(const lv_paged_cache& c, uint32_t s, u
     return a <= b && b <= tokens && b - a <= len && len <= uint64_t(c.table_ld) * c.page_rows;
 }
 
-// The sequence of row t: the last s with starts[s] <= t (seqs: t belongs to nobody).  Ends for any contents of starts.
+// The sequence of row t: the last s with starts[s] <= t (seqs: t belongs to nobody); for a whole warp, 32 places at a time.  Ends for any contents of starts.
 __device__ __forceinline__ uint32_t paged_owner(const lv_paged_cache& c, uint32_t t) {
-    if (t < c.starts[0]) return c.seqs;
-    uint32_t lo = 0, hi = c.seqs;                // starts[lo] <= t < starts[hi], were starts[seqs + 1] infinite
-    if (t >= c.starts[hi]) return c.seqs;
-    while (hi - lo > 1) {
-        const uint32_t mid = (lo + hi) / 2;
-        if (c.starts[mid] <= t) lo = mid;
-        else hi = mid;
+    const uint32_t lane = threadIdx.x & 31u, end = c.starts[c.seqs];
+    uint32_t lo = 0, n = c.seqs;                 // of the places lo .. lo + n - 1
+    while (true) {
+        const uint32_t step = (n + 31) / 32;
+        const uint32_t below = __ballot_sync(0xffffffffu, lane * step < n && c.starts[lo + lane * step] <= t);
+        if (below == 0) return c.seqs;           // (in front of the first)
+        const uint32_t last = uint32_t(__popc(below)) - 1;
+        lo += last * step;
+        n = min(step, n - last * step);
+        if (step == 1) break;
     }
-    return lo;
+    return t < end ? lo : c.seqs;
 }
 
 __host__ __device__ __forceinline__ bool paged_is8(int type) { return type == LV_TYPE_I8 || type == LV_TYPE_E4M3; }

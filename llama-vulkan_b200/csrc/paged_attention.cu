@@ -79,7 +79,7 @@ __global__ void __launch_bounds__(32 * kPrWarps) paged_rows_kernel(const PagedAt
     pdl_launch_dependents();
     pdl_wait();
     const lv_paged_attention_args& a = p.a;
-    const lv_paged_cache& c = a.cache;
+    const PagedCache& c = p.c;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, quad = lane >> 2, tq = lane & 3;
     const uint32_t split = blockIdx.x % p.splits, kv = blockIdx.y, r0 = blockIdx.x / p.splits * S::kRows;
     PagedSeq q;
@@ -506,7 +506,7 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedAttn p, uint
     pdl_launch_dependents();
     pdl_wait();
     const lv_paged_attention_args& a = p.a;
-    const lv_paged_cache& c = a.cache;
+    const PagedCache& c = p.c;
     const uint32_t lane = threadIdx.x & 31u;
     const uint64_t job = uint64_t(blockIdx.x) * 4 + threadIdx.x / 32;
     const uint32_t t = uint32_t(job / a.heads), h = uint32_t(job - uint64_t(t) * a.heads);
@@ -629,6 +629,7 @@ extern "C" int lv_paged_attention(lv_ctx* ctx, const lv_paged_attention_args* a,
     if (!a->tokens || !a->max_new) return LV_OK;
     PagedAttn p{};
     p.a = *a;
+    p.c = paged_cache(a->cache);
     p.group = a->heads / a->cache.kv_heads;
     p.chunk = plan.chunk;
     p.splits = plan.splits;

@@ -16,6 +16,7 @@ constexpr int kPtRows = 256, kPtKeys = 128;      // rows of a block and keys of 
 
 struct PagedAttn {
     lv_paged_attention_args a;
+    PagedCache c;                // a.cache
     uint32_t group;              // query heads of a key/value head
     uint32_t chunk, splits;      // keys of a split (from the first key that a block of rows sees), upper bound of the splits
     float* part_o;               // [token][head][split][dim]: sums of the splits
@@ -35,7 +36,7 @@ __device__ __forceinline__ PagedRange paged_range(const PagedAttn& p, const Page
 
 // A sequence of the launch; false (reported): it contradicts itself or the stated bounds
 __device__ __forceinline__ bool paged_attention_seq(const PagedAttn& p, uint32_t s, PagedSeq* q) {
-    if (paged_seq(p.a.cache, s, p.a.tokens, q) && q->n <= p.a.max_new && q->len <= p.a.max_len) return true;
+    if (paged_seq(p.c, s, p.a.tokens, q) && q->n <= p.a.max_new && q->len <= p.a.max_len) return true;
     if (threadIdx.x == 0) atomicOr(p.err, ERR_BAD_INDEX);
     return false;
 }

@@ -80,7 +80,7 @@ __global__ void __launch_bounds__(kPtThreads) paged_tc_kernel(const PagedAttn p)
     __shared__ uint64_t q_full, k_full[kPtStages], k_empty[kPtStages], v_full[kPtStages], v_empty[kPtStages], s_full[2], p_full[2], o_full[2], drained;
     __shared__ uint32_t s_tmem;
     const lv_paged_attention_args& a = p.a;
-    const lv_paged_cache& c = a.cache;
+    const PagedCache& c = p.c;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 
     if (threadIdx.x == 0) {

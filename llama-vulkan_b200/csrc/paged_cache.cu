@@ -9,7 +9,7 @@
 namespace lv {
 
 struct PagedAppend {
-    lv_paged_cache c;
+    PagedCache c;
     const void* in[2];
     const float* angles;
     uint32_t ld, angle_ld, angle_pairs, tokens;
@@ -25,7 +25,7 @@ template <int L, int PARTS>
 __global__ void __launch_bounds__(256) paged_append_kernel(const PagedAppend p) {
     pdl_launch_dependents();
     pdl_wait();
-    const lv_paged_cache& c = p.c;
+    const PagedCache& c = p.c;
     constexpr uint32_t kHeads = kAppendRows * (32 / L);
     const uint32_t lane = threadIdx.x & 31u, H = c.kv_heads, groups = (H + kHeads - 1) / kHeads;
     const uint64_t job = uint64_t(blockIdx.x) * (blockDim.x / 32) + threadIdx.x / 32;
@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const PagedAppend p) 
 }
 
 struct PagedRead {
-    lv_paged_cache c;
+    PagedCache c;
     void* out[2];
     int out_type;
     size_t seq_stride, head_stride, row_stride;
@@ -125,28 +125,41 @@ constexpr int kReadRows = 4;
 __global__ void __launch_bounds__(256) paged_read_kernel(const PagedRead p) {
     pdl_launch_dependents();
     pdl_wait();
-    const lv_paged_cache& c = p.c;
+    const PagedCache& c = p.c;
     const uint32_t units = c.dim / 8, each = blockDim.x / units, H = c.kv_heads, s = blockIdx.z, which = blockIdx.y / H, h = blockIdx.y - which * H;
     const uint32_t len = c.lens[s], i0 = threadIdx.x / units, u = threadIdx.x - i0 * units;
     if (len > uint64_t(c.table_ld) * c.page_rows) {
         if (threadIdx.x == 0) atomicOr(p.err, ERR_BAD_INDEX);
         return;
     }
-    if (p.first >= len || i0 >= each) return;
+    if (p.first >= len || uint64_t(blockIdx.x) * each * kReadRows >= len - p.first) return;
     const uint32_t rows = min(p.rows, len - p.first);
-    const uint64_t base = uint64_t(blockIdx.x) * each * kReadRows + i0;
     const void* in = which ? c.v : c.k;
     const float* scales = which ? c.v_scale : c.k_scale;
+    // the rows of a warp, looked up by a lane each: 32 / units (rounded up) of every pass
+    const uint32_t lane = threadIdx.x & 31u, first_i0 = (threadIdx.x & ~31u) / units, span = (threadIdx.x | 31u) / units - first_i0 + 1;
     uint64_t row[kReadRows];
     bool here[kReadRows];
+    auto look_up = [&](uint32_t k, uint32_t at, uint64_t* found) {
+        const uint64_t i = uint64_t(blockIdx.x) * each * kReadRows + k * each + at;
+        if (k >= kReadRows || at >= each || i >= rows) return false;
+        if (paged_row(c, c.table + size_t(s) * c.table_ld, p.first + uint32_t(i), h, found)) return true;
+        atomicOr(p.err, ERR_BAD_INDEX);
+        return false;
+    };
+    if (kReadRows * span <= 32) {
+        uint64_t mine = 0;
+        const bool there = look_up(lane / span, first_i0 + lane % span, &mine);
+        const uint32_t all_there = __ballot_sync(0xffffffffu, there);
 #pragma unroll
-    for (int k = 0; k < kReadRows; ++k) {
-        const uint64_t i = base + k * each;
-        here[k] = i < rows;
-        if (here[k] && !paged_row(c, c.table + size_t(s) * c.table_ld, p.first + uint32_t(i), h, &row[k])) {
-            atomicOr(p.err, ERR_BAD_INDEX);
-            here[k] = false;
+        for (int k = 0; k < kReadRows; ++k) {
+            const uint32_t from = k * span + i0 - first_i0;
+            row[k] = __shfl_sync(0xffffffffu, mine, int(from));
+            here[k] = ((all_there >> from) & 1u) != 0;
         }
+    } else {                                                             // (heads of 16 values)
+#pragma unroll
+        for (int k = 0; k < kReadRows; ++k) here[k] = look_up(k, i0, &row[k]);
     }
     uint4 v[kReadRows];                                                  // eight values, or (the first two words) codes
     float f[kReadRows];
@@ -175,7 +188,7 @@ __global__ void __launch_bounds__(256) paged_read_kernel(const PagedRead p) {
             x = unpack_values4(make_uint2(v[k].x, v[k].y), c.type);
             y = unpack_values4(make_uint2(v[k].z, v[k].w), c.type);
         }
-        const size_t to = s * p.seq_stride + h * p.head_stride + (base + k * each) * p.row_stride + 8 * u;
+        const size_t to = s * p.seq_stride + h * p.head_stride + (uint64_t(blockIdx.x) * each * kReadRows + k * each + i0) * p.row_stride + 8 * u;
         if (p.out_type == LV_TYPE_F32) {
             store_values4(p.out[which], to, LV_TYPE_F32, x);
             store_values4(p.out[which], to + 4, LV_TYPE_F32, y);
@@ -195,7 +208,7 @@ extern "C" int lv_paged_locate(const lv_paged_cache* cache, const uint32_t* tabl
     LV_REQUIRE(table_row && value_index, "null argument");
     LV_REQUIRE(head < cache->kv_heads && position < uint64_t(cache->table_ld) * cache->page_rows, "paged cache: no such head or position");
     uint64_t row;
-    LV_REQUIRE(paged_row(*cache, table_row, position, head, &row), "paged cache: the table names no page of the cache there");
+    LV_REQUIRE(paged_row(paged_cache(*cache), table_row, position, head, &row), "paged cache: the table names no page of the cache there");
     *value_index = row * cache->dim;
     return LV_OK;
 }
@@ -212,7 +225,7 @@ extern "C" int lv_paged_append(lv_ctx* ctx, const lv_paged_cache* cache, const v
     LV_ENTER(ctx);
     if (!tokens) return LV_OK;
     PagedAppend p{};
-    p.c = *cache;
+    p.c = paged_cache(*cache);
     p.in[0] = k;
     p.in[1] = v;
     p.angles = angles;
@@ -241,7 +254,7 @@ extern "C" int lv_paged_read(lv_ctx* ctx, const lv_paged_cache* cache, void* k_o
     LV_ENTER(ctx);
     if (!rows) return LV_OK;
     PagedRead p{};
-    p.c = *cache;
+    p.c = paged_cache(*cache);
     p.out[0] = k_out;
     p.out[1] = v_out;
     p.out_type = out_type;

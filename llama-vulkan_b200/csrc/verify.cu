@@ -62,10 +62,12 @@ __global__ void __launch_bounds__(kProbThreads, 2) probabilities_kernel(const Pr
     const float T = p.temperature ? p.temperature[row] : 1.f;
     const float f = T == 0.f ? 1.f : 1.4426950408889634f / T;            // e^(z / T) as a power of two
     const uint32_t lo = min(p.vocab, rank * p.each), hi = min(p.vocab, lo + p.each);
-    // values i .. i + 3; those behind the end count as -inf
+    // values i .. i + 3; those behind the end count as -inf.  (Vectors first, the few values behind the last whole one in a branch of their own: the loads of
+    // several calls are on their way together.)
+    const uint32_t whole_hi = VEC ? lo + (hi - lo) / 4 * 4 : lo;
     auto load4 = [&](uint32_t i) {
         float4 v = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-        if (VEC && i + 3 < hi) return *reinterpret_cast<const float4*>(x + i);
+        if (i < whole_hi) return *reinterpret_cast<const float4*>(x + i);
         if (i < hi) v.x = x[i];
         if (i + 1 < hi) v.y = x[i + 1];
         if (i + 2 < hi) v.z = x[i + 2];
@@ -73,7 +75,7 @@ __global__ void __launch_bounds__(kProbThreads, 2) probabilities_kernel(const Pr
         return v;
     };
     auto store4 = [&](uint32_t i, const float4& v) {
-        if (VEC && i + 3 < hi) {
+        if (i < whole_hi) {
             *reinterpret_cast<float4*>(y + i) = v;
             return;
         }
@@ -96,8 +98,13 @@ __global__ void __launch_bounds__(kProbThreads, 2) probabilities_kernel(const Pr
     if constexpr (HELD) {
 #pragma unroll
         for (int k = 0; k < kProbGroups; ++k) v[k] = load4(lo + 4 * threadIdx.x + k * kStep);
+        if (T == 0.f) {
 #pragma unroll
-        for (int k = 0; k < kProbGroups; ++k) look(v[k], lo + 4 * threadIdx.x + k * kStep);
+            for (int k = 0; k < kProbGroups; ++k) look(v[k], lo + 4 * threadIdx.x + k * kStep);
+        } else {
+#pragma unroll
+            for (int k = 0; k < kProbGroups; ++k) top = fmaxf(fmaxf(top, fmaxf(v[k].x, v[k].y)), fmaxf(v[k].z, v[k].w));
+        }
     } else {
         for (uint32_t i = lo + 4 * threadIdx.x; i < hi; i += kStep) look(load4(i), i);
     }
@@ -221,8 +228,9 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const lv_verify_
     // runs of 128 values: those of this warp
     const uint32_t each = (a.vocab + 128 * kVerifyCluster * kVerifyWarps - 1) / (128 * kVerifyCluster * kVerifyWarps);
     const uint64_t lo = uint64_t(rank * kVerifyWarps + warp) * each * 128;
+    const uint32_t whole_hi = VEC ? a.vocab / 4 * 4 : 0;
     auto load4 = [&](const float* x, uint64_t i) {
-        if (VEC && i + 3 < a.vocab) return *reinterpret_cast<const float4*>(x + i);
+        if (VEC && i < whole_hi) return *reinterpret_cast<const float4*>(x + i);
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
         if (i < a.vocab) v.x = x[i];
         if (i + 1 < a.vocab) v.y = x[i + 1];
@@ -231,21 +239,37 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const lv_verify_
         return v;
     };
     struct Four { double w[4]; };
-    auto weights = [&](uint64_t i, bool rest) {
-        const float4 x = load4(p, i);
-        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (rest) y = q ? load4(q, i) : make_float4(i == drafted, i + 1 == drafted, i + 2 == drafted, i + 3 == drafted);
+    auto draft4 = [&](uint64_t i) { return q ? load4(q, i) : make_float4(i == drafted, i + 1 == drafted, i + 2 == drafted, i + 3 == drafted); };
+    auto differences = [](const float4& x, const float4& y) {
         Four f = {{double(x.x) - double(y.x), double(x.y) - double(y.y), double(x.z) - double(y.z), double(x.w) - double(y.w)}};
 #pragma unroll
         for (int k = 0; k < 4; ++k) f.w[k] = f.w[k] > 0.0 ? f.w[k] : 0.0;
         return f;
     };
+    auto weights = [&](uint64_t i, bool rest) { return differences(load4(p, i), rest ? draft4(i) : make_float4(0.f, 0.f, 0.f, 0.f)); };
     bool rest = accepted < n;
     double mine = 0.0, total = 0.0, cta0 = 0.0, cta1 = 0.0;
     for (int attempt = 0;; ++attempt) {
         mine = 0.0;
-#pragma unroll 4
-        for (uint32_t k = 0; k < each; ++k) {
+        uint32_t k = 0;
+        if (VEC && lo + 128 * each <= whole_hi) {                        // whole runs: eight loads on their way at a time
+            for (; k + 4 <= each; k += 4) {
+                float4 x[4], y[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint64_t i = lo + 128 * (k + j) + 4 * lane;
+                    x[j] = *reinterpret_cast<const float4*>(p + i);
+                    y[j] = rest && q ? *reinterpret_cast<const float4*>(q + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (rest && !q) y[j] = draft4(lo + 128 * (k + j) + 4 * lane);
+                    const Four f = differences(x[j], y[j]);
+                    mine += (f.w[0] + f.w[1]) + (f.w[2] + f.w[3]);
+                }
+            }
+        }
+        for (; k < each; ++k) {
             const Four f = weights(lo + 128 * k + 4 * lane, rest);
             mine += (f.w[0] + f.w[1]) + (f.w[2] + f.w[3]);
         }

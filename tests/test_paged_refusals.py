@@ -113,3 +113,19 @@ def test_rows_lie_where_the_table_says():
     refused(lib.lv_paged_locate(C.byref(c), row, 60, 0, C.byref(out)), "no page")          # a page that is not there
     refused(lib.lv_paged_locate(C.byref(c), row, 80, 0, C.byref(out)), "no such")          # behind the table
     refused(lib.lv_paged_locate(C.byref(c), row, 0, 8, C.byref(out)), "no such")
+
+
+@pytest.mark.parametrize("page_rows", [1, 2, 3, 5, 7, 16, 20, 100, 127, 128, 129, 641, 65535, 65537, 1000003, (1 << 30) - 1, 1 << 30, (1 << 30) + 1, (1 << 31) - 1])
+def test_positions_are_divided_exactly(page_rows):
+    """The multiplication that stands for the division by page_rows, at multiples of it, their neighbours and random positions."""
+    lib, out = pkg.load_kernels(), C.c_uint64()
+    slots = min(((1 << 31) - 1) // page_rows, 200000)
+    c = cache(pages=slots, page_rows=page_rows, kv_heads=1, dim=16, table_ld=slots)
+    table = np.arange(slots, dtype=np.uint32)
+    row = table.ctypes.data_as(C.POINTER(C.c_uint32))
+    most = slots * page_rows - 1
+    rng = np.random.default_rng(page_rows)
+    at = {0, most} | {int(m) * page_rows + e for m in rng.integers(0, slots, 300) for e in (-1, 0, 1)} | {int(p) for p in rng.integers(0, most + 1, 300)}
+    for position in (p for p in at if 0 <= p <= most):
+        assert lib.lv_paged_locate(C.byref(c), row, position, 0, C.byref(out)) == pkg.LV_OK
+        assert out.value == position * 16
