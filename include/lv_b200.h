@@ -663,7 +663,7 @@ typedef struct lv_paged_cache {
     float* k_scale;                 /* 8-bit types: f32 [pages][kv_heads][page_rows]; else unused */
     float* v_scale;
     int type;                       /* LV_TYPE_F16, LV_TYPE_BF16, LV_TYPE_I8 or LV_TYPE_E4M3 */
-    uint32_t pages, page_rows, kv_heads;
+    uint32_t pages, page_rows, kv_heads;        /* fewer than 2^32 rows in all */
     uint32_t dim;                   /* of a head: a multiple of 16, at most 256 */
     const uint32_t* table;          /* [seqs][table_ld] */
     uint32_t table_ld;

@@ -36,10 +36,10 @@ inline PagedCache paged_cache(const lv_paged_cache& c) {
     return p;
 }
 
-// Row (of k or v, and of the scales) of a head's position; false: the table names no page of the cache.  64 bits: a cache has more than 2^32 values.
-__host__ __device__ __forceinline__ bool paged_row(const PagedCache& c, const uint32_t* table_row, uint32_t position, uint32_t head, uint64_t* row) {
+// Row (of k or v, and of the scales) of a head's position; false: the table names no page of the cache.  A cache has fewer than 2^32 rows, whose bytes need 64 bits.
+__host__ __device__ __forceinline__ bool paged_row(const PagedCache& c, const uint32_t* table_row, uint32_t position, uint32_t head, uint32_t* row) {
     const uint32_t slot = uint32_t((uint64_t(position) * c.by_rows.mul) >> (31 + c.by_rows.shift)), page = slot < c.table_ld ? table_row[slot] : c.pages;
-    *row = (uint64_t(page) * c.kv_heads + head) * c.page_rows + (position - slot * c.page_rows);
+    *row = (page * c.kv_heads + head) * c.page_rows + (position - slot * c.page_rows);
     return page < c.pages;
 }
 
@@ -123,22 +123,25 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 
-// Values c .. c + 3 of a head's vector turned by a token's angles: the pairs (2 i, 2 i + 1), every product and sum rounded by itself, so that the
-// codes that a rotated key is stored as are the same wherever it is rotated
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+
+// Two pairs of a head's vector turned by {cos, sin}: every product and sum rounded by itself, so that the codes that a rotated key is stored as are the same
+// wherever it is rotated
+__device__ __forceinline__ float4 rotate4(float4 v, float2 t0, float2 t1) {
+    return make_float4(__fsub_rn(__fmul_rn(v.x, t0.x), __fmul_rn(v.y, t0.y)), __fadd_rn(__fmul_rn(v.y, t0.x), __fmul_rn(v.x, t0.y)),
+                       __fsub_rn(__fmul_rn(v.z, t1.x), __fmul_rn(v.w, t1.y)), __fadd_rn(__fmul_rn(v.w, t1.x), __fmul_rn(v.z, t1.y)));
+}
+// values c .. c + 3 by a token's angles
 __device__ __forceinline__ float4 rotate4(float4 v, const float* angles, uint32_t c, uint32_t pairs) {
-    if (c < 2 * pairs) {
-        const float2 t = *reinterpret_cast<const float2*>(angles + c);
-        const float x = v.x;
-        v.x = __fsub_rn(__fmul_rn(x, t.x), __fmul_rn(v.y, t.y));
-        v.y = __fadd_rn(__fmul_rn(v.y, t.x), __fmul_rn(x, t.y));
-    }
-    if (c + 2 < 2 * pairs) {
-        const float2 t = *reinterpret_cast<const float2*>(angles + c + 2);
-        const float z = v.z;
-        v.z = __fsub_rn(__fmul_rn(z, t.x), __fmul_rn(v.w, t.y));
-        v.w = __fadd_rn(__fmul_rn(v.w, t.x), __fmul_rn(z, t.y));
-    }
-    return v;
+    const float2 still = make_float2(1.f, 0.f);
+    const float2 t0 = c < 2 * pairs ? *reinterpret_cast<const float2*>(angles + c) : still, t1 = c + 2 < 2 * pairs ? *reinterpret_cast<const float2*>(angles + c + 2) : still;
+    const float4 u = rotate4(v, t0, t1);
+    // (a value that is not turned is not multiplied either)
+    return make_float4(c < 2 * pairs ? u.x : v.x, c < 2 * pairs ? u.y : v.y, c + 2 < 2 * pairs ? u.z : v.z, c + 2 < 2 * pairs ? u.w : v.w);
 }
 
 // What is wrong with a cache's description (LV_OK: nothing)
@@ -148,7 +151,8 @@ inline int paged_check(const lv_paged_cache* c) {
     LV_REQUIRE(!paged_is8(c->type) || (c->k_scale && c->v_scale), "paged cache: 8-bit values need scales");
     LV_REQUIRE(c->dim && c->dim % 16 == 0 && c->dim <= 256, "paged cache: head size");
     LV_REQUIRE(c->pages && c->page_rows && c->kv_heads && c->kv_heads <= 65535 && c->table_ld && c->seqs && c->seqs <= 65535, "paged cache: bad sizes");
-    LV_REQUIRE(uint64_t(c->table_ld) * c->page_rows <= 0x7fffffffull && c->pages < 0xffffffffu, "paged cache: positions of a sequence are below 2^31");
+    LV_REQUIRE(uint64_t(c->table_ld) * c->page_rows <= 0x7fffffffull, "paged cache: positions of a sequence are below 2^31");
+    LV_REQUIRE(uint64_t(c->pages) * c->page_rows <= 0xffffffffull && uint64_t(c->pages) * c->page_rows * c->kv_heads <= 0xffffffffull, "paged cache: rows are below 2^32");
     LV_REQUIRE(aligned16(c->k) && aligned16(c->v), "paged cache: k and v are 16-byte aligned");
     return LV_OK;
 }

@@ -95,7 +95,7 @@ __global__ void __launch_bounds__(32 * kPrWarps) paged_rows_kernel(const PagedAt
     // ---- the ring: slices warp, warp + 4, .. of the split ----
     uint8_t* ring = smem + S::kQ + warp * kPrStages * S::kStage;
     const uint32_t ring_at = smem_u32(ring);
-    uint64_t next_row = 0;
+    uint32_t next_row = 0;
     bool next_there = false;
     auto look_up = [&](uint32_t slice) {                                 // a lane per key
         const uint64_t j = uint64_t(lo) + uint64_t(slice) * S::kKeys + lane;
@@ -106,19 +106,22 @@ __global__ void __launch_bounds__(32 * kPrWarps) paged_rows_kernel(const PagedAt
         }
         if (!next_there) next_row = 0;
     };
+    // a lane copies the same unit of every row that is its
+    constexpr int kPer = S::kKeys * S::kUnits / 32;                      // units of keys, and of values, per lane
+    const uint32_t my_unit = lane % S::kUnits;
+    const uint8_t *my_k = static_cast<const uint8_t*>(c.k) + my_unit * 16, *my_v = static_cast<const uint8_t*>(c.v) + my_unit * 16;
+    const bool my_part = my_unit * 16 < row_bytes;
     auto issue = [&](uint32_t stage) {
         const uint32_t to = ring_at + stage * S::kStage;
         const uint32_t there = __ballot_sync(0xffffffffu, next_there);
         if (lane == 0) s_valid[warp][stage] = there;
-        constexpr int kPer = S::kKeys * S::kUnits / 32;                  // units of keys, and of values, per lane
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
-            const uint32_t at = lane + 32 * i, r = at / S::kUnits, u = at % S::kUnits;
-            const uint64_t row = __shfl_sync(0xffffffffu, next_row, int(r));
-            const bool here = ((there >> r) & 1u) != 0 && u * 16 < row_bytes;
-            const size_t from = here ? row * row_bytes + u * 16 : 0;
-            cp_async16_zfill(to + S::at(r, u), static_cast<const uint8_t*>(c.k) + from, here);
-            cp_async16_zfill(to + S::kHalf + S::at(r, u), static_cast<const uint8_t*>(c.v) + from, here);
+            const uint32_t r = (lane + 32 * i) / S::kUnits;
+            const uint64_t from = uint64_t(__shfl_sync(0xffffffffu, next_row, int(r))) * row_bytes;
+            const bool here = ((there >> r) & 1u) != 0 && my_part;
+            cp_async16_zfill(to + S::at(r, my_unit), here ? my_k + from : static_cast<const uint8_t*>(c.k), here);
+            cp_async16_zfill(to + S::kHalf + S::at(r, my_unit), here ? my_v + from : static_cast<const uint8_t*>(c.v), here);
         }
         if constexpr (S::kEight) {
             cp_async4_zfill(to + 2 * S::kHalf + 4 * lane, c.k_scale + next_row, next_there);

@@ -20,7 +20,34 @@
 
 namespace lv {
 
-constexpr int kPtSoftmax = 8, kPtLoaders = 4, kPtThreads = 32 * (kPtSoftmax + kPtLoaders + 1), kPtStages = 2;
+// Warps: eight of the softmax, four loaders, four of which one issues the products.  Registers move from the latter eight to the former: a row's 128 scores are held at a
+// time.  512 threads are launched with 128 registers each: (8 x 176 + 8 x 80) x 32 = 512 x 128.
+constexpr int kPtSoftmax = 8, kPtLoaders = 4, kPtThreads = 512, kPtStages = 2, kPtManyRegs = 176, kPtFewRegs = 80;
+
+template <int N>
+__device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+// two f32 at a time
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\tfma.rn.f32x2 z, x, y, z;\n\tmov.b64 {%0, %1}, z;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
 
 __device__ __forceinline__ void tmem_load32(uint32_t* u, uint32_t at) {
     asm volatile(
@@ -71,13 +98,13 @@ struct TcMeta {                                                          // of a
 __device__ __forceinline__ uint32_t tile_at(uint32_t r, uint32_t u) { return (u >> 3) * (128 * 128) + r * 128 + (((u & 7u) ^ (r & 7u)) << 4); }
 
 template <int KIND, int D>
-__global__ void __launch_bounds__(kPtThreads) paged_tc_kernel(const PagedAttn p) {
+__global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn p) {
     using S = TcShape<KIND, D>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023u) & ~uintptr_t(1023));
     uint8_t *s_q = smem, *s_k = smem + 2 * S::kTile, *s_v = s_k + kPtStages * S::kTile;
     __shared__ __align__(16) TcMeta meta[kPtStages];
-    __shared__ uint64_t q_full, k_full[kPtStages], k_empty[kPtStages], v_full[kPtStages], v_empty[kPtStages], s_full[2], p_full[2], o_full[2], drained;
+    __shared__ uint64_t q_full, k_full[kPtStages], k_empty[kPtStages], v_full[kPtStages], v_empty[kPtStages], s_full[2], p_full[2][2], o_full[2], drained;
     __shared__ uint32_t s_tmem;
     const lv_paged_attention_args& a = p.a;
     const PagedCache& c = p.c;
@@ -87,7 +114,7 @@ __global__ void __launch_bounds__(kPtThreads) paged_tc_kernel(const PagedAttn p)
         mbar_init(&q_full, kPtSoftmax);
         mbar_init(&drained, 1);
         for (int i = 0; i < kPtStages; ++i) { mbar_init(&k_full[i], kPtLoaders); mbar_init(&v_full[i], kPtLoaders); mbar_init(&k_empty[i], 1); mbar_init(&v_empty[i], 1); }
-        for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); mbar_init(&o_full[i], 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i][0], 4); mbar_init(&p_full[i][1], 4); mbar_init(&o_full[i], 1); }
         fence_mbar_init();
     }
     pdl_wait();
@@ -119,6 +146,7 @@ __global__ void __launch_bounds__(kPtThreads) paged_tc_kernel(const PagedAttn p)
     const uint32_t tmem_o = tmem + 256;                                  // S of the two tiles in columns 0 and 128, O in 256 and 384
 
     if (warp < kPtSoftmax) {
+        more_registers<kPtManyRegs>();
         // ---- queries, then a row per thread ---------------------------------------------------------
         const uint32_t tile = warp >> 2, quarter = warp & 3, lanes = quarter * 32u << 16;
         float row_factor = 1.f;                                          // of this thread's row
@@ -161,48 +189,42 @@ __global__ void __launch_bounds__(kPtThreads) paged_tc_kernel(const PagedAttn p)
             for (uint32_t j = 0; j < steps; ++j) {
                 const uint32_t st = j % kPtStages;
                 // (after a lost wait the warp goes through the remaining steps without work)
-                ok = ok && mbar_wait_all(&s_full[tile], j & 1u, p.err) && mbar_wait_all(&v_full[st], (j / kPtStages) & 1u, p.err);
+                ok = ok && mbar_wait_warp(&v_full[st], (j / kPtStages) & 1u, p.err) && mbar_wait_warp_tc(&s_full[tile], j & 1u, p.err);
                 if (!ok) continue;
                 tc_fence_after_sync();
                 const TcMeta& m = meta[st];
                 const int j0 = int(j * kPtKeys);
+                float2 s[kPtKeys / 2];
+                {
+                    uint32_t* u = reinterpret_cast<uint32_t*>(s);
+#pragma unroll
+                    for (int i = 0; i < kPtKeys; i += 32) tmem_load32(u + i, s_at + i);
+                    tc_wait_load();
+                }
                 const uint4 there = *reinterpret_cast<const uint4*>(m.there);
                 const bool open = (there.x & there.y & there.z & there.w) == 0xffffffffu && j0 + kPtKeys - 1 <= warp_hi && j0 >= warp_lo;
-                float s[64];
-                // the scores of keys 64 half .. + 63 without the row's factor, hidden ones -inf
-                auto scores = [&](int half) {
-                    uint32_t* u = reinterpret_cast<uint32_t*>(s);
-                    tmem_load32(u, s_at + 64 * half);
-                    tmem_load32(u + 32, s_at + 64 * half + 32);
-                    tc_wait_load();
-                    if constexpr (S::kEight) {
+                if constexpr (S::kEight) {
 #pragma unroll
-                        for (int i = 0; i < 64; i += 4) {
-                            const float4 k = *reinterpret_cast<const float4*>(&m.ks[64 * half + i]);
-                            s[i] *= k.x;
-                            s[i + 1] *= k.y;
-                            s[i + 2] *= k.z;
-                            s[i + 3] *= k.w;
-                        }
+                    for (int i = 0; i < kPtKeys / 2; i += 2) {
+                        const float4 k = *reinterpret_cast<const float4*>(&m.ks[2 * i]);
+                        s[i] = mul2(s[i], make_float2(k.x, k.y));
+                        s[i + 1] = mul2(s[i + 1], make_float2(k.z, k.w));
                     }
-                    if (!open) {
-                        const uint32_t w0 = half ? there.z : there.x, w1 = half ? there.w : there.y;
-#pragma unroll
-                        for (int i = 0; i < 64; ++i) {
-                            const int key = j0 + 64 * half + i;
-                            s[i] = (((i < 32 ? w0 : w1) >> (i & 31)) & 1u) != 0 && key <= key_hi && key >= key_lo ? s[i] : -INFINITY;
-                        }
-                    }
-                };
-                float top = -INFINITY;
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    scores(half);
-                    float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                    for (int i = 0; i < 64; ++i) t4[i & 3] = fmaxf(t4[i & 3], s[i]);
-                    top = fmaxf(top, fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])));
                 }
+                if (!open) {
+                    const uint32_t w[4] = {there.x, there.y, there.z, there.w};
+#pragma unroll
+                    for (int i = 0; i < kPtKeys / 2; ++i) {
+                        const int key = j0 + 2 * i;
+                        const uint32_t two = w[i / 16] >> ((2 * i) & 31);
+                        s[i].x = (two & 1u) != 0 && key <= key_hi && key >= key_lo ? s[i].x : -INFINITY;
+                        s[i].y = (two & 2u) != 0 && key + 1 <= key_hi && key + 1 >= key_lo ? s[i].y : -INFINITY;
+                    }
+                }
+                float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int i = 0; i < kPtKeys / 2; ++i) tops[i & 3] = fmaxf(tops[i & 3], fmaxf(s[i].x, s[i].y));
+                float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
                 if constexpr (!S::kBf16) top *= row_factor;              // (the scale over a power of two: positive)
                 float keep = 1.f;
                 bool moved = false;
@@ -233,34 +255,36 @@ __global__ void __launch_bounds__(kPtThreads) paged_tc_kernel(const PagedAttn p)
                     }
                 }
                 const float base = ref == -INFINITY ? 0.f : ref, down = S::kEight ? __uint_as_float((254u - unit) << 23) : 1.f;
-                // weights of the second half (whose scores are at hand), then of the first: 32 columns each, in the last and first quarter of the scores'
+                const float2 minus = make_float2(-base, -base), factor = make_float2(row_factor, row_factor), downs = make_float2(down, down);
+                // weights, half of the keys at a time; they take the first columns of the scores
+                float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-                for (int half = 1; half >= 0; --half) {
-                    if (half == 0) scores(0);
-                    float sums[4] = {0.f, 0.f, 0.f, 0.f};
+                for (int half = 0; half < 2; ++half) {
                     uint32_t u[32];
 #pragma unroll
-                    for (int i = 0; i < 64; i += 2) {
-                        float w0 = exp2_fast(S::kBf16 ? s[i] - base : fmaf(s[i], row_factor, -base)), w1 = exp2_fast(S::kBf16 ? s[i + 1] - base : fmaf(s[i + 1], row_factor, -base));
-                        sums[i & 3] += w0;
-                        sums[(i & 3) + 1] += w1;
+                    for (int i = 0; i < 32; ++i) {
+                        const float2 z = s[32 * half + i], x = S::kBf16 ? add2(z, minus) : fma2(z, factor, minus);
+                        float2 w = make_float2(exp2_fast(x.x), exp2_fast(x.y));
+                        sums[i & 1] = add2(sums[i & 1], w);
                         if constexpr (S::kEight) {
-                            const float2 v = *reinterpret_cast<const float2*>(&m.vs[64 * half + i]);
-                            // (a hidden key's scale may be anything)
-                            w0 = open || s[i] != -INFINITY ? w0 * (v.x * down) : 0.f;
-                            w1 = open || s[i + 1] != -INFINITY ? w1 * (v.y * down) : 0.f;
+                            const float2 v = *reinterpret_cast<const float2*>(&m.vs[64 * half + 2 * i]);
+                            w = mul2(w, mul2(v, downs));
+                            if (!open) {                                 // (a hidden key's scale may be anything)
+                                w.x = z.x != -INFINITY ? w.x : 0.f;
+                                w.y = z.y != -INFINITY ? w.y : 0.f;
+                            }
                         }
-                        u[i / 2] = pack16<S::kBf16>(w0, w1);
+                        u[i] = pack16<S::kBf16>(w.x, w.y);
                     }
-                    l += (sums[0] + sums[1]) + (sums[2] + sums[3]);
-                    tmem_store32(s_at + 96 * half, u);
+                    tmem_store32(s_at + 32 * half, u);
+                    tmem_wait_store();
+                    tc_fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&p_full[tile][half]);
                 }
-                tmem_wait_store();
-                tc_fence_before_sync();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[tile]);
+                l += (sums[0].x + sums[1].x) + (sums[0].y + sums[1].y);
             }
-            ok = ok && mbar_wait_all(&o_full[tile], 0, p.err);
+            ok = ok && mbar_wait_warp_tc(&o_full[tile], 0, p.err);
             if (ok) {
                 tc_fence_after_sync();
                 const uint32_t t = q.row0 + (r0 + row) / p.group, h = kv * p.group + (r0 + row) % p.group;
@@ -299,10 +323,11 @@ __global__ void __launch_bounds__(kPtThreads) paged_tc_kernel(const PagedAttn p)
             tc_fence_before_sync();
         }
     } else if (warp < kPtSoftmax + kPtLoaders) {
+        fewer_registers<kPtFewRegs>();
         // ---- keys and values: a warp per 32 rows of every step, a lane looks one up -------------------------
         const uint32_t part = warp - kPtSoftmax;
         const uint32_t* table = c.table + size_t(blockIdx.z) * c.table_ld;
-        uint64_t next_row = 0;
+        uint32_t next_row = 0;
         bool next_there = false;
         auto look_up = [&](uint32_t step) {
             const uint64_t j = uint64_t(lo) + uint64_t(step) * kPtKeys + 32 * part + lane;
@@ -334,37 +359,47 @@ __global__ void __launch_bounds__(kPtThreads) paged_tc_kernel(const PagedAttn p)
         if constexpr (!S::kEight) {
             constexpr uint32_t kUnits = D / 8, kPer = kUnits;            // 16-byte units of a row, and of a lane in a step
             const uint32_t row_bytes = c.dim * 2;
-            // two tiles (keys, values) a step; a tile is published while the next two are on their way
-            for (uint32_t item = 0; item < 2 * steps + 2; ++item) {
-                if (item < 2 * steps) {
-                    const uint32_t step = item >> 1, st = step % kPtStages, values = item & 1u;
+            const uint32_t my_unit = lane % kUnits;
+            const uint8_t *my_k = static_cast<const uint8_t*>(c.k) + my_unit * 16, *my_v = static_cast<const uint8_t*>(c.v) + my_unit * 16;
+            // two tiles (keys, values) a step; a tile is published while the next two are on their way, or before a wait for a place
+            uint32_t published = 0;
+            auto publish_to = [&](uint32_t end) {
+                for (; published < end; ++published) publish(published & 1u ? &v_full[(published >> 1) % kPtStages] : &k_full[(published >> 1) % kPtStages]);
+            };
+            for (uint32_t item = 0; item < 2 * steps; ++item) {
+                const uint32_t step = item >> 1, st = step % kPtStages, values = item & 1u;
+                if (step >= kPtStages) {
                     uint64_t* empty = values ? &v_empty[st] : &k_empty[st];
-                    ok = step < kPtStages || mbar_wait_all(empty, (step / kPtStages - 1) & 1u, p.err);
+                    const uint32_t phase = (step / kPtStages - 1) & 1u;
+                    if (!__any_sync(0xffffffffu, mbar_poll(empty, phase))) {
+                        cp_async_wait<0>();
+                        publish_to(item);
+                    }
+                    ok = mbar_wait_warp(empty, phase, p.err);
                     if (!ok) break;
-                    const uint32_t there = __ballot_sync(0xffffffffu, next_there);
-                    const uint32_t to = smem_u32((values ? s_v : s_k) + st * S::kTile);
-                    const uint8_t* from = static_cast<const uint8_t*>(values ? c.v : c.k);
+                }
+                const uint32_t there = __ballot_sync(0xffffffffu, next_there);
+                const uint32_t to = smem_u32((values ? s_v : s_k) + st * S::kTile);
+                const uint8_t* from = values ? my_v : my_k;
 #pragma unroll
-                    for (int i = 0; i < int(kPer); ++i) {
-                        const uint32_t at = lane + 32 * i, r = at / kUnits, u = at % kUnits;
-                        const uint64_t row = __shfl_sync(0xffffffffu, next_row, int(r));
-                        if (u * 16 >= row_bytes) continue;
-                        const bool here = ((there >> r) & 1u) != 0;
-                        cp_async16_zfill(to + tile_at(32 * part + r, u), from + (here ? row * row_bytes + u * 16 : 0), here);
-                    }
-                    if (values) {
-                        write_meta(st, there);
-                        look_up(step + 1);
-                    }
+                for (int i = 0; i < int(kPer); ++i) {
+                    const uint32_t r = (lane + 32 * i) / kUnits;
+                    const uint64_t off = uint64_t(__shfl_sync(0xffffffffu, next_row, int(r))) * row_bytes;
+                    const bool here = ((there >> r) & 1u) != 0 && my_unit * 16 < row_bytes;
+                    cp_async16_zfill(to + tile_at(32 * part + r, my_unit), here ? from + off : static_cast<const uint8_t*>(c.k), here);
+                }
+                if (values) {
+                    write_meta(st, there);
+                    look_up(step + 1);
                 }
                 cp_async_commit();
-                if (item >= 2) {
-                    const uint32_t done = item - 2, st = (done >> 1) % kPtStages;
+                if (item >= 2 && published < item - 1) {
                     cp_async_wait<2>();
-                    publish(done & 1u ? &v_full[st] : &k_full[st]);
+                    publish_to(item - 1);
                 }
             }
             cp_async_wait<0>();
+            if (ok) publish_to(2 * steps);
         } else {
             constexpr uint32_t kUnits = D / 16, kPer = kUnits;           // units of 16 codes
             uint4 code[kPer];
@@ -373,11 +408,11 @@ __global__ void __launch_bounds__(kPtThreads) paged_tc_kernel(const PagedAttn p)
 #pragma unroll
                 for (int i = 0; i < int(kPer); ++i) {
                     const uint32_t at = lane + 32 * i, r = at / kUnits, u = at % kUnits;
-                    const uint64_t row = __shfl_sync(0xffffffffu, next_row, int(r));
+                    const uint32_t row = __shfl_sync(0xffffffffu, next_row, int(r));
                     // (codes 0 of int8 are 0x80 here: their sign bits are flipped)
                     code[i] = KIND == LV_TYPE_I8 ? make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u) : make_uint4(0u, 0u, 0u, 0u);
                     if (((there >> r) & 1u) != 0 && u * 16 < c.dim) {
-                        const uint4 w = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(base) + row * c.dim + u * 16));
+                        const uint4 w = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(base) + uint64_t(row) * c.dim + u * 16));
                         code[i] = KIND == LV_TYPE_I8 ? make_uint4(w.x ^ 0x80808080u, w.y ^ 0x80808080u, w.z ^ 0x80808080u, w.w ^ 0x80808080u) : w;
                     }
                 }
@@ -397,12 +432,12 @@ __global__ void __launch_bounds__(kPtThreads) paged_tc_kernel(const PagedAttn p)
             for (uint32_t step = 0; step < steps && ok; ++step) {
                 const uint32_t st = step % kPtStages, phase = (step / kPtStages - 1) & 1u;
                 const uint32_t there = fetch(c.k);
-                ok = step < kPtStages || mbar_wait_all(&k_empty[st], phase, p.err);
+                ok = step < kPtStages || mbar_wait_warp(&k_empty[st], phase, p.err);
                 if (!ok) break;
                 convert(s_k + st * S::kTile);
                 publish(&k_full[st]);
                 fetch(c.v);
-                ok = step < kPtStages || mbar_wait_all(&v_empty[st], phase, p.err);
+                ok = step < kPtStages || mbar_wait_warp(&v_empty[st], phase, p.err);
                 if (!ok) break;
                 convert(s_v + st * S::kTile);
                 write_meta(st, there);
@@ -410,7 +445,9 @@ __global__ void __launch_bounds__(kPtThreads) paged_tc_kernel(const PagedAttn p)
                 look_up(step + 1);
             }
         }
-    } else if (lane == 0) {
+    } else {
+        fewer_registers<kPtFewRegs>();
+        if (warp != kPtSoftmax + kPtLoaders || lane != 0) goto meet;
         // ---- products ------------------------------------------------------------------------------
         constexpr uint32_t kind = (1u << 4) | (S::kBf16 ? (1u << 7) | (1u << 10) : 0u) | (uint32_t(128 >> 4) << 24);
         const uint32_t s_desc = kind | (uint32_t(kPtKeys >> 3) << 17), o_desc = kind | (1u << 16) | ((c.dim >> 3) << 17);      // (V is MN-major)
@@ -434,13 +471,16 @@ __global__ void __launch_bounds__(kPtThreads) paged_tc_kernel(const PagedAttn p)
             const uint32_t st = j % kPtStages, next = (j + 1) % kPtStages;
             ok = mbar_wait(&v_full[st], (j / kPtStages) & 1u, p.err);
             for (uint32_t tile = 0; tile < tiles && ok; ++tile) {
-                ok = mbar_wait(&p_full[tile], j & 1u, p.err);
-                if (!ok) break;
-                tc_fence_after_sync();
                 const uint64_t vd = v_desc + ((st * S::kTile) >> 4);
+                for (uint32_t half = 0; half < 2 && ok; ++half) {
+                    ok = mbar_wait(&p_full[tile][half], j & 1u, p.err);
+                    if (!ok) break;
+                    tc_fence_after_sync();
 #pragma unroll
-                for (uint32_t k = 0; k < kPtKeys / 16; ++k)              // 16 keys: 8 columns of P, two groups of eight rows of V
-                    tc_mma_f16_ta(tmem_o + tile * 128, tmem + tile * 128 + (k < 4 ? 8 * k : 64 + 8 * k), vd + 128u * k, o_desc, j != 0 || k != 0);
+                    for (uint32_t k = 0; k < kPtKeys / 32; ++k)          // 16 keys: 8 columns of P, two groups of eight rows of V
+                        tc_mma_f16_ta(tmem_o + tile * 128, tmem + tile * 128 + 32 * half + 8 * k, vd + 128u * (4 * half + k), o_desc, j != 0 || half != 0 || k != 0);
+                }
+                if (!ok) break;
                 if (tile + 1 == tiles) tc_commit(&v_empty[st]);
                 if (j + 1 == steps) {
                     tc_commit(&o_full[tile]);
@@ -457,6 +497,7 @@ __global__ void __launch_bounds__(kPtThreads) paged_tc_kernel(const PagedAttn p)
         tc_commit(&drained);
         mbar_drain(&drained, 0);
     }
+meet:
     __syncthreads();
     if (warp == kPtSoftmax + kPtLoaders) {
         tc_fence_after_sync();

@@ -13,7 +13,6 @@ struct PagedAppend {
     const void* in[2];
     const float* angles;
     uint32_t ld, angle_ld, angle_pairs, tokens;
-    int in_type;
     uint32_t* err;
 };
 
@@ -21,7 +20,8 @@ struct PagedAppend {
 // places are looked up, which is a chain of four dependent loads, once for the heads of a warp.
 // FIGURES_APPEND
 constexpr int kAppendRows = 4;
-template <int L, int PARTS>
+// IN, KIND: types of the values given and stored
+template <int IN, int KIND, int L, int PARTS>
 __global__ void __launch_bounds__(256) paged_append_kernel(const PagedAppend p) {
     pdl_launch_dependents();
     pdl_wait();
@@ -39,12 +39,12 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const PagedAppend p) 
         for (int i = 0; i < PARTS; ++i) {
             const uint32_t at = at0 + 4 * L * i, h = h0 + k * (32 / L);
             v[k][i] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (at < c.dim && h < H) v[k][i] = load_values4(p.in[which], size_t(t) * p.ld + size_t(h) * c.dim + at, p.in_type);
+            if (at < c.dim && h < H) v[k][i] = load_values4(p.in[which], size_t(t) * p.ld + size_t(h) * c.dim + at, IN);
         }
     const uint32_t s = paged_owner(c, t);
     PagedSeq q;
     if (s == c.seqs) return;
-    uint64_t row0;                                                       // of head 0
+    uint32_t row0;                                                       // of head 0
     if (!paged_seq(c, s, p.tokens, &q) || !paged_row(c, c.table + size_t(s) * c.table_ld, q.len - q.n + (t - q.row0), 0, &row0)) {
         if (lane == 0) atomicOr(p.err, ERR_BAD_INDEX);
         return;
@@ -54,57 +54,72 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const PagedAppend p) 
         for (int i = 0; i < PARTS; ++i) {
             const uint32_t at = at0 + 4 * L * i;
             if (at >= c.dim) continue;
+            if (at + 2 < 2 * p.angle_pairs) {                            // (both pairs)
+                const float2 t0 = *reinterpret_cast<const float2*>(p.angles + size_t(t) * p.angle_ld + at), t1 = *reinterpret_cast<const float2*>(p.angles + size_t(t) * p.angle_ld + at + 2);
 #pragma unroll
-            for (int k = 0; k < kAppendRows; ++k) v[k][i] = rotate4(v[k][i], p.angles + size_t(t) * p.angle_ld, at, p.angle_pairs);
+                for (int k = 0; k < kAppendRows; ++k) v[k][i] = rotate4(v[k][i], t0, t1);
+            } else {
+#pragma unroll
+                for (int k = 0; k < kAppendRows; ++k) v[k][i] = rotate4(v[k][i], p.angles + size_t(t) * p.angle_ld, at, p.angle_pairs);
+            }
         }
     }
-    void* out = which ? c.v : c.k;
-    const float top = c.type == LV_TYPE_I8 ? 127.f : 448.f;
+    constexpr bool kEight = KIND == LV_TYPE_I8 || KIND == LV_TYPE_E4M3;
+    uint8_t* out = static_cast<uint8_t*>(which ? c.v : c.k) + (uint64_t(row0 + h0 * c.page_rows) * c.dim + at0) * (kEight ? 1 : 2);
+    const size_t step = size_t(32 / L) * c.page_rows * c.dim * (kEight ? 1 : 2);
+    if constexpr (!kEight) {
 #pragma unroll
-    for (int k = 0; k < kAppendRows; ++k) {
-        const uint32_t h = h0 + k * (32 / L);
-        const uint64_t row = row0 + uint64_t(h) * c.page_rows;
-        if (!paged_is8(c.type)) {
+        for (int k = 0; k < kAppendRows; ++k)
+#pragma unroll
+            for (int i = 0; i < PARTS; ++i)
+                if (at0 + 4 * L * i < c.dim && h0 + k * (32 / L) < H) store_values4(out + k * step, 4 * L * i, KIND, v[k][i]);
+    } else {
+        constexpr float top = KIND == LV_TYPE_I8 ? 127.f : 448.f;
+        // the largest magnitudes, of each row in all its lanes: bits of non-negative numbers are in their order, NaN above all
+        float most[kAppendRows];
+#pragma unroll
+        for (int k = 0; k < kAppendRows; ++k) {
+            float m = 0.f;
+#pragma unroll
+            for (int i = 0; i < PARTS; ++i) m = max_nan(max_nan(m, max_nan(fabsf(v[k][i].x), fabsf(v[k][i].y))), max_nan(fabsf(v[k][i].z), fabsf(v[k][i].w)));
+            uint32_t u = __float_as_uint(m);
+            if constexpr (L == 32) {
+                u = __reduce_max_sync(0xffffffffu, u);
+            } else {
+#pragma unroll
+                for (int o = L / 2; o > 0; o >>= 1) u = max(u, __shfl_xor_sync(0xffffffffu, u, o));
+            }
+            most[k] = __uint_as_float(u);
+        }
+        // a lane divides for a row: the k-th of a head's lanes for its row of step k
+        static_assert(kAppendRows == 4, "");
+        const uint32_t mine = lane % L;
+        const float a = mine & 2u ? (mine & 1u ? most[3] : most[2]) : mine & 1u ? most[1] : most[0];
+        const bool fine = a < INFINITY, live = fine && a >= kPagedTiny;
+        const float f = live ? top / a : 0.f;
+        const uint32_t h_mine = h0 + mine * (32 / L);
+        if (mine < kAppendRows && h_mine < H) (which ? c.v_scale : c.k_scale)[row0 + h_mine * c.page_rows] = live ? a / top : fine ? 0.f : NAN;
+#pragma unroll
+        for (int k = 0; k < kAppendRows; ++k) {
+            const float g = __shfl_sync(0xffffffffu, f, int((lane & ~uint32_t(L - 1)) + k));
+            if (h0 + k * (32 / L) >= H) continue;
 #pragma unroll
             for (int i = 0; i < PARTS; ++i) {
-                const uint32_t at = at0 + 4 * L * i;
-                if (at < c.dim && h < H) store_values4(out, row * c.dim + at, c.type, v[k][i]);
+                if (at0 + 4 * L * i >= c.dim) continue;
+                // (rounded by themselves: a product that is fused with the sum below would round values between two codes otherwise)
+                float4 y = make_float4(__fmul_rn(v[k][i].x, g), __fmul_rn(v[k][i].y, g), __fmul_rn(v[k][i].z, g), __fmul_rn(v[k][i].w, g));
+                if (g == 0.f) y = make_float4(0.f, 0.f, 0.f, 0.f);       // (times infinity or NaN)
+                uint32_t u;
+                if constexpr (KIND == LV_TYPE_I8) {
+                    // 1.5 2^23 + y: the sum's rounding to whole numbers (ties to even) is the code's, its low byte the code
+                    constexpr float kWhole = 12582912.f;
+                    u = __byte_perm(__byte_perm(__float_as_uint(y.x + kWhole), __float_as_uint(y.y + kWhole), 0x0040), __byte_perm(__float_as_uint(y.z + kWhole), __float_as_uint(y.w + kWhole), 0x0040), 0x5410);
+                } else {
+                    u = uint32_t(__nv_cvt_float2_to_fp8x2(make_float2(y.x, y.y), __NV_SATFINITE, __NV_E4M3)) |
+                        (uint32_t(__nv_cvt_float2_to_fp8x2(make_float2(y.z, y.w), __NV_SATFINITE, __NV_E4M3)) << 16);
+                }
+                *reinterpret_cast<uint32_t*>(out + k * step + 4 * L * i) = u;
             }
-            continue;
-        }
-        // the largest magnitude by its bits, which are in the order of the numbers; infinities and NaN are above all numbers
-        uint32_t most = 0;
-#pragma unroll
-        for (int i = 0; i < PARTS; ++i) {
-            const float4 x = v[k][i];
-            most = max(most, max(max(__float_as_uint(x.x) & 0x7fffffffu, __float_as_uint(x.y) & 0x7fffffffu), max(__float_as_uint(x.z) & 0x7fffffffu, __float_as_uint(x.w) & 0x7fffffffu)));
-        }
-        if constexpr (L == 32) {
-            most = __reduce_max_sync(0xffffffffu, most);
-        } else {
-#pragma unroll
-            for (int o = L / 2; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-        }
-        const float a = __uint_as_float(most);
-        const bool fine = most < 0x7f800000u, live = fine && a >= kPagedTiny;
-        const float f = live ? top / a : 0.f;
-        if (h >= H) continue;
-        if (lane % L == 0) (which ? c.v_scale : c.k_scale)[row] = live ? a / top : fine ? 0.f : NAN;
-#pragma unroll
-        for (int i = 0; i < PARTS; ++i) {
-            const uint32_t at = at0 + 4 * L * i;
-            if (at >= c.dim) continue;
-            const float4 x = v[k][i];
-            const float4 y = live ? make_float4(x.x * f, x.y * f, x.z * f, x.w * f) : make_float4(0.f, 0.f, 0.f, 0.f);
-            uint32_t u;
-            if (c.type == LV_TYPE_I8) {
-                u = (uint32_t(__float2int_rn(y.x)) & 0xffu) | ((uint32_t(__float2int_rn(y.y)) & 0xffu) << 8) | ((uint32_t(__float2int_rn(y.z)) & 0xffu) << 16) |
-                    (uint32_t(__float2int_rn(y.w)) << 24);
-            } else {
-                u = uint32_t(__nv_cvt_float2_to_fp8x2(make_float2(y.x, y.y), __NV_SATFINITE, __NV_E4M3)) |
-                    (uint32_t(__nv_cvt_float2_to_fp8x2(make_float2(y.z, y.w), __NV_SATFINITE, __NV_E4M3)) << 16);
-            }
-            *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(out) + row * c.dim + at) = u;
         }
     }
 }
@@ -122,6 +137,7 @@ struct PagedRead {
 // sequences).
 // FIGURES_READ
 constexpr int kReadRows = 4;
+template <int KIND, int OUT>
 __global__ void __launch_bounds__(256) paged_read_kernel(const PagedRead p) {
     pdl_launch_dependents();
     pdl_wait();
@@ -138,9 +154,10 @@ __global__ void __launch_bounds__(256) paged_read_kernel(const PagedRead p) {
     const float* scales = which ? c.v_scale : c.k_scale;
     // the rows of a warp, looked up by a lane each: 32 / units (rounded up) of every pass
     const uint32_t lane = threadIdx.x & 31u, first_i0 = (threadIdx.x & ~31u) / units, span = (threadIdx.x | 31u) / units - first_i0 + 1;
-    uint64_t row[kReadRows];
+    constexpr bool kEight = KIND == LV_TYPE_I8 || KIND == LV_TYPE_E4M3;
+    uint32_t row[kReadRows];
     bool here[kReadRows];
-    auto look_up = [&](uint32_t k, uint32_t at, uint64_t* found) {
+    auto look_up = [&](uint32_t k, uint32_t at, uint32_t* found) {
         const uint64_t i = uint64_t(blockIdx.x) * each * kReadRows + k * each + at;
         if (k >= kReadRows || at >= each || i >= rows) return false;
         if (paged_row(c, c.table + size_t(s) * c.table_ld, p.first + uint32_t(i), h, found)) return true;
@@ -148,7 +165,7 @@ __global__ void __launch_bounds__(256) paged_read_kernel(const PagedRead p) {
         return false;
     };
     if (kReadRows * span <= 32) {
-        uint64_t mine = 0;
+        uint32_t mine = 0;
         const bool there = look_up(lane / span, first_i0 + lane % span, &mine);
         const uint32_t all_there = __ballot_sync(0xffffffffu, there);
 #pragma unroll
@@ -166,8 +183,8 @@ __global__ void __launch_bounds__(256) paged_read_kernel(const PagedRead p) {
 #pragma unroll
     for (int k = 0; k < kReadRows; ++k) {
         if (!here[k]) continue;
-        const size_t at = row[k] * c.dim + 8 * u;
-        if (paged_is8(c.type)) {
+        const size_t at = uint64_t(row[k]) * c.dim + 8 * u;
+        if constexpr (kEight) {
             const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(in) + at);
             v[k] = make_uint4(w.x, w.y, 0u, 0u);
             f[k] = scales[row[k]];
@@ -175,28 +192,55 @@ __global__ void __launch_bounds__(256) paged_read_kernel(const PagedRead p) {
             v[k] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(in) + at);
         }
     }
+    const size_t step = each * p.row_stride, base = s * p.seq_stride + h * p.head_stride + (uint64_t(blockIdx.x) * each * kReadRows + i0) * p.row_stride + 8 * u;
 #pragma unroll
     for (int k = 0; k < kReadRows; ++k) {
         if (!here[k]) continue;
         float4 x, y;
-        if (paged_is8(c.type)) {
-            x = code_values4(v[k].x, c.type);
-            y = code_values4(v[k].y, c.type);
+        if constexpr (kEight) {
+            x = code_values4(v[k].x, KIND);
+            y = code_values4(v[k].y, KIND);
             x = make_float4(x.x * f[k], x.y * f[k], x.z * f[k], x.w * f[k]);
             y = make_float4(y.x * f[k], y.y * f[k], y.z * f[k], y.w * f[k]);
         } else {
-            x = unpack_values4(make_uint2(v[k].x, v[k].y), c.type);
-            y = unpack_values4(make_uint2(v[k].z, v[k].w), c.type);
+            x = unpack_values4(make_uint2(v[k].x, v[k].y), KIND);
+            y = unpack_values4(make_uint2(v[k].z, v[k].w), KIND);
         }
-        const size_t to = s * p.seq_stride + h * p.head_stride + (uint64_t(blockIdx.x) * each * kReadRows + k * each + i0) * p.row_stride + 8 * u;
-        if (p.out_type == LV_TYPE_F32) {
+        const size_t to = base + k * step;
+        if constexpr (OUT == LV_TYPE_F32) {
             store_values4(p.out[which], to, LV_TYPE_F32, x);
             store_values4(p.out[which], to + 4, LV_TYPE_F32, y);
         } else {
-            const uint2 a = pack_values4(x, p.out_type), b = pack_values4(y, p.out_type);
+            const uint2 a = pack_values4(x, OUT), b = pack_values4(y, OUT);
             *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out[which]) + to) = make_uint4(a.x, a.y, b.x, b.y);
         }
     }
+}
+
+template <int IN, int KIND>
+static int append_launch(lv_ctx* ctx, const PagedAppend& p, dim3 grid) {
+    if (p.c.dim <= 64) LV_CUDA(launch_pdl(ctx, paged_append_kernel<IN, KIND, 16, 1>, grid, dim3(256), 0, p));
+    else if (p.c.dim <= 128) LV_CUDA(launch_pdl(ctx, paged_append_kernel<IN, KIND, 32, 1>, grid, dim3(256), 0, p));
+    else LV_CUDA(launch_pdl(ctx, paged_append_kernel<IN, KIND, 32, 2>, grid, dim3(256), 0, p));
+    return LV_OK;
+}
+template <int IN>
+static int append_launch_from(lv_ctx* ctx, const PagedAppend& p, dim3 grid) {
+    switch (p.c.type) {
+        case LV_TYPE_F16: return append_launch<IN, LV_TYPE_F16>(ctx, p, grid);
+        case LV_TYPE_BF16: return append_launch<IN, LV_TYPE_BF16>(ctx, p, grid);
+        case LV_TYPE_I8: return append_launch<IN, LV_TYPE_I8>(ctx, p, grid);
+        default: return append_launch<IN, LV_TYPE_E4M3>(ctx, p, grid);
+    }
+}
+template <int KIND>
+static int read_launch_from(lv_ctx* ctx, const PagedRead& p, dim3 grid) {
+    switch (p.out_type) {
+        case LV_TYPE_F32: LV_CUDA(launch_pdl(ctx, paged_read_kernel<KIND, LV_TYPE_F32>, grid, dim3(256), 0, p)); break;
+        case LV_TYPE_F16: LV_CUDA(launch_pdl(ctx, paged_read_kernel<KIND, LV_TYPE_F16>, grid, dim3(256), 0, p)); break;
+        default: LV_CUDA(launch_pdl(ctx, paged_read_kernel<KIND, LV_TYPE_BF16>, grid, dim3(256), 0, p)); break;
+    }
+    return LV_OK;
 }
 
 }  // namespace lv
@@ -207,9 +251,9 @@ extern "C" int lv_paged_locate(const lv_paged_cache* cache, const uint32_t* tabl
     if (const int rc = paged_check(cache)) return rc;
     LV_REQUIRE(table_row && value_index, "null argument");
     LV_REQUIRE(head < cache->kv_heads && position < uint64_t(cache->table_ld) * cache->page_rows, "paged cache: no such head or position");
-    uint64_t row;
+    uint32_t row;
     LV_REQUIRE(paged_row(paged_cache(*cache), table_row, position, head, &row), "paged cache: the table names no page of the cache there");
-    *value_index = row * cache->dim;
+    *value_index = uint64_t(row) * cache->dim;
     return LV_OK;
 }
 
@@ -233,13 +277,13 @@ extern "C" int lv_paged_append(lv_ctx* ctx, const lv_paged_cache* cache, const v
     p.angle_ld = angle_ld;
     p.angle_pairs = angle_pairs;
     p.tokens = tokens;
-    p.in_type = in_type;
     p.err = ctx->d_err;
     const dim3 grid(uint32_t((warps + 7) / 8));
-    if (cache->dim <= 64) LV_CUDA(launch_pdl(ctx, paged_append_kernel<16, 1>, grid, dim3(256), 0, p));
-    else if (cache->dim <= 128) LV_CUDA(launch_pdl(ctx, paged_append_kernel<32, 1>, grid, dim3(256), 0, p));
-    else LV_CUDA(launch_pdl(ctx, paged_append_kernel<32, 2>, grid, dim3(256), 0, p));
-    return LV_OK;
+    switch (in_type) {
+        case LV_TYPE_F32: return append_launch_from<LV_TYPE_F32>(ctx, p, grid);
+        case LV_TYPE_F16: return append_launch_from<LV_TYPE_F16>(ctx, p, grid);
+        default: return append_launch_from<LV_TYPE_BF16>(ctx, p, grid);
+    }
 }
 
 extern "C" int lv_paged_read(lv_ctx* ctx, const lv_paged_cache* cache, void* k_out, void* v_out, int out_type, size_t seq_stride, size_t head_stride, size_t row_stride,
@@ -264,6 +308,11 @@ extern "C" int lv_paged_read(lv_ctx* ctx, const lv_paged_cache* cache, void* k_o
     p.first = first;
     p.rows = rows;
     p.err = ctx->d_err;
-    LV_CUDA(launch_pdl(ctx, paged_read_kernel, dim3(uint32_t(blocks), 2 * cache->kv_heads, cache->seqs), dim3(256), 0, p));
-    return LV_OK;
+    const dim3 grid(uint32_t(blocks), 2 * cache->kv_heads, cache->seqs);
+    switch (cache->type) {
+        case LV_TYPE_F16: return read_launch_from<LV_TYPE_F16>(ctx, p, grid);
+        case LV_TYPE_BF16: return read_launch_from<LV_TYPE_BF16>(ctx, p, grid);
+        case LV_TYPE_I8: return read_launch_from<LV_TYPE_I8>(ctx, p, grid);
+        default: return read_launch_from<LV_TYPE_E4M3>(ctx, p, grid);
+    }
 }
