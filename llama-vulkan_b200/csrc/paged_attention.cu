@@ -18,7 +18,7 @@
 
 namespace lv {
 
-constexpr int kPrWarps = 4, kPrStages = 3;
+constexpr int kPrWarps = 4, kPrStages = 2, kPrKeys8 = 32, kPrCtas = 3, kPrRounds = 8;
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
@@ -48,7 +48,7 @@ __device__ __forceinline__ uint32_t pack16_rest(float lo, float hi, uint32_t rou
 template <int KIND, int D, bool EXACT, int MT>
 struct RowsShape {
     static constexpr bool kEight = KIND == LV_TYPE_I8 || KIND == LV_TYPE_E4M3, kBf16 = KIND == LV_TYPE_BF16;
-    static constexpr int kKeys = kEight ? 32 : 16;                       // of a slice
+    static constexpr int kKeys = kEight ? kPrKeys8 : 16;                      // of a slice
     static constexpr int kRowBytes = kEight ? D : 2 * D, kUnits = kRowBytes / 16;
     static constexpr int kHalf = kKeys * kRowBytes;                      // bytes of the keys (or values) of a slice
     static constexpr int kStage = 2 * kHalf + (kEight ? 2 * kKeys * 4 : 0);
@@ -70,8 +70,14 @@ struct RowsShape {
     }
 };
 
+// place of value d of row r where the warps' outputs meet: 16-byte units moved so that a store by eight rows and four columns falls into different banks
+__device__ __forceinline__ uint32_t merged_at(uint32_t r, uint32_t d) {
+    const uint32_t unit = d >> 2;
+    return ((unit ^ (((unit >> 3) * 2 + r) & 7u)) << 2) + (d & 3u);
+}
+
 template <int KIND, int D, bool EXACT, int MT>
-__global__ void __launch_bounds__(32 * kPrWarps) paged_rows_kernel(const PagedAttn p) {
+__global__ void __launch_bounds__(32 * kPrWarps, D <= 128 ? (MT == 1 ? kPrCtas : 2) : 1) paged_rows_kernel(const PagedAttn p) {
     using S = RowsShape<KIND, D, EXACT, MT>;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ float s_factor[S::kRows], s_ref[kPrWarps][S::kRows], s_l[kPrWarps][S::kRows];
@@ -124,8 +130,10 @@ __global__ void __launch_bounds__(32 * kPrWarps) paged_rows_kernel(const PagedAt
             cp_async16_zfill(to + S::kHalf + S::at(r, my_unit), here ? my_v + from : static_cast<const uint8_t*>(c.v), here);
         }
         if constexpr (S::kEight) {
-            cp_async4_zfill(to + 2 * S::kHalf + 4 * lane, c.k_scale + next_row, next_there);
-            cp_async4_zfill(to + 2 * S::kHalf + 4 * (S::kKeys + lane), c.v_scale + next_row, next_there);
+            if (S::kKeys == 32 || lane < S::kKeys) {
+                cp_async4_zfill(to + 2 * S::kHalf + 4 * lane, c.k_scale + next_row, next_there);
+                cp_async4_zfill(to + 2 * S::kHalf + 4 * (S::kKeys + lane), c.v_scale + next_row, next_there);
+            }
         }
     };
     const uint32_t slices = (hi - lo + S::kKeys - 1) / S::kKeys;
@@ -137,39 +145,48 @@ __global__ void __launch_bounds__(32 * kPrWarps) paged_rows_kernel(const PagedAt
         cp_async_commit();
     }
 
-    // ---- queries: rotated, divided by a power of two, in one or two 16-bit planes ----
-    for (uint32_t r = warp; r < S::kRows; r += kPrWarps) {
-        constexpr int kParts = D == 256 ? 2 : 1;
-        float4 x[kParts];
-        float top = 0.f;
-        const uint32_t t = q.row0 + (r0 + r) / p.group, h = kv * p.group + (r0 + r) % p.group;
+    // ---- queries: rotated, divided by a power of two, in one or two 16-bit planes; all of a warp's rows are asked for at once ----
+    {
+        constexpr int kParts = D == 256 ? 2 : 1, kOwn = S::kRows / kPrWarps;
+        float4 x[kOwn][kParts];
+        float2 turn[kOwn][kParts][2];
 #pragma unroll
-        for (int i = 0; i < kParts; ++i) {
-            const uint32_t d = 4 * (lane + 32 * i);
-            x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (r < rows && d < c.dim) {
-                x[i] = load_values4(a.q, size_t(t) * a.q_ld + size_t(h) * c.dim + d, a.q_type);
-                if (a.angles != nullptr) x[i] = rotate4(x[i], a.angles + size_t(t) * a.angle_ld, d, a.angle_pairs);
+        for (int k = 0; k < kOwn; ++k) {
+            const uint32_t r = warp + kPrWarps * k, t = q.row0 + (r0 + r) / p.group, h = kv * p.group + (r0 + r) % p.group;
+#pragma unroll
+            for (int i = 0; i < kParts; ++i) {
+                const uint32_t d = 4 * (lane + 32 * i);
+                const bool here = r < rows && d < c.dim;
+                x[k][i] = here ? load_values4(a.q, size_t(t) * a.q_ld + size_t(h) * c.dim + d, a.q_type) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    turn[k][i][e] = here && a.angles != nullptr && d + 2 * e < 2 * a.angle_pairs ? *reinterpret_cast<const float2*>(a.angles + size_t(t) * a.angle_ld + d + 2 * e) : make_float2(1.f, 0.f);
             }
-            top = fmaxf(fmaxf(top, fmaxf(fabsf(x[i].x), fabsf(x[i].y))), fmaxf(fabsf(x[i].z), fabsf(x[i].w)));
         }
-        float f = 1.f;                                                   // 2^-e of the largest value (f16 operands)
-        if constexpr (!S::kBf16) {
-            top = warp_max(top);
-            f = paged_row_unit(top);
-        }
-        if (lane == 0) s_factor[r] = a.scale * kPaLog2e / f;
 #pragma unroll
-        for (int i = 0; i < kParts; ++i) {
-            const uint32_t d = 4 * (lane + 32 * i);
-            if (d >= D) continue;
-            const float v[4] = {x[i].x * f, x[i].y * f, x[i].z * f, x[i].w * f};
+        for (int k = 0; k < kOwn; ++k) {
+            const uint32_t r = warp + kPrWarps * k;
+            float top = 0.f;
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const uint32_t col = S::column(d + 2 * k), at = r * (2 * D) + (((col >> 3) ^ (r & 7u)) << 4) + (col & 7u) * 2;
-                const uint32_t u = pack16<S::kBf16>(v[2 * k], v[2 * k + 1]);
-                *reinterpret_cast<uint32_t*>(smem + at) = u;
-                if constexpr (EXACT) *reinterpret_cast<uint32_t*>(smem + S::kRows * D * 2 + at) = pack16_rest<S::kBf16>(v[2 * k], v[2 * k + 1], u);
+            for (int i = 0; i < kParts; ++i) {
+                if (a.angles != nullptr) x[k][i] = rotate4(x[k][i], turn[k][i][0], turn[k][i][1]);
+                top = fmaxf(fmaxf(top, fmaxf(fabsf(x[k][i].x), fabsf(x[k][i].y))), fmaxf(fabsf(x[k][i].z), fabsf(x[k][i].w)));
+            }
+            float f = 1.f;                                               // 2^-e of the largest value (f16 operands)
+            if constexpr (!S::kBf16) f = paged_row_unit(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top))));
+            if (lane == 0) s_factor[r] = a.scale * kPaLog2e / f;
+#pragma unroll
+            for (int i = 0; i < kParts; ++i) {
+                const uint32_t d = 4 * (lane + 32 * i);
+                if (d >= D) continue;
+                const float v[4] = {x[k][i].x * f, x[k][i].y * f, x[k][i].z * f, x[k][i].w * f};
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const uint32_t col = S::column(d + 2 * e), at = r * (2 * D) + (((col >> 3) ^ (r & 7u)) << 4) + (col & 7u) * 2;
+                    const uint32_t u = pack16<S::kBf16>(v[2 * e], v[2 * e + 1]);
+                    *reinterpret_cast<uint32_t*>(smem + at) = u;
+                    if constexpr (EXACT) *reinterpret_cast<uint32_t*>(smem + S::kRows * D * 2 + at) = pack16_rest<S::kBf16>(v[2 * e], v[2 * e + 1], u);
+                }
             }
         }
     }
@@ -253,20 +270,27 @@ __global__ void __launch_bounds__(32 * kPrWarps) paged_rows_kernel(const PagedAt
                     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                         for (int k = 0; k < 4; ++k) load_q(x[plane][mt][k], plane, mt, 4 * blk + k);
+                uint32_t w[kNt][4];
 #pragma unroll
                 for (int j = 0; j < kNt; ++j) {
                     const uint4 u = *reinterpret_cast<const uint4*>(here + S::at(8 * j + quad, 4 * blk + tq));
-                    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+                    w[j][0] = u.x;
+                    w[j][1] = u.y;
+                    w[j][2] = u.z;
+                    w[j][3] = u.w;
+                }
+                // (neighbouring products belong to different sums: none waits for the one before)
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const uint32_t v = KIND == LV_TYPE_I8 ? w[k] ^ 0x80808080u : w[k];
+                for (int k = 0; k < 4; ++k)
+#pragma unroll
+                    for (int j = 0; j < kNt; ++j) {
+                        const uint32_t v = KIND == LV_TYPE_I8 ? w[j][k] ^ 0x80808080u : w[j][k];
                         const uint32_t b0 = codes_f16<KIND>(v, false), b1 = codes_f16<KIND>(v, true);
 #pragma unroll
                         for (int plane = 0; plane < S::kPlanes; ++plane)
 #pragma unroll
                             for (int mt = 0; mt < MT; ++mt) mma16<false>(s[mt][j], x[plane][mt][k], b0, b1);
                     }
-                }
             }
         }
 
@@ -301,7 +325,7 @@ __global__ void __launch_bounds__(32 * kPrWarps) paged_rows_kernel(const PagedAt
         float keep[MT][2];
         bool moved = false;
         if constexpr (S::kEight) {
-            const uint32_t mine = paged_scale_exponent(reinterpret_cast<const float*>(here + 2 * S::kHalf)[S::kKeys + lane]);
+            const uint32_t mine = paged_scale_exponent(reinterpret_cast<const float*>(here + 2 * S::kHalf)[S::kKeys + lane % S::kKeys]);
             const uint32_t top = min(max(__reduce_max_sync(0xffffffffu, mine), 1u), 253u);
             if (top > unit) {                                            // (unit 0: nothing yet, all outputs are zero)
                 const float f = paged_unit_step(unit, top);
@@ -383,7 +407,7 @@ __global__ void __launch_bounds__(32 * kPrWarps) paged_rows_kernel(const PagedAt
             }
         } else {
 #pragma unroll
-            for (int kk = 0; kk < 2; ++kk) {
+            for (int kk = 0; kk < S::kKeys / 16; ++kk) {
                 uint32_t x[S::kPlanes][MT][4];
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt)
@@ -457,17 +481,18 @@ __global__ void __launch_bounds__(32 * kPrWarps) paged_rows_kernel(const PagedAt
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            float* to = merged + (warp * S::kRows + 16 * mt + quad + 8 * i) * D;
+            const uint32_t r = 16 * mt + quad + 8 * i;
+            float* to = merged + (warp * S::kRows + r) * D;
             if constexpr (!S::kEight) {
 #pragma unroll
-                for (int j = 0; j < kOt; ++j) *reinterpret_cast<float2*>(to + 8 * j + 2 * tq) = make_float2(o[mt][j][2 * i], o[mt][j][2 * i + 1]);
+                for (int j = 0; j < kOt; ++j) *reinterpret_cast<float2*>(to + merged_at(r, 8 * j + 2 * tq)) = make_float2(o[mt][j][2 * i], o[mt][j][2 * i + 1]);
             } else {
                 constexpr int kRun = D == 64 ? 8 : 16;                   // neighbouring values of a column
 #pragma unroll
                 for (int j = 0; j < kOt; j += 4)
 #pragma unroll
                     for (int e = 0; e < 2; ++e)
-                        *reinterpret_cast<float4*>(to + j / kRun * 128 + kRun * (2 * tq + e) + j % kRun) =
+                        *reinterpret_cast<float4*>(to + merged_at(r, j / kRun * 128 + kRun * (2 * tq + e) + j % kRun)) =
                             make_float4(o[mt][j][2 * i + e] * up, o[mt][j + 1][2 * i + e] * up, o[mt][j + 2][2 * i + e] * up, o[mt][j + 3][2 * i + e] * up);
             }
         }
@@ -487,7 +512,7 @@ __global__ void __launch_bounds__(32 * kPrWarps) paged_rows_kernel(const PagedAt
 #pragma unroll
         for (int w = 0; w < kPrWarps; ++w) {
             const float f = s_ref[w][r] == -INFINITY ? 0.f : exp2_fast(s_ref[w][r] - top);
-            const float4 x = *reinterpret_cast<const float4*>(merged + (w * S::kRows + r) * D + d);
+            const float4 x = *reinterpret_cast<const float4*>(merged + (w * S::kRows + r) * D + merged_at(r, d));
             if (s_ref[w][r] == -INFINITY && s_l[w][r] == 0.f) continue;
             total = fmaf(s_l[w][r], f, total);
             v = make_float4(fmaf(x.x, f, v.x), fmaf(x.y, f, v.y), fmaf(x.z, f, v.z), fmaf(x.w, f, v.w));
@@ -523,23 +548,38 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedAttn p, uint
     const size_t part = (size_t(t) * a.heads + h) * p.splits;
     const float sink = paged_sink(p, h);
     float top = sink - kPaLift;
-    for (uint32_t i = lane; i < n; i += 32) top = fmaxf(top, p.part_rl[part + i].x);
+    float2 mine = lane < n ? p.part_rl[part + lane] : make_float2(-INFINITY, 0.f);
+    top = fmaxf(top, mine.x);
+    for (uint32_t i = lane + 32; i < n; i += 32) top = fmaxf(top, p.part_rl[part + i].x);
     top = warp_max(top);
     float4 v[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
-    float total = paged_sink_weight(sink, top);
-    for (uint32_t i = 0; i < n; ++i) {
-        const float2 rl = p.part_rl[part + i];
-        if (rl.x == -INFINITY && rl.y == 0.f) continue;
-        const float f = exp2_fast(rl.x - top);
-        total = fmaf(rl.y, f, total);
+    float total = 0.f;
+    for (uint32_t b = 0; b < n; b += 32) {
+        if (b != 0) mine = b + lane < n ? p.part_rl[part + b + lane] : make_float2(-INFINITY, 0.f);
+        // weight of this lane's split; one that saw nothing has none
+        const float mine_f = mine.x == -INFINITY ? mine.y : exp2_fast(mine.x - top);          // (0, or NaN)
+        if (!(mine.x == -INFINITY && mine.y == 0.f)) total = fmaf(mine.y, mine_f, total);
+        const uint32_t end = min(32u, n - b);
+        for (uint32_t i = 0; i < end; i += 4) {
+            float4 x[4][2];
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const uint32_t d = 4 * (lane + 32 * k);
-            if (d >= c.dim) continue;
-            const float4 x = *reinterpret_cast<const float4*>(p.part_o + (part + i) * c.dim + d);
-            v[k] = make_float4(fmaf(x.x, f, v[k].x), fmaf(x.y, f, v[k].y), fmaf(x.z, f, v[k].z), fmaf(x.w, f, v[k].w));
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const uint32_t d = 4 * (lane + 32 * k);
+                    x[e][k] = i + e < end && d < c.dim ? *reinterpret_cast<const float4*>(p.part_o + (part + b + i + e) * c.dim + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float f = __shfl_sync(0xffffffffu, mine_f, int(min(i + e, 31u)));
+                if (i + e >= end || f == 0.f) continue;
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+                    v[k] = make_float4(fmaf(x[e][k].x, f, v[k].x), fmaf(x[e][k].y, f, v[k].y), fmaf(x[e][k].z, f, v[k].z), fmaf(x[e][k].w, f, v[k].w));
+            }
         }
     }
+    total = warp_sum(total) + paged_sink_weight(sink, top);
     const float f = total == 0.f ? 0.f : 1.f / total;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
@@ -565,10 +605,9 @@ static PagedPlan paged_plan(const lv_ctx* ctx, const lv_paged_attention_args& a)
     plan.rows = plan.many ? kPtRows : rows <= 16 || a.cache.dim > 128 ? 16 : 32;
     plan.blocks = (rows + plan.rows - 1) / plan.rows;
     const uint64_t seen = a.window ? std::min<uint64_t>(a.max_len, uint64_t(a.window) + std::min(a.max_new, plan.rows)) : a.max_len;
-    const uint32_t unit = plan.many ? kPtKeys : kPrWarps * (paged_is8(a.cache.type) ? 32 : 16);
+    const uint32_t unit = plan.many ? kPtKeys : kPrWarps * (paged_is8(a.cache.type) ? kPrKeys8 : 16);
     const uint64_t ctas = uint64_t(a.cache.seqs) * a.cache.kv_heads * plan.blocks;
-    // CTAs for two per SM; with fewer than eight rounds of them the long sequences would end alone
-    const uint64_t want = plan.many ? uint64_t(ctx->sm_count) * (ctas > uint64_t(ctx->sm_count) ? 6 : 1) : 2ull * ctx->sm_count * (ctas > uint64_t(ctx->sm_count) ? 8 : 1);
+    const uint64_t want = plan.many ? uint64_t(ctx->sm_count) * (ctas > uint64_t(ctx->sm_count) ? 6 : 1) : uint64_t(kPrCtas) * ctx->sm_count * (a.cache.seqs > 1 ? kPrRounds : 1);
     uint64_t splits = std::max<uint64_t>(1, std::min<uint64_t>((want + ctas - 1) / ctas, (seen + unit - 1) / unit));
     uint64_t chunk = ((seen + splits - 1) / splits + unit - 1) / unit * unit;
     plan.chunk = uint32_t(std::max<uint64_t>(chunk, unit));
