@@ -1,16 +1,19 @@
 // Attention of many new tokens over a cache in pages, on the tcgen05 tensor cores (16-bit outputs).
 //
-// A CTA takes 256 rows -- (token, query head) pairs of one key/value head, in two tiles of 128 -- and walks their keys in steps of 128:
+// A CTA takes up to 256 rows -- (token, query head) pairs of one key/value head -- and walks their keys in steps of 128:
 //
-//   S = Q K^T          tensor memory, a tile of 128 x 128 f32 per row tile
+//   S = Q K^T          tensor memory, 128 x 128 f32
 //   P = 2^(S - r)      a row per thread; 16-bit weights go to tensor memory over the scores that they came from
 //   O += P V           P from tensor memory, V as an MN-major operand (its rows are keys)
 //
-// The two tiles take turns: the tensor cores work for one while the other's weights are computed, and each key and value is fetched once for both.  One lane issues all
-// products, in this order for every step: P V of a tile, then S of the tile's next step, so that the scores never overwrite weights that are still to be
-// read, and a finished S says that the tile's last P V has finished too.
-// Keys and values lie in pages, whose rows four warps fetch: 16-bit rows by 16-byte cp.async straight to their places in the 128-byte swizzle, 8-bit codes through
-// registers, converted to f16 on the way (exact).  Rows that no query sees are written as zeros.  References, f16 ranges and scales as in paged_attention.cu.
+// in two units that take turns: the tensor cores work for one while the other's weights are computed.  With more than 128 rows a unit is a tile of 128 of them, and each
+// key and value is fetched once for both; with fewer the units are the even and the odd steps of the same rows, each with its own O, which are added at the end.
+// One lane issues all products, in this order: P V of a unit, then the unit's next S, so that the scores never overwrite weights that are still to be
+// read, and a finished S says that the unit's last P V has finished too.
+// Keys and values lie in pages, whose rows four warps fetch: 16-bit rows by 16-byte cp.async straight to their places in the 128-byte swizzle; 8-bit codes by cp.async to a
+// ring in which every lane has places of its own, from there converted to f16 (exact).  Rows that no query sees are written as zeros.  References, f16
+// ranges and scales as in paged_attention_rows.cuh.
+// FIGURES_TC
 //
 // Every wait is bounded; one that gives up sets the error word, and the CTA drains and frees its tensor memory.
 #include <algorithm>
@@ -22,7 +25,7 @@ namespace lv {
 
 // Warps: eight of the softmax, four loaders, four of which one issues the products.  Registers move from the latter eight to the former: a row's 128 scores are held at a
 // time.  512 threads are launched with 128 registers each: (8 x 176 + 8 x 80) x 32 = 512 x 128.
-constexpr int kPtSoftmax = 8, kPtLoaders = 4, kPtThreads = 512, kPtStages = 2, kPtManyRegs = 176, kPtFewRegs = 80;
+constexpr int kPtSoftmax = 8, kPtLoaders = 4, kPtThreads = 512, kPtStages = 2, kPtRing = 3, kPtManyRegs = 176, kPtFewRegs = 80;
 
 template <int N>
 __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
@@ -80,18 +83,31 @@ __device__ __forceinline__ uint64_t values_desc(uint32_t smem_addr, uint32_t blo
     return uint64_t((smem_addr >> 4) & 0x3fffu) | (uint64_t(block >> 4) << 16) | (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) | (uint64_t(2) << 61);
 }
 
+struct TcMeta {                                                          // of a step's keys
+    float ks[kPtKeys], vs[kPtKeys];
+    uint32_t there[4], exponent[4];
+};
+struct TcShared {
+    TcMeta meta[kPtStages];
+    uint64_t k_full[kPtStages], k_empty[kPtStages], v_full[kPtStages], v_empty[kPtStages], s_full[2], p_full[2][2], o_full[2], q_full, drained;
+    float factor[kPtRows], ref[128], l[128];                             // of the rows; of the second unit of the same rows
+    uint32_t unit, tmem;
+    float ring_scales[kPtRing][kPtLoaders][32];                          // 8-bit caches: scales on their way
+    uint32_t ring_there[kPtRing][kPtLoaders];
+};
+
 template <int KIND, int D>
 struct TcShape {
     static constexpr bool kEight = KIND == LV_TYPE_I8 || KIND == LV_TYPE_E4M3, kBf16 = KIND == LV_TYPE_BF16;
     static constexpr int kBlocks = D / 64;                               // of 64 columns
     static constexpr uint32_t kBlock = 128 * 128;                        // bytes of 128 rows of one
     static constexpr uint32_t kTile = kBlocks * kBlock;                  // of a query tile, and of a step's keys or values
-    static constexpr size_t kSmem = 1024 + (2 + 2 * kPtStages) * kTile;
-};
-
-struct TcMeta {                                                          // of a step's keys
-    float ks[kPtKeys], vs[kPtKeys];
-    uint32_t there[4], exponent[4];
+    static constexpr uint32_t kRaw = kEight ? 128 * D : 0;               // of a step's codes
+    // a step's keys are free as soon as its scores are there: one place for them is enough where codes on their way need room
+    static constexpr uint32_t kKeyStages = kEight ? 1 : kPtStages;
+    // queries (two tiles), keys and values, codes
+    static constexpr uint32_t kShared = (2 + kKeyStages + kPtStages) * kTile + kPtRing * kRaw;
+    static constexpr size_t kSmem = kShared + sizeof(TcShared);
 };
 
 // byte of 16-byte unit u of row r in a tile
@@ -100,23 +116,13 @@ __device__ __forceinline__ uint32_t tile_at(uint32_t r, uint32_t u) { return (u 
 template <int KIND, int D>
 __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn p) {
     using S = TcShape<KIND, D>;
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023u) & ~uintptr_t(1023));
-    uint8_t *s_q = smem, *s_k = smem + 2 * S::kTile, *s_v = s_k + kPtStages * S::kTile;
-    __shared__ __align__(16) TcMeta meta[kPtStages];
-    __shared__ uint64_t q_full, k_full[kPtStages], k_empty[kPtStages], v_full[kPtStages], v_empty[kPtStages], s_full[2], p_full[2][2], o_full[2], drained;
-    __shared__ uint32_t s_tmem;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    uint8_t *s_q = smem, *s_k = smem + 2 * S::kTile, *s_v = s_k + S::kKeyStages * S::kTile, *s_raw = s_v + kPtStages * S::kTile;
+    TcShared& sh = *reinterpret_cast<TcShared*>(smem + S::kShared);
     const lv_paged_attention_args& a = p.a;
     const PagedCache& c = p.c;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 
-    if (threadIdx.x == 0) {
-        mbar_init(&q_full, kPtSoftmax);
-        mbar_init(&drained, 1);
-        for (int i = 0; i < kPtStages; ++i) { mbar_init(&k_full[i], kPtLoaders); mbar_init(&v_full[i], kPtLoaders); mbar_init(&k_empty[i], 1); mbar_init(&v_empty[i], 1); }
-        for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i][0], 4); mbar_init(&p_full[i][1], 4); mbar_init(&o_full[i], 1); }
-        fence_mbar_init();
-    }
     pdl_wait();
     const uint32_t split = blockIdx.x % p.splits, kv = blockIdx.y;
     PagedSeq q;
@@ -127,7 +133,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn
         pdl_launch_dependents();
         return;
     }
-    const uint32_t r0 = (n_blocks - 1 - back) * kPtRows, rows = min(uint32_t(kPtRows), all_rows - r0), tiles = rows > 128 ? 2 : 1;
+    const uint32_t r0 = (n_blocks - 1 - back) * kPtRows, rows = min(uint32_t(kPtRows), all_rows - r0);
     const PagedRange all = paged_range(p, q, r0, r0 + rows - 1);
     const uint64_t begin = uint64_t(all.lo) + uint64_t(split) * p.chunk;
     if (begin >= all.hi) {
@@ -135,64 +141,88 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn
         return;
     }
     const uint32_t lo = uint32_t(begin), hi = uint32_t(min(uint64_t(all.hi), begin + p.chunk)), steps = (hi - lo + kPtKeys - 1) / kPtKeys;
+    // unit w: tile w mod 2 of step w / 2, or (two: false) step w
+    const bool two = rows > 128;
+    const uint32_t units = two ? 2 * steps : steps;
+    auto tile_rows = [&](uint32_t unit) { return two ? (unit ? rows - 128 : 128u) : rows; };
+    if (threadIdx.x == 0) {
+        if (smem_u32(smem) & 1023u) atomicOr(p.err, ERR_BAD_INDEX);      // (the swizzle's rows begin at 1024 bytes; never seen)
+        mbar_init(&sh.q_full, kPtSoftmax);
+        mbar_init(&sh.drained, 1);
+        for (int i = 0; i < kPtStages; ++i) { mbar_init(&sh.k_full[i], kPtLoaders); mbar_init(&sh.v_full[i], kPtLoaders); mbar_init(&sh.k_empty[i], 1); mbar_init(&sh.v_empty[i], 1); }
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t warps = (tile_rows(i) + 31) / 32;             // those with rows
+            mbar_init(&sh.s_full[i], 1);
+            mbar_init(&sh.p_full[i][0], warps);
+            mbar_init(&sh.p_full[i][1], warps);
+            mbar_init(&sh.o_full[i], 1);
+        }
+        fence_mbar_init();
+    }
     if (warp == kPtSoftmax + kPtLoaders) {
-        tc_alloc(&s_tmem, 512);
+        tc_alloc(&sh.tmem, 512);
         pdl_launch_dependents();        // (not before: a CTA of the next launch could take the tensor memory that this one needs, and wait for it)
     }
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
-    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&s_tmem);
-    const uint32_t tmem_o = tmem + 256;                                  // S of the two tiles in columns 0 and 128, O in 256 and 384
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&sh.tmem);
+    const uint32_t tmem_o = tmem + 256;                                  // S of the two units in columns 0 and 128, O in 256 and 384
 
     if (warp < kPtSoftmax) {
         more_registers<kPtManyRegs>();
-        // ---- queries, then a row per thread ---------------------------------------------------------
-        const uint32_t tile = warp >> 2, quarter = warp & 3, lanes = quarter * 32u << 16;
-        float row_factor = 1.f;                                          // of this thread's row
-        for (uint32_t i = 0; i < 32; i += 4) {                           // four rows of the warp at a time
-            float4 x[4];
+        // ---- queries, a warp per sixteenth of the rows at a time, then a row per thread ----------------------
+        constexpr int kBatch = 8;
+        for (uint32_t i0 = kBatch * warp; i0 < (two ? 256u : 128u); i0 += kBatch * kPtSoftmax) {
+            float4 x[kBatch];
+            float2 turn[kBatch][2];
+            const uint32_t d = 4 * lane;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const uint32_t r = r0 + 32 * warp + i + k, t = q.row0 + r / p.group, h = kv * p.group + r % p.group, d = 4 * lane;
-                x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (r < r0 + rows && d < c.dim) x[k] = load_values4(a.q, size_t(t) * a.q_ld + size_t(h) * c.dim + d, a.q_type);
+            for (int k = 0; k < kBatch; ++k) {
+                const uint32_t r = r0 + i0 + k, t = q.row0 + r / p.group, h = kv * p.group + r % p.group;
+                const bool here = i0 + k < rows && d < c.dim;
+                x[k] = here ? load_values4(a.q, size_t(t) * a.q_ld + size_t(h) * c.dim + d, a.q_type) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    turn[k][e] = here && a.angles != nullptr && d + 2 * e < 2 * a.angle_pairs ? *reinterpret_cast<const float2*>(a.angles + size_t(t) * a.angle_ld + d + 2 * e) : make_float2(1.f, 0.f);
             }
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const uint32_t r = r0 + 32 * warp + i + k, t = q.row0 + r / p.group, d = 4 * lane, at_row = 32 * quarter + i + k;
-                if (a.angles != nullptr && r < r0 + rows && d < c.dim) x[k] = rotate4(x[k], a.angles + size_t(t) * a.angle_ld, d, a.angle_pairs);
+            for (int k = 0; k < kBatch; ++k) {
+                if (a.angles != nullptr) x[k] = rotate4(x[k], turn[k][0], turn[k][1]);
                 float f = a.scale * kPaLog2e;
                 if constexpr (!S::kBf16) {
-                    const float u = paged_row_unit(warp_max(fmaxf(fmaxf(fabsf(x[k].x), fabsf(x[k].y)), fmaxf(fabsf(x[k].z), fabsf(x[k].w)))));
-                    if (i + k == uint32_t(lane)) row_factor = f / u;
+                    const float top = fmaxf(fmaxf(fabsf(x[k].x), fabsf(x[k].y)), fmaxf(fabsf(x[k].z), fabsf(x[k].w)));
+                    const float u = paged_row_unit(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top))));
+                    if (lane == 0) sh.factor[i0 + k] = f / u;
                     f = u;
                 }
-                if (d < D) *reinterpret_cast<uint2*>(s_q + tile * S::kTile + tile_at(at_row, d >> 3) + (d & 4u) * 2) =
+                if (d < D) *reinterpret_cast<uint2*>(s_q + ((i0 + k) >> 7) * S::kTile + tile_at((i0 + k) & 127u, d >> 3) + (d & 4u) * 2) =
                     make_uint2(pack16<S::kBf16>(x[k].x * f, x[k].y * f), pack16<S::kBf16>(x[k].z * f, x[k].w * f));
             }
         }
         fence_proxy_async();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&q_full);
-        if (tile < tiles) {
-            const uint32_t row = 128 * tile + 32 * quarter + lane, before = q.len - q.n;
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * kPtSoftmax) : "memory");
+        if (lane == 0) mbar_arrive(&sh.q_full);
+        const uint32_t mine = warp >> 2, quarter = warp & 3, lanes = quarter * 32u << 16;
+        const uint32_t base_row = two ? 128 * mine : 0, row = base_row + 32 * quarter + lane, before = q.len - q.n;
+        const uint32_t s_at = tmem + lanes + mine * 128, o_at = tmem_o + lanes + mine * 128;
+        float ref = -INFINITY, l = 0.f;
+        uint32_t unit = 0;
+        bool ok = true;
+        if (base_row + 32 * quarter < rows) {
+            const float row_factor = S::kBf16 ? 1.f : sh.factor[row];
             const uint32_t pos = before + (r0 + min(row, rows - 1)) / p.group;
             const int key_hi = row < rows ? int(pos) - int(lo) : -1, key_lo = int(paged_first_key(pos, a.window)) - int(lo);
             // keys that every row of the warp sees
-            const uint32_t w0 = r0 + min(128 * tile + 32 * quarter, rows - 1), w1 = r0 + min(128 * tile + 32 * quarter + 31, rows - 1);
-            const int warp_hi = int(before + w0 / p.group) - int(lo), warp_lo = int(paged_first_key(before + w1 / p.group, a.window)) - int(lo);
-            const uint32_t s_at = tmem + lanes + tile * 128, o_at = tmem_o + lanes + tile * 128;
-            float ref = -INFINITY, l = 0.f;
-            uint32_t unit = 0;
-            bool ok = true;
-            for (uint32_t j = 0; j < steps; ++j) {
-                const uint32_t st = j % kPtStages;
+            const uint32_t first = r0 + base_row + 32 * quarter, last = r0 + min(base_row + 32 * quarter + 31, rows - 1);
+            const int warp_hi = int(before + first / p.group) - int(lo), warp_lo = int(paged_first_key(before + last / p.group, a.window)) - int(lo);
+            for (uint32_t w = mine; w < units; w += 2) {
+                const uint32_t turn = w >> 1, j = two ? turn : w, st = j % kPtStages;
                 // (after a lost wait the warp goes through the remaining steps without work)
-                ok = ok && mbar_wait_warp(&v_full[st], (j / kPtStages) & 1u, p.err) && mbar_wait_warp_tc(&s_full[tile], j & 1u, p.err);
+                ok = ok && mbar_wait_warp(&sh.v_full[st], (j / kPtStages) & 1u, p.err) && mbar_wait_warp_tc(&sh.s_full[mine], turn & 1u, p.err);
                 if (!ok) continue;
                 tc_fence_after_sync();
-                const TcMeta& m = meta[st];
+                const TcMeta& m = sh.meta[st];
                 const int j0 = int(j * kPtKeys);
                 float2 s[kPtKeys / 2];
                 {
@@ -212,13 +242,13 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn
                     }
                 }
                 if (!open) {
-                    const uint32_t w[4] = {there.x, there.y, there.z, there.w};
+                    const uint32_t bits[4] = {there.x, there.y, there.z, there.w};
 #pragma unroll
                     for (int i = 0; i < kPtKeys / 2; ++i) {
                         const int key = j0 + 2 * i;
-                        const uint32_t two = w[i / 16] >> ((2 * i) & 31);
-                        s[i].x = (two & 1u) != 0 && key <= key_hi && key >= key_lo ? s[i].x : -INFINITY;
-                        s[i].y = (two & 2u) != 0 && key + 1 <= key_hi && key + 1 >= key_lo ? s[i].y : -INFINITY;
+                        const uint32_t pair = bits[i / 16] >> ((2 * i) & 31);
+                        s[i].x = (pair & 1u) != 0 && key <= key_hi && key >= key_lo ? s[i].x : -INFINITY;
+                        s[i].y = (pair & 2u) != 0 && key + 1 <= key_hi && key + 1 >= key_lo ? s[i].y : -INFINITY;
                     }
                 }
                 float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -244,7 +274,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn
                     ref = next;
                     moved = true;
                 }
-                if (j != 0 && __any_sync(0xffffffffu, moved)) {          // (S of this step is there, so P V of the last one has ended)
+                if (turn != 0 && __any_sync(0xffffffffu, moved)) {       // (S of this step is there, so the unit's last P V has ended)
                     for (uint32_t d = 0; d < c.dim; d += 16) {
                         uint32_t u[16];
                         tc_load16(u, o_at + d);
@@ -264,64 +294,90 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn
 #pragma unroll
                     for (int i = 0; i < 32; ++i) {
                         const float2 z = s[32 * half + i], x = S::kBf16 ? add2(z, minus) : fma2(z, factor, minus);
-                        float2 w = make_float2(exp2_fast(x.x), exp2_fast(x.y));
-                        sums[i & 1] = add2(sums[i & 1], w);
+                        float2 e = make_float2(exp2_fast(x.x), exp2_fast(x.y));
+                        sums[i & 1] = add2(sums[i & 1], e);
                         if constexpr (S::kEight) {
                             const float2 v = *reinterpret_cast<const float2*>(&m.vs[64 * half + 2 * i]);
-                            w = mul2(w, mul2(v, downs));
+                            e = mul2(e, mul2(v, downs));
                             if (!open) {                                 // (a hidden key's scale may be anything)
-                                w.x = z.x != -INFINITY ? w.x : 0.f;
-                                w.y = z.y != -INFINITY ? w.y : 0.f;
+                                e.x = z.x != -INFINITY ? e.x : 0.f;
+                                e.y = z.y != -INFINITY ? e.y : 0.f;
                             }
                         }
-                        u[i] = pack16<S::kBf16>(w.x, w.y);
+                        u[i] = pack16<S::kBf16>(e.x, e.y);
                     }
                     tmem_store32(s_at + 32 * half, u);
                     tmem_wait_store();
                     tc_fence_before_sync();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&p_full[tile][half]);
+                    if (lane == 0) mbar_arrive(&sh.p_full[mine][half]);
                 }
                 l += (sums[0].x + sums[1].x) + (sums[0].y + sums[1].y);
             }
-            ok = ok && mbar_wait_warp_tc(&o_full[tile], 0, p.err);
-            if (ok) {
-                tc_fence_after_sync();
-                const uint32_t t = q.row0 + (r0 + row) / p.group, h = kv * p.group + (r0 + row) % p.group;
-                const bool mine = row < rows, whole = p.splits == 1;
-                float f = S::kEight ? __uint_as_float(max(unit, 1u) << 23) : 1.f;
-                const size_t part = (size_t(t) * a.heads + h) * p.splits + split, to = size_t(t) * a.out_ld + size_t(h) * c.dim;
-                if (whole) {
-                    const float sink = mine ? paged_sink(p, h) : -INFINITY, top = fmaxf(ref, sink - kPaLift);
-                    const float g = ref == -INFINITY ? 0.f : exp2_fast(ref - top), total = fmaf(l, g, paged_sink_weight(sink, top));
-                    f = total == 0.f ? 0.f : f * g / total;
-                } else if (mine) {
-                    p.part_rl[part] = make_float2(ref, l);
+            if (mine < units) ok = ok && mbar_wait_warp_tc(&sh.o_full[mine], 0, p.err);
+        }
+        float2 part1 = make_float2(-INFINITY, 0.f);                      // reference and sum of the other unit of the same rows
+        uint32_t unit1 = 0;
+        if (!two) {
+            if (mine == 1) {
+                sh.ref[32 * quarter + lane] = ref;
+                sh.l[32 * quarter + lane] = l;
+                if (warp == 4 && lane == 0) sh.unit = unit;              // (the same in all warps that have rows)
+            }
+            asm volatile("bar.sync 1, %0;" ::"n"(32 * kPtSoftmax) : "memory");
+            if (mine == 0) {
+                part1 = make_float2(sh.ref[32 * quarter + lane], sh.l[32 * quarter + lane]);
+                unit1 = sh.unit;
+            }
+        }
+        if (ok && base_row + 32 * quarter < rows && (two || mine == 0)) {
+            tc_fence_after_sync();
+            const uint32_t t = q.row0 + (r0 + row) / p.group, h = kv * p.group + (r0 + row) % p.group;
+            const bool inside = row < rows, whole = p.splits == 1;
+            const size_t part = (size_t(t) * a.heads + h) * p.splits + split, to = size_t(t) * a.out_ld + size_t(h) * c.dim;
+            const bool none0 = ref == -INFINITY && l == 0.f, none1 = part1.x == -INFINITY && part1.y == 0.f;
+            const float sink = whole && inside ? paged_sink(p, h) : -INFINITY, top = fmaxf(fmaxf(ref, part1.x), sink - kPaLift);
+            float f0 = ref == -INFINITY ? 0.f : exp2_fast(ref - top), f1 = part1.x == -INFINITY ? 0.f : exp2_fast(part1.x - top);
+            float total = (none0 ? 0.f : l * f0) + (none1 ? 0.f : part1.y * f1);
+            if (whole) {
+                total += paged_sink_weight(sink, top);
+                const float g = total == 0.f ? 0.f : 1.f / total;
+                f0 *= g;
+                f1 *= g;
+            } else if (inside) {
+                p.part_rl[part] = make_float2(top, total);
+            }
+            if constexpr (S::kEight) {
+                f0 *= __uint_as_float(max(unit, 1u) << 23);
+                f1 *= __uint_as_float(max(unit1, 1u) << 23);
+            }
+            const bool other = !two && units > 1;
+            for (uint32_t d = 0; d < c.dim; d += 16) {
+                uint32_t u[16], u1[16];
+                tc_load16(u, o_at + d);
+                if (other) tc_load16(u1, o_at + 128 + d);
+                tc_wait_load();
+                if (!inside) continue;
+                float v[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    v[i] = none0 ? 0.f : __uint_as_float(u[i]) * f0;
+                    if (other && !none1) v[i] = fmaf(__uint_as_float(u1[i]), f1, v[i]);
                 }
-                const bool none = ref == -INFINITY && l == 0.f;
-                for (uint32_t d = 0; d < c.dim; d += 16) {
-                    uint32_t u[16];
-                    tc_load16(u, o_at + d);
-                    tc_wait_load();
-                    if (!mine) continue;
-                    float v[16];
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) v[i] = none ? 0.f : __uint_as_float(u[i]) * f;
-#pragma unroll
-                    for (int i = 0; i < 16; i += 8) {
-                        const float4 x = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]), y = make_float4(v[i + 4], v[i + 5], v[i + 6], v[i + 7]);
-                        if (whole) {
-                            const uint2 xx = pack_values4(x, a.out_type), yy = pack_values4(y, a.out_type);
-                            *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + to + d + i) = make_uint4(xx.x, xx.y, yy.x, yy.y);
-                        } else {
-                            *reinterpret_cast<float4*>(p.part_o + part * c.dim + d + i) = x;
-                            *reinterpret_cast<float4*>(p.part_o + part * c.dim + d + i + 4) = y;
-                        }
+                for (int i = 0; i < 16; i += 8) {
+                    const float4 x = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]), y = make_float4(v[i + 4], v[i + 5], v[i + 6], v[i + 7]);
+                    if (whole) {
+                        const uint2 xx = pack_values4(x, a.out_type), yy = pack_values4(y, a.out_type);
+                        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + to + d + i) = make_uint4(xx.x, xx.y, yy.x, yy.y);
+                    } else {
+                        *reinterpret_cast<float4*>(p.part_o + part * c.dim + d + i) = x;
+                        *reinterpret_cast<float4*>(p.part_o + part * c.dim + d + i + 4) = y;
                     }
                 }
             }
-            tc_fence_before_sync();
         }
+        tc_fence_before_sync();
     } else if (warp < kPtSoftmax + kPtLoaders) {
         fewer_registers<kPtFewRegs>();
         // ---- keys and values: a warp per 32 rows of every step, a lane looks one up -------------------------
@@ -343,33 +399,22 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn
             __syncwarp();
             if (lane == 0) mbar_arrive(bar);
         };
-        auto write_meta = [&](uint32_t st, uint32_t there) {
-            TcMeta& m = meta[st];
-            if constexpr (S::kEight) {
-                const float ks = next_there ? c.k_scale[next_row] : 0.f, vs = next_there ? c.v_scale[next_row] : 0.f;
-                m.ks[32 * part + lane] = ks;
-                m.vs[32 * part + lane] = vs;
-                const uint32_t e = __reduce_max_sync(0xffffffffu, paged_scale_exponent(vs));
-                if (lane == 0) m.exponent[part] = e;
-            }
-            if (lane == 0) m.there[part] = there;
-        };
         bool ok = true;
         look_up(0);
+        // items: keys of a step, then its values
         if constexpr (!S::kEight) {
             constexpr uint32_t kUnits = D / 8, kPer = kUnits;            // 16-byte units of a row, and of a lane in a step
-            const uint32_t row_bytes = c.dim * 2;
-            const uint32_t my_unit = lane % kUnits;
+            const uint32_t row_bytes = c.dim * 2, my_unit = lane % kUnits;
             const uint8_t *my_k = static_cast<const uint8_t*>(c.k) + my_unit * 16, *my_v = static_cast<const uint8_t*>(c.v) + my_unit * 16;
-            // two tiles (keys, values) a step; a tile is published while the next two are on their way, or before a wait for a place
+            // a tile is published while the next two are on their way, or before a wait for a place
             uint32_t published = 0;
             auto publish_to = [&](uint32_t end) {
-                for (; published < end; ++published) publish(published & 1u ? &v_full[(published >> 1) % kPtStages] : &k_full[(published >> 1) % kPtStages]);
+                for (; published < end; ++published) publish(published & 1u ? &sh.v_full[(published >> 1) % kPtStages] : &sh.k_full[(published >> 1) % kPtStages]);
             };
             for (uint32_t item = 0; item < 2 * steps; ++item) {
                 const uint32_t step = item >> 1, st = step % kPtStages, values = item & 1u;
                 if (step >= kPtStages) {
-                    uint64_t* empty = values ? &v_empty[st] : &k_empty[st];
+                    uint64_t* empty = values ? &sh.v_empty[st] : &sh.k_empty[st];
                     const uint32_t phase = (step / kPtStages - 1) & 1u;
                     if (!__any_sync(0xffffffffu, mbar_poll(empty, phase))) {
                         cp_async_wait<0>();
@@ -389,7 +434,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn
                     cp_async16_zfill(to + tile_at(32 * part + r, my_unit), here ? from + off : static_cast<const uint8_t*>(c.k), here);
                 }
                 if (values) {
-                    write_meta(st, there);
+                    if (lane == 0) sh.meta[st].there[part] = there;
                     look_up(step + 1);
                 }
                 cp_async_commit();
@@ -402,48 +447,65 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn
             if (ok) publish_to(2 * steps);
         } else {
             constexpr uint32_t kUnits = D / 16, kPer = kUnits;           // units of 16 codes
-            uint4 code[kPer];
-            auto fetch = [&](const void* base) {
-                const uint32_t there = __ballot_sync(0xffffffffu, next_there);
+            const uint32_t my_unit = lane % kUnits;
+            const uint8_t *my_k = static_cast<const uint8_t*>(c.k) + my_unit * 16, *my_v = static_cast<const uint8_t*>(c.v) + my_unit * 16;
+            // place of this lane's codes in the ring
+            auto ring = [&](uint32_t slot) { return s_raw + slot * S::kRaw + part * (S::kRaw / 4) + lane * 16; };
+            float key_scale = 0.f;
+            auto issue = [&](uint32_t item) {
+                if (item < 2 * steps) {
+                    const uint32_t slot = item % kPtRing, values = item & 1u, there = __ballot_sync(0xffffffffu, next_there);
+                    const uint32_t to = smem_u32(ring(slot));
+                    const uint8_t* from = values ? my_v : my_k;
 #pragma unroll
-                for (int i = 0; i < int(kPer); ++i) {
-                    const uint32_t at = lane + 32 * i, r = at / kUnits, u = at % kUnits;
-                    const uint32_t row = __shfl_sync(0xffffffffu, next_row, int(r));
-                    // (codes 0 of int8 are 0x80 here: their sign bits are flipped)
-                    code[i] = KIND == LV_TYPE_I8 ? make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u) : make_uint4(0u, 0u, 0u, 0u);
-                    if (((there >> r) & 1u) != 0 && u * 16 < c.dim) {
-                        const uint4 w = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(base) + uint64_t(row) * c.dim + u * 16));
-                        code[i] = KIND == LV_TYPE_I8 ? make_uint4(w.x ^ 0x80808080u, w.y ^ 0x80808080u, w.z ^ 0x80808080u, w.w ^ 0x80808080u) : w;
+                    for (int i = 0; i < int(kPer); ++i) {
+                        const uint32_t r = (lane + 32 * i) / kUnits;
+                        const uint64_t off = uint64_t(__shfl_sync(0xffffffffu, next_row, int(r))) * c.dim;
+                        const bool here = ((there >> r) & 1u) != 0 && my_unit * 16 < c.dim;
+                        cp_async16_zfill(to + 512 * i, here ? from + off : static_cast<const uint8_t*>(c.k), here);
                     }
+                    cp_async4_zfill(smem_u32(&sh.ring_scales[slot][part][lane]), (values ? c.v_scale : c.k_scale) + next_row, next_there);
+                    if (lane == 0) sh.ring_there[slot][part] = there;
+                    if (values) look_up((item >> 1) + 1);
                 }
-                return there;
+                cp_async_commit();
             };
-            auto convert = [&](uint8_t* to) {
+            for (uint32_t item = 0; item < kPtRing; ++item) issue(item);
+            for (uint32_t item = 0; item < 2 * steps; ++item) {
+                const uint32_t step = item >> 1, values = item & 1u, slot = item % kPtRing, stages = values ? kPtStages : S::kKeyStages, st = step % stages;
+                cp_async_wait<kPtRing - 1>();
+                if (step >= stages) ok = mbar_wait_warp(values ? &sh.v_empty[st] : &sh.k_empty[st], (step / stages - 1) & 1u, p.err);
+                if (!ok) break;
+                const uint8_t* from = ring(slot);
+                uint8_t* to = (values ? s_v : s_k) + st * S::kTile;
 #pragma unroll
                 for (int i = 0; i < int(kPer); ++i) {
-                    const uint32_t at = lane + 32 * i, r = at / kUnits, u = at % kUnits;
-                    const uint4 w = code[i];
-                    *reinterpret_cast<uint4*>(to + tile_at(32 * part + r, 2 * u)) =
+                    const uint32_t r = (lane + 32 * i) / kUnits;
+                    uint4 w = *reinterpret_cast<const uint4*>(from + 512 * i);
+                    if constexpr (KIND == LV_TYPE_I8) w = make_uint4(w.x ^ 0x80808080u, w.y ^ 0x80808080u, w.z ^ 0x80808080u, w.w ^ 0x80808080u);
+                    *reinterpret_cast<uint4*>(to + tile_at(32 * part + r, 2 * my_unit)) =
                         make_uint4(codes_f16<KIND>(w.x, false), codes_f16<KIND>(w.x, true), codes_f16<KIND>(w.y, false), codes_f16<KIND>(w.y, true));
-                    *reinterpret_cast<uint4*>(to + tile_at(32 * part + r, 2 * u + 1)) =
+                    *reinterpret_cast<uint4*>(to + tile_at(32 * part + r, 2 * my_unit + 1)) =
                         make_uint4(codes_f16<KIND>(w.z, false), codes_f16<KIND>(w.z, true), codes_f16<KIND>(w.w, false), codes_f16<KIND>(w.w, true));
                 }
-            };
-            for (uint32_t step = 0; step < steps && ok; ++step) {
-                const uint32_t st = step % kPtStages, phase = (step / kPtStages - 1) & 1u;
-                const uint32_t there = fetch(c.k);
-                ok = step < kPtStages || mbar_wait_warp(&k_empty[st], phase, p.err);
-                if (!ok) break;
-                convert(s_k + st * S::kTile);
-                publish(&k_full[st]);
-                fetch(c.v);
-                ok = step < kPtStages || mbar_wait_warp(&v_empty[st], phase, p.err);
-                if (!ok) break;
-                convert(s_v + st * S::kTile);
-                write_meta(st, there);
-                publish(&v_full[st]);
-                look_up(step + 1);
+                // (a step's scales: those of the keys wait in a register for the place that the values' wait has made free)
+                const float scale = sh.ring_scales[slot][part][lane];
+                TcMeta& m = sh.meta[st];
+                if (values) {
+                    m.vs[32 * part + lane] = scale;
+                    m.ks[32 * part + lane] = key_scale;
+                    const uint32_t e = __reduce_max_sync(0xffffffffu, paged_scale_exponent(scale));
+                    if (lane == 0) {
+                        m.exponent[part] = e;
+                        m.there[part] = sh.ring_there[slot][part];
+                    }
+                } else {
+                    key_scale = scale;
+                }
+                publish(values ? &sh.v_full[st] : &sh.k_full[st]);
+                issue(item + kPtRing);
             }
+            cp_async_wait<0>();
         }
     } else {
         fewer_registers<kPtFewRegs>();
@@ -453,49 +515,40 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn
         const uint32_t s_desc = kind | (uint32_t(kPtKeys >> 3) << 17), o_desc = kind | (1u << 16) | ((c.dim >> 3) << 17);      // (V is MN-major)
         const uint64_t q_desc = tc_smem_desc(smem_u32(s_q)), k_desc = tc_smem_desc(smem_u32(s_k)), v_desc = values_desc(smem_u32(s_v), S::kBlock);
         const uint32_t k_steps = c.dim / 16;
-        auto scores = [&](uint32_t tile, uint32_t j) {
-            const uint64_t qd = q_desc + ((tile * S::kTile) >> 4), kd = k_desc + (((j % kPtStages) * S::kTile) >> 4);
+        bool ok = mbar_wait(&sh.q_full, 0, p.err);
+        auto scores = [&](uint32_t w) {
+            const uint32_t tile = w & 1u, j = two ? w >> 1 : w, st = j % S::kKeyStages;
+            if (!two || tile == 0) ok = ok && mbar_wait(&sh.k_full[st], (j / S::kKeyStages) & 1u, p.err);
+            if (!ok) return;
+            tc_fence_after_sync();
+            const uint64_t qd = q_desc + ((two && tile ? S::kTile : 0u) >> 4), kd = k_desc + ((st * S::kTile) >> 4);
             for (uint32_t k = 0; k < k_steps; ++k) {
                 const uint32_t off = (((k >> 2) * S::kBlock) >> 4) + (k & 3u) * 2;
                 tc_mma_f16(tmem + tile * 128, qd + off, kd + off, s_desc, k != 0);
             }
-            tc_commit(&s_full[tile]);
-            if (tile + 1 == tiles) tc_commit(&k_empty[j % kPtStages]);
+            tc_commit(&sh.s_full[tile]);
+            if (!two || tile == 1) tc_commit(&sh.k_empty[st]);
         };
-        bool ok = mbar_wait(&q_full, 0, p.err) && mbar_wait(&k_full[0], 0, p.err);
-        if (ok) {
-            tc_fence_after_sync();
-            for (uint32_t tile = 0; tile < tiles; ++tile) scores(tile, 0);
-        }
-        for (uint32_t j = 0; j < steps && ok; ++j) {
-            const uint32_t st = j % kPtStages, next = (j + 1) % kPtStages;
-            ok = mbar_wait(&v_full[st], (j / kPtStages) & 1u, p.err);
-            for (uint32_t tile = 0; tile < tiles && ok; ++tile) {
-                const uint64_t vd = v_desc + ((st * S::kTile) >> 4);
-                for (uint32_t half = 0; half < 2 && ok; ++half) {
-                    ok = mbar_wait(&p_full[tile][half], j & 1u, p.err);
-                    if (!ok) break;
-                    tc_fence_after_sync();
-#pragma unroll
-                    for (uint32_t k = 0; k < kPtKeys / 32; ++k)          // 16 keys: 8 columns of P, two groups of eight rows of V
-                        tc_mma_f16_ta(tmem_o + tile * 128, tmem + tile * 128 + 32 * half + 8 * k, vd + 128u * (4 * half + k), o_desc, j != 0 || half != 0 || k != 0);
-                }
+        for (uint32_t w = 0; w < min(units, 2u) && ok; ++w) scores(w);
+        for (uint32_t w = 0; w < units && ok; ++w) {
+            const uint32_t tile = w & 1u, turn = w >> 1, j = two ? turn : w, st = j % kPtStages;
+            if (!two || tile == 0) ok = mbar_wait(&sh.v_full[st], (j / kPtStages) & 1u, p.err);
+            const uint64_t vd = v_desc + ((st * S::kTile) >> 4);
+            for (uint32_t half = 0; half < 2 && ok; ++half) {
+                ok = mbar_wait(&sh.p_full[tile][half], turn & 1u, p.err);
                 if (!ok) break;
-                if (tile + 1 == tiles) tc_commit(&v_empty[st]);
-                if (j + 1 == steps) {
-                    tc_commit(&o_full[tile]);
-                } else {
-                    if (tile == 0) {
-                        ok = mbar_wait(&k_full[next], ((j + 1) / kPtStages) & 1u, p.err);
-                        if (!ok) break;
-                        tc_fence_after_sync();
-                    }
-                    scores(tile, j + 1);
-                }
+                tc_fence_after_sync();
+#pragma unroll
+                for (uint32_t k = 0; k < kPtKeys / 32; ++k)              // 16 keys: 8 columns of P, two groups of eight rows of V
+                    tc_mma_f16_ta(tmem_o + tile * 128, tmem + tile * 128 + 32 * half + 8 * k, vd + 128u * (4 * half + k), o_desc, turn != 0 || half != 0 || k != 0);
             }
+            if (!ok) break;
+            if (!two || tile == 1) tc_commit(&sh.v_empty[st]);
+            if (w + 2 < units) scores(w + 2);
+            else tc_commit(&sh.o_full[tile]);
         }
-        tc_commit(&drained);
-        mbar_drain(&drained, 0);
+        tc_commit(&sh.drained);
+        mbar_drain(&sh.drained, 0);
     }
 meet:
     __syncthreads();
