@@ -36,9 +36,12 @@ inline PagedCache paged_cache(const lv_paged_cache& c) {
     return p;
 }
 
+// Entry of a sequence's table row that a position lies in
+__host__ __device__ __forceinline__ uint32_t paged_slot(const PagedCache& c, uint32_t position) { return uint32_t((uint64_t(position) * c.by_rows.mul) >> (31 + c.by_rows.shift)); }
+
 // Row (of k or v, and of the scales) of a head's position; false: the table names no page of the cache.  A cache has fewer than 2^32 rows, whose bytes need 64 bits.
 __host__ __device__ __forceinline__ bool paged_row(const PagedCache& c, const uint32_t* table_row, uint32_t position, uint32_t head, uint32_t* row) {
-    const uint32_t slot = uint32_t((uint64_t(position) * c.by_rows.mul) >> (31 + c.by_rows.shift)), page = slot < c.table_ld ? table_row[slot] : c.pages;
+    const uint32_t slot = paged_slot(c, position), page = slot < c.table_ld ? table_row[slot] : c.pages;
     *row = (page * c.kv_heads + head) * c.page_rows + (position - slot * c.page_rows);
     return page < c.pages;
 }
@@ -87,6 +90,16 @@ __device__ __forceinline__ float4 unpack_values4(uint2 u, int type) {
         b = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
     }
     return make_float4(a.x, a.y, b.x, b.y);
+}
+// as they lie in memory, to be unpacked behind the loads of several: a conversion in the branch of a load would make each wait for the one before
+__device__ __forceinline__ uint4 load_raw4(const void* p, size_t at, int type) {
+    if (type == LV_TYPE_F32) return *reinterpret_cast<const uint4*>(static_cast<const float*>(p) + at);
+    const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + at);
+    return make_uint4(u.x, u.y, 0u, 0u);
+}
+__device__ __forceinline__ float4 unpack_raw4(uint4 u, int type) {
+    if (type == LV_TYPE_F32) return make_float4(__uint_as_float(u.x), __uint_as_float(u.y), __uint_as_float(u.z), __uint_as_float(u.w));
+    return unpack_values4(make_uint2(u.x, u.y), type);
 }
 __device__ __forceinline__ float4 load_values4(const void* p, size_t at, int type) {
     if (type == LV_TYPE_F32) return *reinterpret_cast<const float4*>(static_cast<const float*>(p) + at);

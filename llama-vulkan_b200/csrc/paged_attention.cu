@@ -21,7 +21,7 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedAttn p, uint
     if (s == c.seqs || !paged_seq(c, s, a.tokens, &q) || q.n > a.max_new || q.len > a.max_len) return;       // (reported)
     const uint32_t r = (t - q.row0) * p.group + h % p.group, r0 = r / block_rows * block_rows;
     const PagedRange all = paged_range(p, q, r0, min(r0 + block_rows, q.n * p.group) - 1);
-    const uint32_t n = (all.hi - all.lo + p.chunk - 1) / p.chunk;
+    const uint32_t n = (all.hi - (all.lo & ~p.align) + p.chunk - 1) / p.chunk;
     const size_t part = (size_t(t) * a.heads + h) * p.splits;
     const float sink = paged_sink(p, h);
     float top = sink - kPaLift;
@@ -69,7 +69,7 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedAttn p, uint
 
 struct PagedPlan {
     uint32_t rows, blocks;       // rows of a block, blocks of the longest chunk of new tokens
-    uint32_t chunk, splits;
+    uint32_t chunk, splits, box;
     size_t bytes;
     bool many;
 };
@@ -77,8 +77,9 @@ struct PagedPlan {
 static PagedPlan paged_plan(const lv_ctx* ctx, const lv_paged_attention_args& a) {
     PagedPlan plan{};
     const uint32_t group = a.heads / a.cache.kv_heads, rows = a.max_new * group;
-    // 16-bit outputs of more than 32 rows that share their keys: a tile of the tensor cores
-    plan.many = a.out_type != LV_TYPE_F32 && a.cache.dim <= 128 && rows > 32;
+    // 16-bit outputs of more than 32 rows that share their keys: a tile of the tensor cores, whose copies take eight rows of a page at least
+    plan.box = std::min(a.cache.page_rows & (0u - a.cache.page_rows), uint32_t(kPtKeys));
+    plan.many = a.out_type != LV_TYPE_F32 && a.cache.dim <= 128 && rows > 32 && plan.box >= 8 && uint64_t(a.cache.pages) * a.cache.kv_heads * a.cache.page_rows < (uint64_t(1) << 31);
     plan.rows = plan.many ? kPtRows : std::min((rows + 7) / 8 * 8, a.cache.dim > 128 ? 16u : 32u);
     plan.blocks = (rows + plan.rows - 1) / plan.rows;
     const uint64_t seen = a.window ? std::min<uint64_t>(a.max_len, uint64_t(a.window) + std::min(a.max_new, plan.rows)) : a.max_len;
@@ -88,7 +89,7 @@ static PagedPlan paged_plan(const lv_ctx* ctx, const lv_paged_attention_args& a)
     uint64_t splits = std::max<uint64_t>(1, std::min<uint64_t>((want + ctas - 1) / ctas, (seen + unit - 1) / unit));
     uint64_t chunk = ((seen + splits - 1) / splits + unit - 1) / unit * unit;
     plan.chunk = uint32_t(std::max<uint64_t>(chunk, unit));
-    plan.splits = uint32_t((seen + plan.chunk - 1) / plan.chunk);
+    plan.splits = uint32_t((seen + (plan.many ? kPtKeys - 1 : 0) + plan.chunk - 1) / plan.chunk);
     if (plan.splits == 0) plan.splits = 1;
     plan.bytes = plan.splits == 1 ? 16 : (size_t(a.tokens) * a.heads * plan.splits * (a.cache.dim + 2)) * 4 + 32;
     return plan;
@@ -131,6 +132,8 @@ extern "C" int lv_paged_attention(lv_ctx* ctx, const lv_paged_attention_args* a,
     p.group = a->heads / a->cache.kv_heads;
     p.chunk = plan.chunk;
     p.splits = plan.splits;
+    p.align = plan.many ? kPtKeys - 1 : 0;
+    p.box = plan.box;
     p.part_rl = static_cast<float2*>(scratch);
     p.part_o = static_cast<float*>(scratch) + (size_t(a->tokens) * a->heads * plan.splits * 2 + 3) / 4 * 4;
     p.err = ctx->d_err;

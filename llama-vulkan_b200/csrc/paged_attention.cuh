@@ -18,7 +18,9 @@ struct PagedAttn {
     lv_paged_attention_args a;
     PagedCache c;                // a.cache
     uint32_t group;              // query heads of a key/value head
-    uint32_t chunk, splits;      // keys of a split (from the first key that a block of rows sees), upper bound of the splits
+    uint32_t chunk, splits;      // keys of a split (from the first key that a block of rows sees on), upper bound of the splits
+    uint32_t align;              // splits begin at the block's first key with these bits cleared
+    uint32_t box;                // rows of a TMA box (the kernel for many rows)
     float* part_o;               // [token][head][split][dim]: sums of the splits
     float2* part_rl;             // [token][head][split]: reference and sum of weights
     uint32_t* err;

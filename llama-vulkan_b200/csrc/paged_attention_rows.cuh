@@ -156,7 +156,7 @@ __global__ void __launch_bounds__(32 * kPrWarps, D == 256 ? 1 : NT == 1 ? 4 : NT
     // ---- queries: rotated, divided by a power of two, in one or two 16-bit planes; all of a warp's rows are asked for at once ----
     {
         constexpr int kParts = D == 256 ? 2 : 1, kOwn = S::kRows / kPrWarps;
-        float4 x[kOwn][kParts];
+        uint4 raw[kOwn][kParts];
         float2 turn[kOwn][kParts][2];
 #pragma unroll
         for (int k = 0; k < kOwn; ++k) {
@@ -165,7 +165,7 @@ __global__ void __launch_bounds__(32 * kPrWarps, D == 256 ? 1 : NT == 1 ? 4 : NT
             for (int i = 0; i < kParts; ++i) {
                 const uint32_t d = 4 * (lane + 32 * i);
                 const bool here = r < rows && d < c.dim;
-                x[k][i] = here ? load_values4(a.q, size_t(t) * a.q_ld + size_t(h) * c.dim + d, a.q_type) : make_float4(0.f, 0.f, 0.f, 0.f);
+                raw[k][i] = here ? load_raw4(a.q, size_t(t) * a.q_ld + size_t(h) * c.dim + d, a.q_type) : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
                 for (int e = 0; e < 2; ++e)
                     turn[k][i][e] = here && a.angles != nullptr && d + 2 * e < 2 * a.angle_pairs ? *reinterpret_cast<const float2*>(a.angles + size_t(t) * a.angle_ld + d + 2 * e) : make_float2(1.f, 0.f);
@@ -175,10 +175,12 @@ __global__ void __launch_bounds__(32 * kPrWarps, D == 256 ? 1 : NT == 1 ? 4 : NT
         for (int k = 0; k < kOwn; ++k) {
             const uint32_t r = warp + kPrWarps * k;
             float top = 0.f;
+            float4 x[kParts];
 #pragma unroll
             for (int i = 0; i < kParts; ++i) {
-                if (a.angles != nullptr) x[k][i] = rotate4(x[k][i], turn[k][i][0], turn[k][i][1]);
-                top = fmaxf(fmaxf(top, fmaxf(fabsf(x[k][i].x), fabsf(x[k][i].y))), fmaxf(fabsf(x[k][i].z), fabsf(x[k][i].w)));
+                x[i] = unpack_raw4(raw[k][i], a.q_type);
+                if (a.angles != nullptr) x[i] = rotate4(x[i], turn[k][i][0], turn[k][i][1]);
+                top = fmaxf(fmaxf(top, fmaxf(fabsf(x[i].x), fabsf(x[i].y))), fmaxf(fabsf(x[i].z), fabsf(x[i].w)));
             }
             float f = 1.f;                                               // 2^-e of the largest value (f16 operands)
             if constexpr (!S::kBf16) f = paged_row_unit(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top))));
@@ -187,7 +189,7 @@ __global__ void __launch_bounds__(32 * kPrWarps, D == 256 ? 1 : NT == 1 ? 4 : NT
             for (int i = 0; i < kParts; ++i) {
                 const uint32_t d = 4 * (lane + 32 * i);
                 if (d >= D) continue;
-                float v[4] = {x[k][i].x * f, x[k][i].y * f, x[k][i].z * f, x[k][i].w * f};
+                float v[4] = {x[i].x * f, x[i].y * f, x[i].z * f, x[i].w * f};
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     const uint32_t col = S::column(d + 2 * e), at = r * (2 * D) + (((col >> 3) ^ (r & 7u)) << 4) + (col & 7u) * 2;

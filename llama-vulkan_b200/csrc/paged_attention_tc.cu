@@ -10,22 +10,24 @@
 // key and value is fetched once for both; with fewer the units are the even and the odd steps of the same rows, each with its own O, which are added at the end.
 // One lane issues all products, in this order: P V of a unit, then the unit's next S, so that the scores never overwrite weights that are still to be
 // read, and a finished S says that the unit's last P V has finished too.
-// Keys and values lie in pages, whose rows four warps fetch: 16-bit rows by 16-byte cp.async straight to their places in the 128-byte swizzle; 8-bit codes by cp.async to a
-// ring in which every lane has places of its own, from there converted to f16 (exact).  Rows that no query sees are written as zeros.  References, f16
-// ranges and scales as in paged_attention_rows.cuh.
+// Keys and values come by TMA, a box for the rows of a page or for a part of them (the largest power of two that divides the page, at least eight rows: the swizzle's
+// pattern): 16-bit rows straight into the operands' swizzle, 8-bit codes into a ring, from which four warps convert them to f16 (exact).  cp.async by the same four
+// warps was tried first and kept the load and store unit so busy that every other warp of the CTA waited for it (1142 us against FIGURES_TMA).  Places that no query sees are not
+// fetched, or zeroed behind the copy: their weights are zero, but zero times NaN is not.  References, f16 ranges and scales as in paged_attention_rows.cuh.
 // FIGURES_TC
 //
 // Every wait is bounded; one that gives up sets the error word, and the CTA drains and frees its tensor memory.
-#include <algorithm>
+#include <cuda.h>
 
 #include "paged_attention.cuh"
 #include "tcgen05.cuh"
+#include "tmap.h"
 
 namespace lv {
 
-// Warps: eight of the softmax, four loaders, four of which one issues the products.  Registers move from the latter eight to the former: a row's 128 scores are held at a
-// time.  512 threads are launched with 128 registers each: (8 x 176 + 8 x 80) x 32 = 512 x 128.
-constexpr int kPtSoftmax = 8, kPtLoaders = 4, kPtThreads = 512, kPtStages = 2, kPtRing = 3, kPtManyRegs = 176, kPtFewRegs = 80;
+// Warps: eight of the softmax, four that convert or mend what was copied, four of which one issues the products and one the copies.  Registers move from the latter eight to the former: a row's 128 scores are held at a
+// time.  512 threads are launched with 128 registers each: (8 x 200 + 8 x 56) x 32 = 512 x 128.
+constexpr int kPtSoftmax = 8, kPtHelpers = 4, kPtThreads = 512, kPtStages = 2, kPtRing = 3, kPtManyRegs = 200, kPtFewRegs = 56;
 
 template <int N>
 __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
@@ -78,6 +80,27 @@ __device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t* u) {
 }
 __device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// the largest of three, NaN if one is
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+
+// 2^x for x <= 126 on the multipliers, for a quarter of the weights: the special function unit alone would take as long for the exponentials of a step as the tensor
+// cores for its products.  x = n + f with n whole and |f| <= 1/2; 2^f by a polynomial fitted to it with the least largest relative error (2^-18), n added to the exponent.
+// x below -126 counts as -126: 2^-136 of the largest weight.
+__device__ __forceinline__ float2 exp2_poly2(float2 x) {
+    constexpr float kWhole = 12582912.f;                                 // 1.5 2^23: a sum with it is rounded to a whole number, which its low bits hold
+    x = make_float2(fmaxf(x.x, -126.f), fmaxf(x.y, -126.f));
+    const float2 t = add2(x, make_float2(kWhole, kWhole)), n = add2(t, make_float2(-kWhole, -kWhole)), f = fma2(n, make_float2(-1.f, -1.f), x);
+    float2 y = fma2(make_float2(0x1.3997d4p-7f, 0x1.3997d4p-7f), f, make_float2(0x1.ca1440p-5f, 0x1.ca1440p-5f));
+    y = fma2(y, f, make_float2(0x1.ec06dap-3f, 0x1.ec06dap-3f));
+    y = fma2(y, f, make_float2(0x1.62e0dcp-1f, 0x1.62e0dcp-1f));
+    y = fma2(y, f, make_float2(0x1.ffffe8p-1f, 0x1.ffffe8p-1f));
+    return make_float2(__uint_as_float(__float_as_uint(y.x) + (__float_as_uint(t.x) << 23)), __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(t.y) << 23)));
+}
+
 // V: rows are keys (the K of the product), 64 columns per 128-byte row; groups of eight keys 1024 bytes apart, blocks of 64 columns `block` bytes apart
 __device__ __forceinline__ uint64_t values_desc(uint32_t smem_addr, uint32_t block) {
     return uint64_t((smem_addr >> 4) & 0x3fffu) | (uint64_t(block >> 4) << 16) | (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) | (uint64_t(2) << 61);
@@ -89,11 +112,9 @@ struct TcMeta {                                                          // of a
 };
 struct TcShared {
     TcMeta meta[kPtStages];
-    uint64_t k_full[kPtStages], k_empty[kPtStages], v_full[kPtStages], v_empty[kPtStages], s_full[2], p_full[2][2], o_full[2], q_full, drained;
+    uint64_t k_full[kPtStages], k_empty[kPtStages], v_raw[kPtStages], v_full[kPtStages], v_empty[kPtStages], raw_full[kPtRing], raw_empty[kPtRing], s_full[2], p_full[2][2], o_full[2], q_full, drained;
     float factor[kPtRows], ref[128], l[128];                             // of the rows; of the second unit of the same rows
     uint32_t unit, tmem;
-    float ring_scales[kPtRing][kPtLoaders][32];                          // 8-bit caches: scales on their way
-    uint32_t ring_there[kPtRing][kPtLoaders];
 };
 
 template <int KIND, int D>
@@ -110,11 +131,15 @@ struct TcShape {
     static constexpr size_t kSmem = kShared + sizeof(TcShared);
 };
 
+struct TcMaps {
+    CUtensorMap k, v;
+};
+
 // byte of 16-byte unit u of row r in a tile
 __device__ __forceinline__ uint32_t tile_at(uint32_t r, uint32_t u) { return (u >> 3) * (128 * 128) + r * 128 + (((u & 7u) ^ (r & 7u)) << 4); }
 
 template <int KIND, int D>
-__global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn p) {
+__global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn p, const __grid_constant__ TcMaps maps) {
     using S = TcShape<KIND, D>;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t *s_q = smem, *s_k = smem + 2 * S::kTile, *s_v = s_k + S::kKeyStages * S::kTile, *s_raw = s_v + kPtStages * S::kTile;
@@ -135,7 +160,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn
     }
     const uint32_t r0 = (n_blocks - 1 - back) * kPtRows, rows = min(uint32_t(kPtRows), all_rows - r0);
     const PagedRange all = paged_range(p, q, r0, r0 + rows - 1);
-    const uint64_t begin = uint64_t(all.lo) + uint64_t(split) * p.chunk;
+    const uint64_t begin = uint64_t(all.lo & ~p.align) + uint64_t(split) * p.chunk;        // (steps begin where boxes do)
     if (begin >= all.hi) {
         pdl_launch_dependents();
         return;
@@ -149,7 +174,14 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn
         if (smem_u32(smem) & 1023u) atomicOr(p.err, ERR_BAD_INDEX);      // (the swizzle's rows begin at 1024 bytes; never seen)
         mbar_init(&sh.q_full, kPtSoftmax);
         mbar_init(&sh.drained, 1);
-        for (int i = 0; i < kPtStages; ++i) { mbar_init(&sh.k_full[i], kPtLoaders); mbar_init(&sh.v_full[i], kPtLoaders); mbar_init(&sh.k_empty[i], 1); mbar_init(&sh.v_empty[i], 1); }
+        for (int i = 0; i < kPtStages; ++i) {
+            mbar_init(&sh.k_full[i], S::kEight ? kPtHelpers : 1);
+            mbar_init(&sh.v_raw[i], 1);
+            mbar_init(&sh.v_full[i], kPtHelpers);
+            mbar_init(&sh.k_empty[i], 1);
+            mbar_init(&sh.v_empty[i], 1);
+        }
+        for (int i = 0; i < kPtRing; ++i) { mbar_init(&sh.raw_full[i], 1); mbar_init(&sh.raw_empty[i], kPtHelpers); }
         for (int i = 0; i < 2; ++i) {
             const uint32_t warps = (tile_rows(i) + 31) / 32;             // those with rows
             mbar_init(&sh.s_full[i], 1);
@@ -159,7 +191,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn
         }
         fence_mbar_init();
     }
-    if (warp == kPtSoftmax + kPtLoaders) {
+    if (warp == kPtSoftmax + kPtHelpers) {
         tc_alloc(&sh.tmem, 512);
         pdl_launch_dependents();        // (not before: a CTA of the next launch could take the tensor memory that this one needs, and wait for it)
     }
@@ -174,30 +206,31 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn
         // ---- queries, a warp per sixteenth of the rows at a time, then a row per thread ----------------------
         constexpr int kBatch = 8;
         for (uint32_t i0 = kBatch * warp; i0 < (two ? 256u : 128u); i0 += kBatch * kPtSoftmax) {
-            float4 x[kBatch];
+            uint4 raw[kBatch];
             float2 turn[kBatch][2];
             const uint32_t d = 4 * lane;
 #pragma unroll
             for (int k = 0; k < kBatch; ++k) {
                 const uint32_t r = r0 + i0 + k, t = q.row0 + r / p.group, h = kv * p.group + r % p.group;
                 const bool here = i0 + k < rows && d < c.dim;
-                x[k] = here ? load_values4(a.q, size_t(t) * a.q_ld + size_t(h) * c.dim + d, a.q_type) : make_float4(0.f, 0.f, 0.f, 0.f);
+                raw[k] = here ? load_raw4(a.q, size_t(t) * a.q_ld + size_t(h) * c.dim + d, a.q_type) : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
                 for (int e = 0; e < 2; ++e)
                     turn[k][e] = here && a.angles != nullptr && d + 2 * e < 2 * a.angle_pairs ? *reinterpret_cast<const float2*>(a.angles + size_t(t) * a.angle_ld + d + 2 * e) : make_float2(1.f, 0.f);
             }
 #pragma unroll
             for (int k = 0; k < kBatch; ++k) {
-                if (a.angles != nullptr) x[k] = rotate4(x[k], turn[k][0], turn[k][1]);
+                float4 x = unpack_raw4(raw[k], a.q_type);
+                if (a.angles != nullptr) x = rotate4(x, turn[k][0], turn[k][1]);
                 float f = a.scale * kPaLog2e;
                 if constexpr (!S::kBf16) {
-                    const float top = fmaxf(fmaxf(fabsf(x[k].x), fabsf(x[k].y)), fmaxf(fabsf(x[k].z), fabsf(x[k].w)));
+                    const float top = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
                     const float u = paged_row_unit(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top))));
                     if (lane == 0) sh.factor[i0 + k] = f / u;
                     f = u;
                 }
                 if (d < D) *reinterpret_cast<uint2*>(s_q + ((i0 + k) >> 7) * S::kTile + tile_at((i0 + k) & 127u, d >> 3) + (d & 4u) * 2) =
-                    make_uint2(pack16<S::kBf16>(x[k].x * f, x[k].y * f), pack16<S::kBf16>(x[k].z * f, x[k].w * f));
+                    make_uint2(pack16<S::kBf16>(x.x * f, x.y * f), pack16<S::kBf16>(x.z * f, x.w * f));
             }
         }
         fence_proxy_async();
@@ -241,7 +274,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn
                         s[i + 1] = mul2(s[i + 1], make_float2(k.z, k.w));
                     }
                 }
-                if (!open) {
+                if (__any_sync(0xffffffffu, !open)) {                    // (a vote, so that it is a branch)
                     const uint32_t bits[4] = {there.x, there.y, there.z, there.w};
 #pragma unroll
                     for (int i = 0; i < kPtKeys / 2; ++i) {
@@ -253,9 +286,10 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn
                 }
                 float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int i = 0; i < kPtKeys / 2; ++i) tops[i & 3] = fmaxf(tops[i & 3], fmaxf(s[i].x, s[i].y));
-                float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+                for (int i = 0; i < kPtKeys / 2; ++i) tops[i & 3] = max3_nan(tops[i & 3], s[i].x, s[i].y);
+                float top = max3_nan(max3_nan(tops[0], tops[1], tops[2]), tops[3], tops[3]);
                 if constexpr (!S::kBf16) top *= row_factor;              // (the scale over a power of two: positive)
+                if (!(top < INFINITY)) l = NAN;                          // (exp2_poly2 loses NaN)
                 float keep = 1.f;
                 bool moved = false;
                 if constexpr (S::kEight) {
@@ -294,7 +328,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn
 #pragma unroll
                     for (int i = 0; i < 32; ++i) {
                         const float2 z = s[32 * half + i], x = S::kBf16 ? add2(z, minus) : fma2(z, factor, minus);
-                        float2 e = make_float2(exp2_fast(x.x), exp2_fast(x.y));
+                        float2 e = i % 4 == 3 ? exp2_poly2(x) : make_float2(exp2_fast(x.x), exp2_fast(x.y));
                         sums[i & 1] = add2(sums[i & 1], e);
                         if constexpr (S::kEight) {
                             const float2 v = *reinterpret_cast<const float2*>(&m.vs[64 * half + 2 * i]);
@@ -378,21 +412,26 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn
             }
         }
         tc_fence_before_sync();
-    } else if (warp < kPtSoftmax + kPtLoaders) {
+    } else if (warp < kPtSoftmax + kPtHelpers) {
         fewer_registers<kPtFewRegs>();
-        // ---- keys and values: a warp per 32 rows of every step, a lane looks one up -------------------------
+        // ---- what was copied: a warp per 32 rows of every step, a lane per row --------------------------------
         const uint32_t part = warp - kPtSoftmax;
         const uint32_t* table = c.table + size_t(blockIdx.z) * c.table_ld;
-        uint32_t next_row = 0;
-        bool next_there = false;
-        auto look_up = [&](uint32_t step) {
+        // a row's page is asked for two steps ahead, its scales one
+        bool asked = false, next_there = false;
+        uint32_t page = 0, in_page = 0, next_row = 0;
+        auto ask = [&](uint32_t step) {
             const uint64_t j = uint64_t(lo) + uint64_t(step) * kPtKeys + 32 * part + lane;
-            next_there = j < hi;
-            if (next_there && !paged_row(c, table, uint32_t(j), kv, &next_row)) {
-                atomicOr(p.err, ERR_BAD_INDEX);
-                next_there = false;
-            }
-            if (!next_there) next_row = 0;
+            asked = j >= all.lo && j < hi;
+            if (!asked) return;
+            const uint32_t slot = paged_slot(c, uint32_t(j));
+            in_page = uint32_t(j) - slot * c.page_rows;
+            page = slot < c.table_ld ? table[slot] : c.pages;
+        };
+        auto take = [&]() {
+            next_there = asked && page < c.pages;
+            if (asked && !next_there) atomicOr(p.err, ERR_BAD_INDEX);
+            next_row = next_there ? (page * c.kv_heads + kv) * c.page_rows + in_page : 0;
         };
         auto publish = [&](uint64_t* bar) {
             fence_proxy_async();
@@ -400,159 +439,171 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn
             if (lane == 0) mbar_arrive(bar);
         };
         bool ok = true;
-        look_up(0);
-        // items: keys of a step, then its values
-        if constexpr (!S::kEight) {
-            constexpr uint32_t kUnits = D / 8, kPer = kUnits;            // 16-byte units of a row, and of a lane in a step
-            const uint32_t row_bytes = c.dim * 2, my_unit = lane % kUnits;
-            const uint8_t *my_k = static_cast<const uint8_t*>(c.k) + my_unit * 16, *my_v = static_cast<const uint8_t*>(c.v) + my_unit * 16;
-            // a tile is published while the next two are on their way, or before a wait for a place
-            uint32_t published = 0;
-            auto publish_to = [&](uint32_t end) {
-                for (; published < end; ++published) publish(published & 1u ? &sh.v_full[(published >> 1) % kPtStages] : &sh.k_full[(published >> 1) % kPtStages]);
-            };
-            for (uint32_t item = 0; item < 2 * steps; ++item) {
-                const uint32_t step = item >> 1, st = step % kPtStages, values = item & 1u;
-                if (step >= kPtStages) {
-                    uint64_t* empty = values ? &sh.v_empty[st] : &sh.k_empty[st];
-                    const uint32_t phase = (step / kPtStages - 1) & 1u;
-                    if (!__any_sync(0xffffffffu, mbar_poll(empty, phase))) {
-                        cp_async_wait<0>();
-                        publish_to(item);
-                    }
-                    ok = mbar_wait_warp(empty, phase, p.err);
-                    if (!ok) break;
-                }
-                const uint32_t there = __ballot_sync(0xffffffffu, next_there);
-                const uint32_t to = smem_u32((values ? s_v : s_k) + st * S::kTile);
-                const uint8_t* from = values ? my_v : my_k;
-#pragma unroll
-                for (int i = 0; i < int(kPer); ++i) {
-                    const uint32_t r = (lane + 32 * i) / kUnits;
-                    const uint64_t off = uint64_t(__shfl_sync(0xffffffffu, next_row, int(r))) * row_bytes;
-                    const bool here = ((there >> r) & 1u) != 0 && my_unit * 16 < row_bytes;
-                    cp_async16_zfill(to + tile_at(32 * part + r, my_unit), here ? from + off : static_cast<const uint8_t*>(c.k), here);
-                }
-                if (values) {
-                    if (lane == 0) sh.meta[st].there[part] = there;
-                    look_up(step + 1);
-                }
-                cp_async_commit();
-                if (item >= 2 && published < item - 1) {
-                    cp_async_wait<2>();
-                    publish_to(item - 1);
-                }
+        ask(0);
+        take();
+        [[maybe_unused]] float ks = 0.f, vs = 0.f;
+        if constexpr (S::kEight) {
+            if (next_there) { ks = c.k_scale[next_row]; vs = c.v_scale[next_row]; }
+        }
+        uint32_t there = __ballot_sync(0xffffffffu, next_there);
+        ask(1);
+        for (uint32_t step = 0; step < steps; ++step) {
+            const uint32_t st = step % kPtStages;
+            take();                                                      // of the next step
+            [[maybe_unused]] float next_ks = 0.f, next_vs = 0.f;
+            if constexpr (S::kEight) {
+                if (next_there) { next_ks = c.k_scale[next_row]; next_vs = c.v_scale[next_row]; }
             }
-            cp_async_wait<0>();
-            if (ok) publish_to(2 * steps);
-        } else {
-            constexpr uint32_t kUnits = D / 16, kPer = kUnits;           // units of 16 codes
-            const uint32_t my_unit = lane % kUnits;
-            const uint8_t *my_k = static_cast<const uint8_t*>(c.k) + my_unit * 16, *my_v = static_cast<const uint8_t*>(c.v) + my_unit * 16;
-            // place of this lane's codes in the ring
-            auto ring = [&](uint32_t slot) { return s_raw + slot * S::kRaw + part * (S::kRaw / 4) + lane * 16; };
-            float key_scale = 0.f;
-            auto issue = [&](uint32_t item) {
-                if (item < 2 * steps) {
-                    const uint32_t slot = item % kPtRing, values = item & 1u, there = __ballot_sync(0xffffffffu, next_there);
-                    const uint32_t to = smem_u32(ring(slot));
-                    const uint8_t* from = values ? my_v : my_k;
+            ask(step + 2);
+            TcMeta& m = sh.meta[st];
+            if constexpr (!S::kEight) {
+                ok = mbar_wait_warp(&sh.v_raw[st], (step / kPtStages) & 1u, p.err);
+                if (!ok) break;
+                if (there != 0xffffffffu)
+                    for (uint32_t r = 0; r < 32; ++r)
+                        if (((there >> r) & 1u) == 0 && lane < S::kBlocks * 8) *reinterpret_cast<uint4*>(s_v + st * S::kTile + tile_at(32 * part + r, lane)) = make_uint4(0u, 0u, 0u, 0u);
+            } else {
+                constexpr uint32_t kUnits = D / 16, kPer = kUnits;       // units of 16 codes of a row, and of a lane
+                const uint32_t my_unit = lane % kUnits;
+#pragma unroll
+                for (uint32_t values = 0; values < 2; ++values) {
+                    const uint32_t item = 2 * step + values, slot = item % kPtRing, stages = values ? kPtStages : S::kKeyStages, to_st = step % stages;
+                    ok = ok && mbar_wait_warp(&sh.raw_full[slot], (item / kPtRing) & 1u, p.err);
+                    if (step >= stages) ok = ok && mbar_wait_warp(values ? &sh.v_empty[to_st] : &sh.k_empty[to_st], (step / stages - 1) & 1u, p.err);
+                    if (!ok) break;
+                    const uint8_t* from = s_raw + slot * S::kRaw + my_unit * 16;
+                    uint8_t* to = (values ? s_v : s_k) + to_st * S::kTile;
 #pragma unroll
                     for (int i = 0; i < int(kPer); ++i) {
                         const uint32_t r = (lane + 32 * i) / kUnits;
-                        const uint64_t off = uint64_t(__shfl_sync(0xffffffffu, next_row, int(r))) * c.dim;
-                        const bool here = ((there >> r) & 1u) != 0 && my_unit * 16 < c.dim;
-                        cp_async16_zfill(to + 512 * i, here ? from + off : static_cast<const uint8_t*>(c.k), here);
+                        uint4 w = make_uint4(0u, 0u, 0u, 0u);
+                        if (((there >> r) & 1u) != 0 && my_unit * 16 < c.dim) w = *reinterpret_cast<const uint4*>(from + (32 * part + r) * c.dim);
+                        if constexpr (KIND == LV_TYPE_I8) w = make_uint4(w.x ^ 0x80808080u, w.y ^ 0x80808080u, w.z ^ 0x80808080u, w.w ^ 0x80808080u);
+                        *reinterpret_cast<uint4*>(to + tile_at(32 * part + r, 2 * my_unit)) =
+                            make_uint4(codes_f16<KIND>(w.x, false), codes_f16<KIND>(w.x, true), codes_f16<KIND>(w.y, false), codes_f16<KIND>(w.y, true));
+                        *reinterpret_cast<uint4*>(to + tile_at(32 * part + r, 2 * my_unit + 1)) =
+                            make_uint4(codes_f16<KIND>(w.z, false), codes_f16<KIND>(w.z, true), codes_f16<KIND>(w.w, false), codes_f16<KIND>(w.w, true));
                     }
-                    cp_async4_zfill(smem_u32(&sh.ring_scales[slot][part][lane]), (values ? c.v_scale : c.k_scale) + next_row, next_there);
-                    if (lane == 0) sh.ring_there[slot][part] = there;
-                    if (values) look_up((item >> 1) + 1);
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sh.raw_empty[slot]);
+                    if (values == 0) publish(&sh.k_full[to_st]);
                 }
-                cp_async_commit();
-            };
-            for (uint32_t item = 0; item < kPtRing; ++item) issue(item);
-            for (uint32_t item = 0; item < 2 * steps; ++item) {
-                const uint32_t step = item >> 1, values = item & 1u, slot = item % kPtRing, stages = values ? kPtStages : S::kKeyStages, st = step % stages;
-                cp_async_wait<kPtRing - 1>();
-                if (step >= stages) ok = mbar_wait_warp(values ? &sh.v_empty[st] : &sh.k_empty[st], (step / stages - 1) & 1u, p.err);
                 if (!ok) break;
-                const uint8_t* from = ring(slot);
-                uint8_t* to = (values ? s_v : s_k) + st * S::kTile;
-#pragma unroll
-                for (int i = 0; i < int(kPer); ++i) {
-                    const uint32_t r = (lane + 32 * i) / kUnits;
-                    uint4 w = *reinterpret_cast<const uint4*>(from + 512 * i);
-                    if constexpr (KIND == LV_TYPE_I8) w = make_uint4(w.x ^ 0x80808080u, w.y ^ 0x80808080u, w.z ^ 0x80808080u, w.w ^ 0x80808080u);
-                    *reinterpret_cast<uint4*>(to + tile_at(32 * part + r, 2 * my_unit)) =
-                        make_uint4(codes_f16<KIND>(w.x, false), codes_f16<KIND>(w.x, true), codes_f16<KIND>(w.y, false), codes_f16<KIND>(w.y, true));
-                    *reinterpret_cast<uint4*>(to + tile_at(32 * part + r, 2 * my_unit + 1)) =
-                        make_uint4(codes_f16<KIND>(w.z, false), codes_f16<KIND>(w.z, true), codes_f16<KIND>(w.w, false), codes_f16<KIND>(w.w, true));
-                }
-                // (a step's scales: those of the keys wait in a register for the place that the values' wait has made free)
-                const float scale = sh.ring_scales[slot][part][lane];
-                TcMeta& m = sh.meta[st];
-                if (values) {
-                    m.vs[32 * part + lane] = scale;
-                    m.ks[32 * part + lane] = key_scale;
-                    const uint32_t e = __reduce_max_sync(0xffffffffu, paged_scale_exponent(scale));
-                    if (lane == 0) {
-                        m.exponent[part] = e;
-                        m.there[part] = sh.ring_there[slot][part];
-                    }
-                } else {
-                    key_scale = scale;
-                }
-                publish(values ? &sh.v_full[st] : &sh.k_full[st]);
-                issue(item + kPtRing);
+                m.ks[32 * part + lane] = ks;
+                m.vs[32 * part + lane] = vs;
+                const uint32_t e = __reduce_max_sync(0xffffffffu, paged_scale_exponent(vs));
+                if (lane == 0) m.exponent[part] = e;
             }
-            cp_async_wait<0>();
+            if (lane == 0) m.there[part] = there;
+            publish(&sh.v_full[st]);
+            there = __ballot_sync(0xffffffffu, next_there);
+            if constexpr (S::kEight) { ks = next_ks; vs = next_vs; }
         }
     } else {
         fewer_registers<kPtFewRegs>();
-        if (warp != kPtSoftmax + kPtLoaders || lane != 0) goto meet;
-        // ---- products ------------------------------------------------------------------------------
+        if (warp == kPtSoftmax + kPtHelpers + 1) {
+            // ---- copies: the keys of a step, then its values; a lane per box -----------------------------------------
+            const uint32_t* table = c.table + size_t(blockIdx.z) * c.table_ld;
+            const uint32_t bytes = S::kEight ? p.box * c.dim : S::kBlocks * p.box * 128;
+            uint32_t row = 0, item = 0;
+            bool here = false;
+            for (; item < 2 * steps; ++item) {
+                const uint32_t step = item >> 1, values = item & 1u, st = step % kPtStages, slot = item % kPtRing;
+                if (values == 0) {
+                    const uint64_t j = uint64_t(lo) + uint64_t(step) * kPtKeys + lane * p.box;
+                    here = lane * p.box < kPtKeys && j + p.box > all.lo && j < hi && paged_row(c, table, uint32_t(j), kv, &row);
+                }
+                uint64_t* bar = S::kEight ? &sh.raw_full[slot] : values ? &sh.v_raw[st] : &sh.k_full[st];
+                if constexpr (S::kEight) {
+                    if (item >= kPtRing && !mbar_wait_warp(&sh.raw_empty[slot], (item / kPtRing - 1) & 1u, p.err)) break;
+                } else {
+                    if (step >= kPtStages && !mbar_wait_warp(values ? &sh.v_empty[st] : &sh.k_empty[st], (step / kPtStages - 1) & 1u, p.err)) break;
+                }
+                const uint32_t n = uint32_t(__popc(__ballot_sync(0xffffffffu, here)));
+                if (lane == 0) mbar_expect_tx(bar, n * bytes);
+                __syncwarp();
+                if (here) {
+                    const CUtensorMap* map = values ? &maps.v : &maps.k;
+                    if constexpr (S::kEight) {
+                        tma_load_2d_plain(s_raw + slot * S::kRaw + lane * bytes, map, 0, int(row), bar);
+                    } else {
+                        uint8_t* to = (values ? s_v : s_k) + st * S::kTile + lane * p.box * 128;
+#pragma unroll
+                        for (int block = 0; block < S::kBlocks; ++block) tma_load_2d_plain(to + block * S::kBlock, map, 64 * block, int(row), bar);
+                    }
+                }
+                __syncwarp();
+            }
+            // (a CTA that gives up leaves when its copies have arrived)
+            for (uint32_t i = item - min(item, uint32_t(2 * kPtStages)); i < item; ++i) {
+                const uint32_t step = i >> 1, st = step % kPtStages;
+                if constexpr (S::kEight) {
+                    if (i + kPtRing >= item) mbar_drain(&sh.raw_full[i % kPtRing], (i / kPtRing) & 1u);
+                } else {
+                    mbar_drain(i & 1u ? &sh.v_raw[st] : &sh.k_full[st], (step / kPtStages) & 1u);
+                }
+            }
+        }
+        if (warp != kPtSoftmax + kPtHelpers) goto meet;
+        // ---- products: the whole warp waits and counts, one lane issues (values that are the same in all lanes stay in uniform registers, where the instruction wants them)
         constexpr uint32_t kind = (1u << 4) | (S::kBf16 ? (1u << 7) | (1u << 10) : 0u) | (uint32_t(128 >> 4) << 24);
-        const uint32_t s_desc = kind | (uint32_t(kPtKeys >> 3) << 17), o_desc = kind | (1u << 16) | ((c.dim >> 3) << 17);      // (V is MN-major)
+        constexpr uint32_t s_desc = kind | (uint32_t(kPtKeys >> 3) << 17);
+        const uint32_t o_desc = kind | (1u << 16) | ((c.dim >> 3) << 17);       // (V is MN-major)
         const uint64_t q_desc = tc_smem_desc(smem_u32(s_q)), k_desc = tc_smem_desc(smem_u32(s_k)), v_desc = values_desc(smem_u32(s_v), S::kBlock);
-        const uint32_t k_steps = c.dim / 16;
-        bool ok = mbar_wait(&sh.q_full, 0, p.err);
+        bool ok = mbar_wait_all(&sh.q_full, 0, p.err);
         auto scores = [&](uint32_t w) {
             const uint32_t tile = w & 1u, j = two ? w >> 1 : w, st = j % S::kKeyStages;
-            if (!two || tile == 0) ok = ok && mbar_wait(&sh.k_full[st], (j / S::kKeyStages) & 1u, p.err);
+            if (!two || tile == 0) ok = ok && mbar_wait_all(&sh.k_full[st], (j / S::kKeyStages) & 1u, p.err);
             if (!ok) return;
             tc_fence_after_sync();
             const uint64_t qd = q_desc + ((two && tile ? S::kTile : 0u) >> 4), kd = k_desc + ((st * S::kTile) >> 4);
-            for (uint32_t k = 0; k < k_steps; ++k) {
-                const uint32_t off = (((k >> 2) * S::kBlock) >> 4) + (k & 3u) * 2;
-                tc_mma_f16(tmem + tile * 128, qd + off, kd + off, s_desc, k != 0);
+            const uint32_t to = tmem + tile * 128;
+            if (tc_elect()) {
+#pragma unroll
+                for (uint32_t k = 0; k < D / 16; ++k) {
+                    const uint32_t off = (((k >> 2) * S::kBlock) >> 4) + (k & 3u) * 2;
+                    if (16 * k < c.dim) tc_mma_f16(to, qd + off, kd + off, s_desc, k != 0);
+                }
+                tc_commit(&sh.s_full[tile]);
+                if (!two || tile == 1) tc_commit(&sh.k_empty[st]);
             }
-            tc_commit(&sh.s_full[tile]);
-            if (!two || tile == 1) tc_commit(&sh.k_empty[st]);
+            __syncwarp();
         };
         for (uint32_t w = 0; w < min(units, 2u) && ok; ++w) scores(w);
         for (uint32_t w = 0; w < units && ok; ++w) {
             const uint32_t tile = w & 1u, turn = w >> 1, j = two ? turn : w, st = j % kPtStages;
-            if (!two || tile == 0) ok = mbar_wait(&sh.v_full[st], (j / kPtStages) & 1u, p.err);
+            if (!two || tile == 0) ok = mbar_wait_all(&sh.v_full[st], (j / kPtStages) & 1u, p.err);
             const uint64_t vd = v_desc + ((st * S::kTile) >> 4);
-            for (uint32_t half = 0; half < 2 && ok; ++half) {
-                ok = mbar_wait(&sh.p_full[tile][half], turn & 1u, p.err);
+            const uint32_t to = tmem_o + tile * 128, from = tmem + tile * 128;
+#pragma unroll
+            for (uint32_t half = 0; half < 2; ++half) {
+                ok = ok && mbar_wait_all(&sh.p_full[tile][half], turn & 1u, p.err);
                 if (!ok) break;
                 tc_fence_after_sync();
+                if (tc_elect()) {
 #pragma unroll
-                for (uint32_t k = 0; k < kPtKeys / 32; ++k)              // 16 keys: 8 columns of P, two groups of eight rows of V
-                    tc_mma_f16_ta(tmem_o + tile * 128, tmem + tile * 128 + 32 * half + 8 * k, vd + 128u * (4 * half + k), o_desc, turn != 0 || half != 0 || k != 0);
+                    for (uint32_t k = 0; k < kPtKeys / 32; ++k)          // 16 keys: 8 columns of P, two groups of eight rows of V
+                        tc_mma_f16_ta(to, from + 32 * half + 8 * k, vd + 128u * (4 * half + k), o_desc, half != 0 || k != 0 ? 1u : uint32_t(turn != 0));
+                    if (half == 1 && (!two || tile == 1)) tc_commit(&sh.v_empty[st]);
+                }
+                __syncwarp();
             }
             if (!ok) break;
-            if (!two || tile == 1) tc_commit(&sh.v_empty[st]);
-            if (w + 2 < units) scores(w + 2);
-            else tc_commit(&sh.o_full[tile]);
+            if (w + 2 < units) {
+                scores(w + 2);
+            } else {
+                if (tc_elect()) tc_commit(&sh.o_full[tile]);
+                __syncwarp();
+            }
         }
-        tc_commit(&sh.drained);
+        if (tc_elect()) tc_commit(&sh.drained);
+        __syncwarp();
         mbar_drain(&sh.drained, 0);
+        __syncwarp();
     }
 meet:
     __syncthreads();
-    if (warp == kPtSoftmax + kPtLoaders) {
+    if (warp == kPtSoftmax + kPtHelpers) {
         tc_fence_after_sync();
         tc_free(tmem, 512);
     }
@@ -562,8 +613,21 @@ template <int KIND, int D>
 static int tc_launch(lv_ctx* ctx, const PagedAttn& p, uint32_t blocks) {
     auto* kernel = paged_tc_kernel<KIND, D>;
     const size_t smem = TcShape<KIND, D>::kSmem;
+    TcMaps maps;
+    const uint64_t rows = uint64_t(p.c.pages) * p.c.kv_heads * p.c.page_rows;
+    for (int i = 0; i < 2; ++i) {
+        CUtensorMap* map = i ? &maps.v : &maps.k;
+        const void* base = i ? p.c.v : p.c.k;
+        if (TcShape<KIND, D>::kEight) {
+            const uint64_t dims[2] = {p.c.dim / 8, rows}, strides[1] = {p.c.dim};
+            const uint32_t box[2] = {p.c.dim / 8, p.box};
+            if (const int rc = make_tiled_map(map, base, 2, dims, strides, box)) return rc;
+        } else if (const int rc = make_bf16_map(map, base, rows, p.c.dim, p.c.dim, p.box)) {
+            return rc;
+        }
+    }
     LV_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
-    LV_CUDA(launch_pdl(ctx, kernel, dim3(p.splits * blocks, p.a.cache.kv_heads, p.a.cache.seqs), dim3(kPtThreads), smem, p));
+    LV_CUDA(launch_pdl(ctx, kernel, dim3(p.splits * blocks, p.a.cache.kv_heads, p.a.cache.seqs), dim3(kPtThreads), smem, p, maps));
     return LV_OK;
 }
 
