@@ -85,8 +85,22 @@ static PagedPlan paged_plan(const lv_ctx* ctx, const lv_paged_attention_args& a)
     const uint64_t seen = a.window ? std::min<uint64_t>(a.max_len, uint64_t(a.window) + std::min(a.max_new, plan.rows)) : a.max_len;
     const uint32_t unit = plan.many ? kPtKeys : kPrWarps * (paged_is8(a.cache.type) ? kPrKeys8 : kPrKeys16);
     const uint64_t ctas = uint64_t(a.cache.seqs) * a.cache.kv_heads * plan.blocks;
-    const uint64_t want = plan.many ? uint64_t(ctx->sm_count) * (ctas > uint64_t(ctx->sm_count) ? 6 : 1) : 3ull * ctx->sm_count * (a.cache.seqs > 1 ? kPrRounds : 1);
-    uint64_t splits = std::max<uint64_t>(1, std::min<uint64_t>((want + ctas - 1) / ctas, (seen + unit - 1) / unit));
+    const uint64_t most = std::max<uint64_t>(1, (seen + unit - 1) / unit);
+    uint64_t splits = 1;
+    if (plan.many) {
+        // the split with the fewest steps of 128 keys one after the other: rounds of CTAs, each with about kPtSetUp steps' time beside its own, and the joining, which
+        // moves 8 bytes a value and split at the memory's rate (a step takes about 2 us: 13 MB)
+        uint64_t best = ~uint64_t(0);
+        for (uint64_t n = 1; n <= std::min<uint64_t>(most, 32); ++n) {
+            // (in halves: a last round that is not full costs half a round on average, lengths differ)
+            const uint64_t rounds = ctas * n <= uint64_t(ctx->sm_count) ? 2 : 2 * ctas * n / ctx->sm_count + 1, join = n == 1 ? 0 : 2 + uint64_t(a.tokens) * a.heads * a.cache.dim * 8 * n / (13u << 20);
+            const uint64_t cost = rounds * ((most + n - 1) / n + kPtSetUp) / 2 + join;
+            if (cost < best) { best = cost; splits = n; }
+        }
+    } else {
+        const uint64_t want = 3ull * ctx->sm_count * (a.cache.seqs > 1 ? kPrRounds : 1);
+        splits = std::max<uint64_t>(1, std::min<uint64_t>((want + ctas - 1) / ctas, most));
+    }
     uint64_t chunk = ((seen + splits - 1) / splits + unit - 1) / unit * unit;
     plan.chunk = uint32_t(std::max<uint64_t>(chunk, unit));
     plan.splits = uint32_t((seen + (plan.many ? kPtKeys - 1 : 0) + plan.chunk - 1) / plan.chunk);

@@ -8,7 +8,7 @@
 //
 // in two units that take turns: the tensor cores work for one while the other's weights are computed.  With more than 128 rows a unit is a tile of 128 of them, and each
 // key and value is fetched once for both; with fewer the units are the even and the odd steps of the same rows, each with its own O, which are added at the end.
-// One lane issues all products, in this order: P V of a unit, then the unit's next S, so that the scores never overwrite weights that are still to be
+// One lane issues a unit's products, in this order: P V, then the next S, so that the scores never overwrite weights that are still to be
 // read, and a finished S says that the unit's last P V has finished too.
 // Keys and values come by TMA, a box for the rows of a page or for a part of them (the largest power of two that divides the page, at least eight rows: the swizzle's
 // pattern): 16-bit rows straight into the operands' swizzle, 8-bit codes into a ring, from which four warps convert them to f16 (exact).  cp.async by the same four
@@ -25,9 +25,9 @@
 
 namespace lv {
 
-// Warps: eight of the softmax, four that convert or mend what was copied, four of which one issues the products and one the copies.  Registers move from the latter eight to the former: a row's 128 scores are held at a
+// Warps: eight of the softmax, four that convert or mend what was copied, four of which two issue the products and one the copies.  Registers move from the latter eight to the former: a row's 128 scores are held at a
 // time.  512 threads are launched with 128 registers each: (8 x 200 + 8 x 56) x 32 = 512 x 128.
-constexpr int kPtSoftmax = 8, kPtHelpers = 4, kPtThreads = 512, kPtStages = 2, kPtRing = 3, kPtManyRegs = 200, kPtFewRegs = 56;
+constexpr int kPtSoftmax = 8, kPtHelpers = 4, kPtThreads = 512, kPtStages = 2, kPtRing = 3, kPtPoly = 4, kPtManyRegs = 200, kPtFewRegs = 56;
 
 template <int N>
 __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
@@ -112,7 +112,7 @@ struct TcMeta {                                                          // of a
 };
 struct TcShared {
     TcMeta meta[kPtStages];
-    uint64_t k_full[kPtStages], k_empty[kPtStages], v_raw[kPtStages], v_full[kPtStages], v_empty[kPtStages], raw_full[kPtRing], raw_empty[kPtRing], s_full[2], p_full[2][2], o_full[2], q_full, drained;
+    uint64_t k_full[kPtStages], k_empty[kPtStages], v_raw[kPtStages], v_full[kPtStages], v_empty[kPtStages], raw_full[kPtRing], raw_empty[kPtRing], s_full[2], p_full[2][2], o_full[2], q_full, drained[2];
     float factor[kPtRows], ref[128], l[128];                             // of the rows; of the second unit of the same rows
     uint32_t unit, tmem;
 };
@@ -124,6 +124,7 @@ struct TcShape {
     static constexpr uint32_t kBlock = 128 * 128;                        // bytes of 128 rows of one
     static constexpr uint32_t kTile = kBlocks * kBlock;                  // of a query tile, and of a step's keys or values
     static constexpr uint32_t kRaw = kEight ? 128 * D : 0;               // of a step's codes
+    // (the keys' barriers are those of even and odd steps in any case: two units that wait for one barrier in turn could take a phase for the next but one)
     // a step's keys are free as soon as its scores are there: one place for them is enough where codes on their way need room
     static constexpr uint32_t kKeyStages = kEight ? 1 : kPtStages;
     // queries (two tiles), keys and values, codes
@@ -173,13 +174,12 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn
     if (threadIdx.x == 0) {
         if (smem_u32(smem) & 1023u) atomicOr(p.err, ERR_BAD_INDEX);      // (the swizzle's rows begin at 1024 bytes; never seen)
         mbar_init(&sh.q_full, kPtSoftmax);
-        mbar_init(&sh.drained, 1);
         for (int i = 0; i < kPtStages; ++i) {
             mbar_init(&sh.k_full[i], S::kEight ? kPtHelpers : 1);
             mbar_init(&sh.v_raw[i], 1);
             mbar_init(&sh.v_full[i], kPtHelpers);
-            mbar_init(&sh.k_empty[i], 1);
-            mbar_init(&sh.v_empty[i], 1);
+            mbar_init(&sh.k_empty[i], two ? 2 : 1);
+            mbar_init(&sh.v_empty[i], two ? 2 : 1);
         }
         for (int i = 0; i < kPtRing; ++i) { mbar_init(&sh.raw_full[i], 1); mbar_init(&sh.raw_empty[i], kPtHelpers); }
         for (int i = 0; i < 2; ++i) {
@@ -188,6 +188,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn
             mbar_init(&sh.p_full[i][0], warps);
             mbar_init(&sh.p_full[i][1], warps);
             mbar_init(&sh.o_full[i], 1);
+            mbar_init(&sh.drained[i], 1);
         }
         fence_mbar_init();
     }
@@ -204,7 +205,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn
     if (warp < kPtSoftmax) {
         more_registers<kPtManyRegs>();
         // ---- queries, a warp per sixteenth of the rows at a time, then a row per thread ----------------------
-        constexpr int kBatch = 8;
+        constexpr int kBatch = 16;
         for (uint32_t i0 = kBatch * warp; i0 < (two ? 256u : 128u); i0 += kBatch * kPtSoftmax) {
             uint4 raw[kBatch];
             float2 turn[kBatch][2];
@@ -249,44 +250,55 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn
             // keys that every row of the warp sees
             const uint32_t first = r0 + base_row + 32 * quarter, last = r0 + min(base_row + 32 * quarter + 31, rows - 1);
             const int warp_hi = int(before + first / p.group) - int(lo), warp_lo = int(paged_first_key(before + last / p.group, a.window)) - int(lo);
+            // a unit's turn at the exponentials, which the other one ends with its own (in its warps that have rows); the first is the first unit's
+            const uint32_t turns = 32 * ((min(tile_rows(0), 128u) + 31) / 32 + (min(tile_rows(1), 128u) + 31) / 32);
+            auto begin_turn = [&]() { asm volatile("bar.sync %0, %1;" ::"r"(2 + mine), "r"(turns) : "memory"); };
+            auto end_turn = [&]() { asm volatile("bar.arrive %0, %1;" ::"r"(3 - mine), "r"(turns) : "memory"); };
+            if (mine == 1) end_turn();
             for (uint32_t w = mine; w < units; w += 2) {
                 const uint32_t turn = w >> 1, j = two ? turn : w, st = j % kPtStages;
-                // (after a lost wait the warp goes through the remaining steps without work)
-                ok = ok && mbar_wait_warp(&sh.v_full[st], (j / kPtStages) & 1u, p.err) && mbar_wait_warp_tc(&sh.s_full[mine], turn & 1u, p.err);
-                if (!ok) continue;
-                tc_fence_after_sync();
+                // (after a lost wait the warp goes through the remaining steps without work: the other unit's wait for it)
+                ok = ok && mbar_wait_all(&sh.v_full[st], (j / kPtStages) & 1u, p.err);
+                if (!ok) { begin_turn(); end_turn(); continue; }
                 const TcMeta& m = sh.meta[st];
                 const int j0 = int(j * kPtKeys);
-                float2 s[kPtKeys / 2];
-                {
-                    uint32_t* u = reinterpret_cast<uint32_t*>(s);
-#pragma unroll
-                    for (int i = 0; i < kPtKeys; i += 32) tmem_load32(u + i, s_at + i);
-                    tc_wait_load();
-                }
                 const uint4 there = *reinterpret_cast<const uint4*>(m.there);
-                const bool open = (there.x & there.y & there.z & there.w) == 0xffffffffu && j0 + kPtKeys - 1 <= warp_hi && j0 >= warp_lo;
-                if constexpr (S::kEight) {
-#pragma unroll
-                    for (int i = 0; i < kPtKeys / 2; i += 2) {
-                        const float4 k = *reinterpret_cast<const float4*>(&m.ks[2 * i]);
-                        s[i] = mul2(s[i], make_float2(k.x, k.y));
-                        s[i + 1] = mul2(s[i + 1], make_float2(k.z, k.w));
-                    }
-                }
-                if (__any_sync(0xffffffffu, !open)) {                    // (a vote, so that it is a branch)
-                    const uint32_t bits[4] = {there.x, there.y, there.z, there.w};
-#pragma unroll
-                    for (int i = 0; i < kPtKeys / 2; ++i) {
-                        const int key = j0 + 2 * i;
-                        const uint32_t pair = bits[i / 16] >> ((2 * i) & 31);
-                        s[i].x = (pair & 1u) != 0 && key <= key_hi && key >= key_lo ? s[i].x : -INFINITY;
-                        s[i].y = (pair & 2u) != 0 && key + 1 <= key_hi && key + 1 >= key_lo ? s[i].y : -INFINITY;
-                    }
-                }
+                const bool open = __all_sync(0xffffffffu, (there.x & there.y & there.z & there.w) == 0xffffffffu && j0 + kPtKeys - 1 <= warp_hi && j0 >= warp_lo);
+                ok = mbar_wait_all(&sh.s_full[mine], turn & 1u, p.err);
+                if (!ok) { begin_turn(); end_turn(); continue; }
+                tc_fence_after_sync();
+                float2 s[kPtKeys / 2];
                 float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                // half of the keys is looked at while the other is on its way
+                tmem_load32(reinterpret_cast<uint32_t*>(s), s_at);
+                tmem_load32(reinterpret_cast<uint32_t*>(s) + 32, s_at + 32);
+                tc_wait_load();
+                tmem_load32(reinterpret_cast<uint32_t*>(s) + 64, s_at + 64);
+                tmem_load32(reinterpret_cast<uint32_t*>(s) + 96, s_at + 96);
 #pragma unroll
-                for (int i = 0; i < kPtKeys / 2; ++i) tops[i & 3] = max3_nan(tops[i & 3], s[i].x, s[i].y);
+                for (int half = 0; half < 2; ++half) {
+                    if (half == 1) tc_wait_load();
+                    if constexpr (S::kEight) {
+#pragma unroll
+                        for (int i = 32 * half; i < 32 * half + 32; i += 2) {
+                            const float4 k = *reinterpret_cast<const float4*>(&m.ks[2 * i]);
+                            s[i] = mul2(s[i], make_float2(k.x, k.y));
+                            s[i + 1] = mul2(s[i + 1], make_float2(k.z, k.w));
+                        }
+                    }
+                    if (!open) {
+                        const uint32_t bits[2] = {half ? there.z : there.x, half ? there.w : there.y};
+#pragma unroll
+                        for (int i = 32 * half; i < 32 * half + 32; ++i) {
+                            const int key = j0 + 2 * i;
+                            const uint32_t pair = bits[(i / 16) & 1] >> ((2 * i) & 31);
+                            s[i].x = (pair & 1u) != 0 && key <= key_hi && key >= key_lo ? s[i].x : -INFINITY;
+                            s[i].y = (pair & 2u) != 0 && key + 1 <= key_hi && key + 1 >= key_lo ? s[i].y : -INFINITY;
+                        }
+                    }
+#pragma unroll
+                    for (int i = 32 * half; i < 32 * half + 32; ++i) tops[i & 3] = max3_nan(tops[i & 3], s[i].x, s[i].y);
+                }
                 float top = max3_nan(max3_nan(tops[0], tops[1], tops[2]), tops[3], tops[3]);
                 if constexpr (!S::kBf16) top *= row_factor;              // (the scale over a power of two: positive)
                 if (!(top < INFINITY)) l = NAN;                          // (exp2_poly2 loses NaN)
@@ -320,7 +332,9 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn
                 }
                 const float base = ref == -INFINITY ? 0.f : ref, down = S::kEight ? __uint_as_float((254u - unit) << 23) : 1.f;
                 const float2 minus = make_float2(-base, -base), factor = make_float2(row_factor, row_factor), downs = make_float2(down, down);
-                // weights, half of the keys at a time; they take the first columns of the scores
+                // weights, half of the keys at a time; they take the first columns of the scores.  The two units take turns at this too: at the same time each would need twice as long
+                // for its exponentials, and the tensor cores would wait for both.
+                begin_turn();
                 float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
@@ -328,7 +342,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn
 #pragma unroll
                     for (int i = 0; i < 32; ++i) {
                         const float2 z = s[32 * half + i], x = S::kBf16 ? add2(z, minus) : fma2(z, factor, minus);
-                        float2 e = i % 4 == 3 ? exp2_poly2(x) : make_float2(exp2_fast(x.x), exp2_fast(x.y));
+                        float2 e = i % kPtPoly == kPtPoly - 1 ? exp2_poly2(x) : make_float2(exp2_fast(x.x), exp2_fast(x.y));
                         sums[i & 1] = add2(sums[i & 1], e);
                         if constexpr (S::kEight) {
                             const float2 v = *reinterpret_cast<const float2*>(&m.vs[64 * half + 2 * i]);
@@ -346,6 +360,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sh.p_full[mine][half]);
                 }
+                end_turn();
                 l += (sums[0].x + sums[1].x) + (sums[0].y + sums[1].y);
             }
             if (mine < units) ok = ok && mbar_wait_warp_tc(&sh.o_full[mine], 0, p.err);
@@ -469,7 +484,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn
                 for (uint32_t values = 0; values < 2; ++values) {
                     const uint32_t item = 2 * step + values, slot = item % kPtRing, stages = values ? kPtStages : S::kKeyStages, to_st = step % stages;
                     ok = ok && mbar_wait_warp(&sh.raw_full[slot], (item / kPtRing) & 1u, p.err);
-                    if (step >= stages) ok = ok && mbar_wait_warp(values ? &sh.v_empty[to_st] : &sh.k_empty[to_st], (step / stages - 1) & 1u, p.err);
+                    if (step >= stages) ok = ok && mbar_wait_warp(values ? &sh.v_empty[to_st] : &sh.k_empty[(step - stages) & 1u], ((step - stages) >> 1) & 1u, p.err);
                     if (!ok) break;
                     const uint8_t* from = s_raw + slot * S::kRaw + my_unit * 16;
                     uint8_t* to = (values ? s_v : s_k) + to_st * S::kTile;
@@ -486,7 +501,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn
                     }
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sh.raw_empty[slot]);
-                    if (values == 0) publish(&sh.k_full[to_st]);
+                    if (values == 0) publish(&sh.k_full[step & 1u]);
                 }
                 if (!ok) break;
                 m.ks[32 * part + lane] = ks;
@@ -505,13 +520,23 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn
             // ---- copies: the keys of a step, then its values; a lane per box -----------------------------------------
             const uint32_t* table = c.table + size_t(blockIdx.z) * c.table_ld;
             const uint32_t bytes = S::kEight ? p.box * c.dim : S::kBlocks * p.box * 128;
-            uint32_t row = 0, item = 0;
-            bool here = false;
+            uint32_t row = 0, item = 0, page = 0, in_page = 0;
+            bool here = false, asked = false;
+            auto ask = [&](uint32_t step) {                              // (a step ahead: the table's answer takes as long as a wait)
+                const uint64_t j = uint64_t(lo) + uint64_t(step) * kPtKeys + lane * p.box;
+                asked = lane * p.box < kPtKeys && j + p.box > all.lo && j < hi;
+                if (!asked) return;
+                const uint32_t slot = paged_slot(c, uint32_t(j));
+                in_page = uint32_t(j) - slot * c.page_rows;
+                page = slot < c.table_ld ? table[slot] : c.pages;
+            };
+            ask(0);
             for (; item < 2 * steps; ++item) {
                 const uint32_t step = item >> 1, values = item & 1u, st = step % kPtStages, slot = item % kPtRing;
                 if (values == 0) {
-                    const uint64_t j = uint64_t(lo) + uint64_t(step) * kPtKeys + lane * p.box;
-                    here = lane * p.box < kPtKeys && j + p.box > all.lo && j < hi && paged_row(c, table, uint32_t(j), kv, &row);
+                    here = asked && page < c.pages;
+                    row = (page * c.kv_heads + kv) * c.page_rows + in_page;
+                    ask(step + 1);
                 }
                 uint64_t* bar = S::kEight ? &sh.raw_full[slot] : values ? &sh.v_raw[st] : &sh.k_full[st];
                 if constexpr (S::kEight) {
@@ -544,61 +569,69 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn
                 }
             }
         }
-        if (warp != kPtSoftmax + kPtHelpers) goto meet;
-        // ---- products: the whole warp waits and counts, one lane issues (values that are the same in all lanes stay in uniform registers, where the instruction wants them)
+        if (warp & 1) goto meet;
+        // ---- products: a warp for each unit (one for both spent 1300 clocks a turn on its waits, as long as the products themselves).  The whole warp waits and counts, one lane
+        // issues: values that are the same in all lanes belong in uniform registers, where the instruction wants them, and a reduction tells the compiler which these are.
         constexpr uint32_t kind = (1u << 4) | (S::kBf16 ? (1u << 7) | (1u << 10) : 0u) | (uint32_t(128 >> 4) << 24);
         constexpr uint32_t s_desc = kind | (uint32_t(kPtKeys >> 3) << 17);
         const uint32_t o_desc = kind | (1u << 16) | ((c.dim >> 3) << 17);       // (V is MN-major)
-        const uint64_t q_desc = tc_smem_desc(smem_u32(s_q)), k_desc = tc_smem_desc(smem_u32(s_k)), v_desc = values_desc(smem_u32(s_v), S::kBlock);
-        bool ok = mbar_wait_all(&sh.q_full, 0, p.err);
-        auto scores = [&](uint32_t w) {
-            const uint32_t tile = w & 1u, j = two ? w >> 1 : w, st = j % S::kKeyStages;
-            if (!two || tile == 0) ok = ok && mbar_wait_all(&sh.k_full[st], (j / S::kKeyStages) & 1u, p.err);
-            if (!ok) return;
+        const uint32_t n = __reduce_max_sync(0xffffffffu, units), both = __reduce_max_sync(0xffffffffu, two ? 1u : 0u), tm = __reduce_max_sync(0xffffffffu, tmem);
+        const uint32_t mine = __reduce_max_sync(0xffffffffu, uint32_t(warp - kPtSoftmax - kPtHelpers) / 2);
+        const uint64_t q_desc = tc_smem_desc(smem_u32(s_q)) + ((both && mine ? S::kTile : 0u) >> 4), k_desc = tc_smem_desc(smem_u32(s_k)), v_desc = values_desc(smem_u32(s_v), S::kBlock);
+        const uint32_t s_at = tm + 128 * mine, o_at = tm + 256 + 128 * mine;
+        auto step_of = [&](uint32_t w) { return both ? w >> 1 : w; };
+        auto wait_keys = [&](uint32_t w) {
+            const uint32_t j = step_of(w);
+            return mbar_wait_all(&sh.k_full[j & 1u], (j >> 1) & 1u, p.err);
+        };
+        auto keys = [&](uint32_t w) { return k_desc + (((step_of(w) % S::kKeyStages) * S::kTile) >> 4); };
+        // (one lane)
+        auto scores = [&](uint32_t w, uint64_t kd) {
+#pragma unroll
+            for (uint32_t k = 0; k < D / 16; ++k) {
+                const uint32_t off = (((k >> 2) * S::kBlock) >> 4) + (k & 3u) * 2;
+                if (16 * k < c.dim) tc_mma_f16(s_at, q_desc + off, kd + off, s_desc, k != 0);
+            }
+            tc_commit(&sh.s_full[mine]);
+            tc_commit(&sh.k_empty[step_of(w) & 1u]);
+        };
+        bool ok = mine < n && mbar_wait_all(&sh.q_full, 0, p.err) && wait_keys(mine);
+        if (ok) {
             tc_fence_after_sync();
-            const uint64_t qd = q_desc + ((two && tile ? S::kTile : 0u) >> 4), kd = k_desc + ((st * S::kTile) >> 4);
-            const uint32_t to = tmem + tile * 128;
+            const uint64_t kd = keys(mine);
+            if (tc_elect()) scores(mine, kd);
+            __syncwarp();
+        }
+        for (uint32_t w = mine; w < n && ok; w += 2) {
+            const uint32_t turn = w >> 1, st = step_of(w) % kPtStages;
+            const bool more = w + 2 < n;
+            // what the products of this turn need beside the weights is waited for first
+            ok = mbar_wait_all(&sh.v_full[st], (step_of(w) / kPtStages) & 1u, p.err) && (!more || wait_keys(w + 2));
+            const uint64_t vd = v_desc + ((st * S::kTile) >> 4), kd = keys(w + 2);
+            ok = ok && mbar_wait_all(&sh.p_full[mine][0], turn & 1u, p.err);
+            if (!ok) break;
+            tc_fence_after_sync();
             if (tc_elect()) {
 #pragma unroll
-                for (uint32_t k = 0; k < D / 16; ++k) {
-                    const uint32_t off = (((k >> 2) * S::kBlock) >> 4) + (k & 3u) * 2;
-                    if (16 * k < c.dim) tc_mma_f16(to, qd + off, kd + off, s_desc, k != 0);
-                }
-                tc_commit(&sh.s_full[tile]);
-                if (!two || tile == 1) tc_commit(&sh.k_empty[st]);
+                for (uint32_t k = 0; k < 4; ++k)                         // 16 keys: 8 columns of P, two groups of eight rows of V
+                    tc_mma_f16_ta(o_at, s_at + 8 * k, vd + 128u * k, o_desc, k != 0 ? 1u : uint32_t(turn != 0));
             }
             __syncwarp();
-        };
-        for (uint32_t w = 0; w < min(units, 2u) && ok; ++w) scores(w);
-        for (uint32_t w = 0; w < units && ok; ++w) {
-            const uint32_t tile = w & 1u, turn = w >> 1, j = two ? turn : w, st = j % kPtStages;
-            if (!two || tile == 0) ok = mbar_wait_all(&sh.v_full[st], (j / kPtStages) & 1u, p.err);
-            const uint64_t vd = v_desc + ((st * S::kTile) >> 4);
-            const uint32_t to = tmem_o + tile * 128, from = tmem + tile * 128;
-#pragma unroll
-            for (uint32_t half = 0; half < 2; ++half) {
-                ok = ok && mbar_wait_all(&sh.p_full[tile][half], turn & 1u, p.err);
-                if (!ok) break;
-                tc_fence_after_sync();
-                if (tc_elect()) {
-#pragma unroll
-                    for (uint32_t k = 0; k < kPtKeys / 32; ++k)          // 16 keys: 8 columns of P, two groups of eight rows of V
-                        tc_mma_f16_ta(to, from + 32 * half + 8 * k, vd + 128u * (4 * half + k), o_desc, half != 0 || k != 0 ? 1u : uint32_t(turn != 0));
-                    if (half == 1 && (!two || tile == 1)) tc_commit(&sh.v_empty[st]);
-                }
-                __syncwarp();
-            }
+            ok = mbar_wait_all(&sh.p_full[mine][1], turn & 1u, p.err);
             if (!ok) break;
-            if (w + 2 < units) {
-                scores(w + 2);
-            } else {
-                if (tc_elect()) tc_commit(&sh.o_full[tile]);
-                __syncwarp();
+            tc_fence_after_sync();
+            if (tc_elect()) {
+#pragma unroll
+                for (uint32_t k = 4; k < 8; ++k) tc_mma_f16_ta(o_at, s_at + 8 * k, vd + 128u * k, o_desc, 1u);
+                tc_commit(&sh.v_empty[st]);
+                if (more) scores(w + 2, kd);
+                else tc_commit(&sh.o_full[mine]);
             }
+            __syncwarp();
         }
-        if (tc_elect()) tc_commit(&sh.drained);
+        if (tc_elect()) tc_commit(&sh.drained[mine]);
         __syncwarp();
-        mbar_drain(&sh.drained, 0);
+        mbar_drain(&sh.drained[mine], 0);
         __syncwarp();
     }
 meet:
