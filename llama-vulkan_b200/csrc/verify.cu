@@ -30,8 +30,8 @@ __device__ __forceinline__ void cluster_all_here() { asm volatile("barrier.clust
 // out = e^((x - m) / T) / sum: a cluster of up to 16 CTAs takes a row, so that all of it lies in registers between the read and the write; the CTAs tell one another
 // their maximum and sum once.  A value is read, raised and written once; longer rows than 16 x 16384 are read and raised a second time.
 // FIGURES_PROBS
-constexpr int kProbThreads = 512, kProbGroups = 8;                       // groups of four values that a thread holds
-constexpr uint32_t kProbHeld = kProbThreads * 4 * kProbGroups;           // of a CTA: 16384
+constexpr int kProbThreads = 512, kProbGroups = 4;                       // groups of four values that a thread holds, or has on their way at a time
+constexpr uint32_t kProbHeld = kProbThreads * 4 * kProbGroups;           // of a CTA: 8192
 constexpr int kProbCluster = 16;
 
 struct Probabilities {
@@ -48,7 +48,7 @@ __device__ __forceinline__ void first_max(float& v, uint32_t& i, float w, uint32
 
 // VEC: rows are 16-byte aligned; HELD: a CTA's values fit its registers
 template <bool VEC, bool HELD>
-__global__ void __launch_bounds__(kProbThreads, 2) probabilities_kernel(const Probabilities p) {
+__global__ void __launch_bounds__(kProbThreads, 3) probabilities_kernel(const Probabilities p) {
     pdl_launch_dependents();
     cluster_here();
     pdl_wait();
@@ -85,8 +85,8 @@ __global__ void __launch_bounds__(kProbThreads, 2) probabilities_kernel(const Pr
         if (i + 3 < hi) y[i + 3] = v.w;
     };
     constexpr uint32_t kStep = kProbThreads * 4;
-    float4 v[HELD ? kProbGroups : 1];
-    float top = -INFINITY;
+    float4 v[kProbGroups];
+    float top = -INFINITY, sum = 0.f, base = 0.f;
     uint32_t at = 0xffffffffu;
     auto look = [&](const float4& w, uint32_t i) {
         // (in the order of the indexes: a later value has to be larger)
@@ -95,19 +95,32 @@ __global__ void __launch_bounds__(kProbThreads, 2) probabilities_kernel(const Pr
         if (w.z > top) { top = w.z; at = i + 2; }
         if (w.w > top) { top = w.w; at = i + 3; }
     };
-    if constexpr (HELD) {
-#pragma unroll
-        for (int k = 0; k < kProbGroups; ++k) v[k] = load4(lo + 4 * threadIdx.x + k * kStep);
-        if (T == 0.f) {
-#pragma unroll
-            for (int k = 0; k < kProbGroups; ++k) look(v[k], lo + 4 * threadIdx.x + k * kStep);
-        } else {
-#pragma unroll
-            for (int k = 0; k < kProbGroups; ++k) top = fmaxf(fmaxf(top, fmaxf(v[k].x, v[k].y)), fmaxf(v[k].z, v[k].w));
-        }
+    auto raise4 = [&](const float4& w) { return make_float4(exp2_fast((w.x - base) * f), exp2_fast((w.y - base) * f), exp2_fast((w.z - base) * f), exp2_fast((w.w - base) * f)); };
+    const uint32_t mine0 = lo + 4 * threadIdx.x;
+    if (T == 0.f) {
+        for (uint32_t i = mine0; i < hi; i += kStep) look(load4(i), i);
     } else {
-        for (uint32_t i = lo + 4 * threadIdx.x; i < hi; i += kStep) look(load4(i), i);
+        // a running maximum of each thread; the exponentials of the values held are taken again below the CTA's
+        for (uint32_t i0 = mine0; i0 < hi; i0 += kStep * kProbGroups) {
+#pragma unroll
+            for (int k = 0; k < kProbGroups; ++k) v[k] = load4(i0 + k * kStep);
+            float most = top;
+#pragma unroll
+            for (int k = 0; k < kProbGroups; ++k) most = fmaxf(fmaxf(most, fmaxf(v[k].x, v[k].y)), fmaxf(v[k].z, v[k].w));
+            if constexpr (!HELD) {
+                base = most == -INFINITY ? 0.f : most;
+                sum *= exp2_fast((top - base) * f);                      // (0 while there is no maximum)
+#pragma unroll
+                for (int k = 0; k < kProbGroups; ++k) {
+                    if (i0 + k * kStep >= hi) continue;
+                    const float4 w = raise4(v[k]);
+                    sum += (w.x + w.y) + (w.z + w.w);
+                }
+            }
+            top = most;
+        }
     }
+    const float own = top;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         const float w = __shfl_xor_sync(0xffffffffu, top, o);
@@ -118,22 +131,17 @@ __global__ void __launch_bounds__(kProbThreads, 2) probabilities_kernel(const Pr
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < kProbThreads / 32; ++w) first_max(top, at, s_top[w], s_at[w]);
-    const float base = top == -INFINITY ? 0.f : top;
-    float sum = 0.f;
-    auto raise4 = [&](const float4& w) { return make_float4(exp2_fast((w.x - base) * f), exp2_fast((w.y - base) * f), exp2_fast((w.z - base) * f), exp2_fast((w.w - base) * f)); };
+    base = top == -INFINITY ? 0.f : top;
     if (T != 0.f) {
         if constexpr (HELD) {
 #pragma unroll
             for (int k = 0; k < kProbGroups; ++k) {
-                if (lo + k * kStep >= hi) continue;
+                if (mine0 + k * kStep >= hi) continue;
                 v[k] = raise4(v[k]);
                 sum += (v[k].x + v[k].y) + (v[k].z + v[k].w);
             }
-        } else {
-            for (uint32_t i = lo + 4 * threadIdx.x; i < hi; i += kStep) {
-                const float4 w = raise4(load4(i));
-                sum += (w.x + w.y) + (w.z + w.w);
-            }
+        } else if (own != -INFINITY) {
+            sum *= exp2_fast((own - base) * f);
         }
         sum = warp_sum(sum);
         if (lane == 0) s_sum[warp] = sum;
@@ -155,18 +163,19 @@ __global__ void __launch_bounds__(kProbThreads, 2) probabilities_kernel(const Pr
     }
     if (T == 0.f) {
         if (at == 0xffffffffu) at = 0;
-        for (uint32_t i = lo + 4 * threadIdx.x; i < hi; i += kStep) store4(i, make_float4(i == at, i + 1 == at, i + 2 == at, i + 3 == at));
+        for (uint32_t i = mine0; i < hi; i += kStep) store4(i, make_float4(i == at, i + 1 == at, i + 2 == at, i + 3 == at));
         return;
     }
     const float g = total == 0.f ? 0.f : (top == -INFINITY ? 1.f : exp2_fast((top - whole) * f)) / total;
-    if constexpr (HELD) {
+    for (uint32_t i0 = mine0; i0 < hi; i0 += kStep * kProbGroups) {
+        if constexpr (!HELD) {
 #pragma unroll
-        for (int k = 0; k < kProbGroups; ++k) store4(lo + 4 * threadIdx.x + k * kStep, make_float4(v[k].x * g, v[k].y * g, v[k].z * g, v[k].w * g));
-    } else {
-        for (uint32_t i = lo + 4 * threadIdx.x; i < hi; i += kStep) {
-            const float4 w = raise4(load4(i));
-            store4(i, make_float4(w.x * g, w.y * g, w.z * g, w.w * g));
+            for (int k = 0; k < kProbGroups; ++k) v[k] = load4(i0 + k * kStep);
+#pragma unroll
+            for (int k = 0; k < kProbGroups; ++k) v[k] = raise4(v[k]);
         }
+#pragma unroll
+        for (int k = 0; k < kProbGroups; ++k) store4(i0 + k * kStep, make_float4(v[k].x * g, v[k].y * g, v[k].z * g, v[k].w * g));
     }
 }
 
@@ -363,9 +372,10 @@ extern "C" int lv_probabilities(lv_ctx* ctx, float* out, uint32_t out_ld, const 
     LV_ENTER(ctx);
     if (!rows) return LV_OK;
     Probabilities p{out, logits, temperature, out_ld, ld, vocab, 0};
-    // as many CTAs as hold the row; with few rows more of them, down to 2048 values each (FIGURES_SPLIT)
+    // few rows: as many CTAs as hold the row, down to 2048 values each; many: eight, which read it a second time from the L2 (vocabulary 128256, 5 rows: 4.5 us held, 5.2 read again; 512 rows on 256000: 127 us with eight, 131 with four)
+    const bool few = uint64_t(rows) * 8 <= 2 * uint64_t(ctx->sm_count);
     uint32_t n = 1;
-    while (n < uint32_t(kProbCluster) && (uint64_t(n) * kProbHeld < vocab || (uint64_t(rows) * n * 2 <= uint64_t(ctx->sm_count) && n < 8 && vocab / (2 * n) >= 2048))) n *= 2;
+    while (n < (few && vocab > 8 * kProbHeld ? uint32_t(kProbCluster) : 8u) && vocab / (2 * n) >= 2048) n *= 2;
     p.each = ((vocab + n - 1) / n + 3) / 4 * 4;
     const bool vec = aligned16(out) && aligned16(logits) && out_ld % 4 == 0 && ld % 4 == 0, held = p.each <= kProbHeld;
     auto* kernel = vec ? (held ? probabilities_kernel<true, true> : probabilities_kernel<true, false>) : (held ? probabilities_kernel<false, true> : probabilities_kernel<false, false>);
