@@ -27,7 +27,7 @@ namespace lv {
 
 // Warps: eight of the softmax, four that convert or mend what was copied, four of which two issue the products and one the copies.  Registers move from the latter eight to the former: a row's 128 scores are held at a
 // time.  512 threads are launched with 128 registers each: (8 x 200 + 8 x 56) x 32 = 512 x 128.
-constexpr int kPtSoftmax = 8, kPtHelpers = 4, kPtThreads = 512, kPtStages = 2, kPtRing = 3, kPtPoly = 4, kPtManyRegs = 200, kPtFewRegs = 56;
+constexpr int kPtSoftmax = 8, kPtHelpers = 4, kPtThreads = 512, kPtStages = 2, kPtRing = 3, kPtManyRegs = 200, kPtFewRegs = 56;
 
 template <int N>
 __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
@@ -81,25 +81,7 @@ __device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t* u) {
 __device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // the largest of three, NaN if one is
-__device__ __forceinline__ float max3_nan(float a, float b, float c) {
-    float y;
-    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
-    return y;
-}
-
-// 2^x for x <= 126 on the multipliers, for a quarter of the weights: the special function unit alone would take as long for the exponentials of a step as the tensor
-// cores for its products.  x = n + f with n whole and |f| <= 1/2; 2^f by a polynomial fitted to it with the least largest relative error (2^-18), n added to the exponent.
-// x below -126 counts as -126: 2^-136 of the largest weight.
-__device__ __forceinline__ float2 exp2_poly2(float2 x) {
-    constexpr float kWhole = 12582912.f;                                 // 1.5 2^23: a sum with it is rounded to a whole number, which its low bits hold
-    x = make_float2(fmaxf(x.x, -126.f), fmaxf(x.y, -126.f));
-    const float2 t = add2(x, make_float2(kWhole, kWhole)), n = add2(t, make_float2(-kWhole, -kWhole)), f = fma2(n, make_float2(-1.f, -1.f), x);
-    float2 y = fma2(make_float2(0x1.3997d4p-7f, 0x1.3997d4p-7f), f, make_float2(0x1.ca1440p-5f, 0x1.ca1440p-5f));
-    y = fma2(y, f, make_float2(0x1.ec06dap-3f, 0x1.ec06dap-3f));
-    y = fma2(y, f, make_float2(0x1.62e0dcp-1f, 0x1.62e0dcp-1f));
-    y = fma2(y, f, make_float2(0x1.ffffe8p-1f, 0x1.ffffe8p-1f));
-    return make_float2(__uint_as_float(__float_as_uint(y.x) + (__float_as_uint(t.x) << 23)), __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(t.y) << 23)));
-}
+__device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
 
 // V: rows are keys (the K of the product), 64 columns per 128-byte row; groups of eight keys 1024 bytes apart, blocks of 64 columns `block` bytes apart
 __device__ __forceinline__ uint64_t values_desc(uint32_t smem_addr, uint32_t block) {
@@ -297,11 +279,10 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn
                         }
                     }
 #pragma unroll
-                    for (int i = 32 * half; i < 32 * half + 32; ++i) tops[i & 3] = max3_nan(tops[i & 3], s[i].x, s[i].y);
+                    for (int i = 32 * half; i < 32 * half + 32; ++i) tops[i & 3] = max3(tops[i & 3], s[i].x, s[i].y);
                 }
-                float top = max3_nan(max3_nan(tops[0], tops[1], tops[2]), tops[3], tops[3]);
+                float top = max3(max3(tops[0], tops[1], tops[2]), tops[3], tops[3]);
                 if constexpr (!S::kBf16) top *= row_factor;              // (the scale over a power of two: positive)
-                if (!(top < INFINITY)) l = NAN;                          // (exp2_poly2 loses NaN)
                 float keep = 1.f;
                 bool moved = false;
                 if constexpr (S::kEight) {
@@ -342,7 +323,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn
 #pragma unroll
                     for (int i = 0; i < 32; ++i) {
                         const float2 z = s[32 * half + i], x = S::kBf16 ? add2(z, minus) : fma2(z, factor, minus);
-                        float2 e = i % kPtPoly == kPtPoly - 1 ? exp2_poly2(x) : make_float2(exp2_fast(x.x), exp2_fast(x.y));
+                        float2 e = make_float2(exp2_fast(x.x), exp2_fast(x.y));
                         sums[i & 1] = add2(sums[i & 1], e);
                         if constexpr (S::kEight) {
                             const float2 v = *reinterpret_cast<const float2*>(&m.vs[64 * half + 2 * i]);
