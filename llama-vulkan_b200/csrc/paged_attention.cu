@@ -98,7 +98,8 @@ static PagedPlan paged_plan(const lv_ctx* ctx, const lv_paged_attention_args& a)
             if (cost < best) { best = cost; splits = n; }
         }
     } else {
-        const uint64_t want = 3ull * ctx->sm_count * (a.cache.seqs > 1 ? kPrRounds : 1);
+        // three CTAs per SM hold blocks of up to 16 rows, two the larger ones; sequences of different lengths share the GPU evenly when there are several rounds of CTAs (16 sequences of up to 6000 keys, blocks of 24 rows: 54.7 us with 6 CTAs per SM, 59.2 with 12; 64 of up to 8192, blocks of 8: 127 with 12, 136 with 6)
+        const uint64_t want = uint64_t(ctx->sm_count) * (a.cache.seqs == 1 ? 3 : plan.rows <= 16 ? 12 : 6);
         splits = std::max<uint64_t>(1, std::min<uint64_t>((want + ctas - 1) / ctas, most));
     }
     uint64_t chunk = ((seen + splits - 1) / splits + unit - 1) / unit * unit;

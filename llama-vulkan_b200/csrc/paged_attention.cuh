@@ -48,7 +48,7 @@ __device__ __forceinline__ float paged_sink(const PagedAttn& p, uint32_t head) {
 __device__ __forceinline__ float paged_sink_weight(float sink, float ref) { return sink == -INFINITY ? 0.f : exp2_fast(sink - ref); }
 
 // paged_attention_rows.cuh: blocks of 8, 16, 24 or 32 rows (heads of more than 128 values: 8 or 16)
-constexpr int kPrWarps = 4, kPrKeys16 = 16, kPrKeys8 = 32, kPrRounds = 4;          // warps; keys of a slice; rounds of CTAs that several sequences are split into
+constexpr int kPrWarps = 4, kPrKeys16 = 16, kPrKeys8 = 32;          // warps; keys of a slice
 int paged_rows_launch_bf16(lv_ctx* ctx, const PagedAttn& p, uint32_t rows, uint32_t blocks);
 int paged_rows_launch_f16(lv_ctx* ctx, const PagedAttn& p, uint32_t rows, uint32_t blocks);
 int paged_rows_launch_i8(lv_ctx* ctx, const PagedAttn& p, uint32_t rows, uint32_t blocks);
