@@ -372,7 +372,7 @@ extern "C" int lv_probabilities(lv_ctx* ctx, float* out, uint32_t out_ld, const 
     LV_ENTER(ctx);
     if (!rows) return LV_OK;
     Probabilities p{out, logits, temperature, out_ld, ld, vocab, 0};
-    // few rows: as many CTAs as hold the row, down to 2048 values each; many: eight, which read it a second time from the L2 (vocabulary 128256, 5 rows: 4.5 us held, 5.2 read again; 512 rows on 256000: 127 us with eight, 131 with four)
+    // few rows: as many CTAs as hold the row, down to 2048 values each; many: eight, which read it a second time from the L2 (5 rows of 32000: 4.5 us held, 5.2 read again; 512 rows of 128000: 127 us with eight, 131 with four and four CTAs per SM)
     const bool few = uint64_t(rows) * 8 <= 2 * uint64_t(ctx->sm_count);
     uint32_t n = 1;
     while (n < (few && vocab > 8 * kProbHeld ? uint32_t(kProbCluster) : 8u) && vocab / (2 * n) >= 2048) n *= 2;
