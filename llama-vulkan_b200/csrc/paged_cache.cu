@@ -18,7 +18,8 @@ struct PagedAppend {
 
 // A warp takes the keys or the values of four (L = 16: eight) heads of a token: L lanes a head, four values a lane and part.  All values are asked for before the
 // places are looked up, which is a chain of four dependent loads, once for the heads of a warp.
-// FIGURES_APPEND
+// 8 sequences of 2048 tokens, f32 to int8, 8 heads of 128: 30 us, 4.5 TB/s of 135 MB (a warp per head: 72 us; four heads: 43; types known when compiled: 30).  One token: 4.7 us,
+// a launch and its chain of loads.
 constexpr int kAppendRows = 4;
 // IN, KIND: types of the values given and stored
 template <int IN, int KIND, int L, int PARTS>
@@ -135,7 +136,8 @@ struct PagedRead {
 
 // A thread takes eight neighbouring values of four rows: 8 or 16 bytes in, 16 (f32: 32) out, in step with its neighbours.  Grid: (rows of one head, heads x {keys, values},
 // sequences).
-// FIGURES_READ
+// e4m3 to bf16, 8 sequences of 3000 to 20000 positions: 115 us, 5.9 TB/s of 675 MB (one row a thread: 229 us; four: 166; the row's place by multiplication instead of division: 139; types
+// known when compiled: 117).  int8 to f16, 1531 positions of 32 heads: 8.7 us of which 5.8 are the memory's.
 constexpr int kReadRows = 4;
 template <int KIND, int OUT>
 __global__ void __launch_bounds__(256) paged_read_kernel(const PagedRead p) {
