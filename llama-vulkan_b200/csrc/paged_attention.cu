@@ -76,6 +76,10 @@ struct PagedPlan {
 
 static PagedPlan paged_plan(const lv_ctx* ctx, const lv_paged_attention_args& a) {
     PagedPlan plan{};
+    if (!a.tokens || !a.max_new) {                                       // nobody has new tokens: nothing is launched
+        plan.bytes = 16;
+        return plan;
+    }
     const uint32_t group = a.heads / a.cache.kv_heads, rows = a.max_new * group;
     // 16-bit outputs of more than 32 rows that share their keys: a tile of the tensor cores, whose copies take eight rows of a page at least
     plan.box = std::min(a.cache.page_rows & (0u - a.cache.page_rows), uint32_t(kPtKeys));

@@ -225,6 +225,18 @@ def test_long_contexts_are_split(gpu):
             assert np.array_equal(Step(d, c, new, 2, out=out, sink=True, max_len=12001 + 20).launch().check().shape, first.shape)
 
 
+def test_a_step_in_which_nobody_has_new_tokens(gpu):
+    rng = np.random.default_rng(6)
+    c = pp.Cache(rng, [40, 0], 2, 64, F16, 16).fill(rng)
+    with Dev(gpu) as d:
+        Step(d, c, [0, 0], 4, out=BF16).launch().check()                 # (two rows of nobody's: as they were)
+        empty = pp.Cache(rng, [0, 0], 2, 64, I8, 16)
+        st = Step(d, empty, [0, 0], 4, out=F32)
+        st.a.tokens = st.a.max_new = st.a.max_len = 0
+        assert gpu.lib.lv_paged_attention_scratch_bytes(gpu.handle, C.byref(st.a)) > 0
+        st.launch().check()
+
+
 def test_two_sequences_share_a_page(gpu):
     rng = np.random.default_rng(5)
     c = pp.Cache(rng, [40, 45], 2, 64, F16, 16).fill(rng)
