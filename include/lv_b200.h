@@ -730,7 +730,7 @@ int lv_probabilities(lv_ctx* ctx, float* out, uint32_t out_ld, const float* logi
  *   then one token is drawn from row starts[s] + (number accepted): from max(target - draft, 0) behind a rejected draft (from target where that leaves
  *   nothing), from target behind the last one: the first index whose cumulative weight is above pick[s] * the whole weight
  * accepted[s]: number of drafts accepted; tokens[starts[s] ..]: the accepted drafts, the drawn token, then 0xFFFFFFFF.  A sequence without rows accepts 0 and draws nothing;
- * a draft >= vocab is reported through the error word and rejected, a row without weight reported, its token 0xFFFFFFFF.
+ * a draft >= vocab is reported through the error word and rejected; a row without weight or of infinite weight, and a pick outside [0, 1), are reported, the token 0xFFFFFFFF.
  * lens (may be null): lens[s] -= number of rejected drafts, whose rows in a paged cache are overwritten by the next step.
  * accept, pick: in [0, 1).  Weights are summed in f64. */
 typedef struct lv_verify_args {

@@ -313,13 +313,14 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const lv_verify_
         if (total > 0.0 || !rest) break;
         rest = false;                                                    // nothing is left behind the draft: from the target itself
     }
+    const bool drawn = total > 0.0 && total < INFINITY && pick >= 0.f && pick < 1.f;
     if (rank == 0) {
         for (uint32_t i = threadIdx.x; i <= n; i += kVerifyThreads)
             if (i != accepted) a.tokens[row0 + i] = i < accepted ? a.drafted[row0 + i] : kNobody;
         if (threadIdx.x == 0) {
             a.accepted[s] = accepted;
             if (a.lens) a.lens[s] -= n - accepted;
-            if (!(total > 0.0)) {
+            if (!drawn) {
                 a.tokens[r] = kNobody;
                 atomicOr(err, ERR_BAD_INDEX);
             }
@@ -329,7 +330,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const lv_verify_
     const double target = double(pick) * total;
     const double from = cta0 + s_before[warp], to = warp + 1 == kVerifyWarps ? cta1 : cta0 + s_before[warp + 1];
     const bool last = rank + 1 == kVerifyCluster && warp + 1 == kVerifyWarps;
-    if (!(total > 0.0) || !(from <= target || (rank == 0 && warp == 0)) || !(target < to || last)) return;
+    if (!drawn || !(from <= target) || !(target < to || last)) return;
     double run = from;
     uint32_t found = kNobody, fallback = kNobody;
     for (uint32_t k = 0; k < each && found == kNobody; ++k) {

@@ -510,6 +510,14 @@ def test_rows_without_weight(gpu):
     assert failed is None and list(n) == [0] and t[0] == 5
 
 
+def test_picks_and_weights_that_name_no_token(gpu):
+    target = np.full((5, 64), 1 / 64, np.float32)
+    target[4, 3] = np.inf
+    pick = np.array([1.0, np.nan, -0.25, 0.5, 0.5], np.float32)
+    n, t, _, failed = run_verify(gpu, target, None, np.zeros(5, np.uint32), [0, 1, 2, 3, 4, 5], np.zeros(5, np.float32), pick)
+    assert failed == pkg.LV_ERR_DEVICE_WAIT and list(n) == [0] * 5 and list(t) == [0xFFFFFFFF] * 3 + [32, 0xFFFFFFFF]
+
+
 # ---- a step of all of them together -------------------------------------------------------------------
 
 def test_a_step_with_drafts(gpu):
