@@ -425,6 +425,20 @@ def test_probabilities_of_rows_without_a_choice(gpu):
         assert np.abs(d.get(out, (10,)) - e / e.sum()).max() < 1e-6
 
 
+@pytest.mark.parametrize("vocab", [50, 40001, 300000])
+def test_probabilities_at_the_smallest_temperatures(gpu, vocab):
+    x = np.random.default_rng(vocab).standard_normal((3, vocab)).astype(np.float32)
+    x[:, 7], x[1, vocab - 2], x[2, ::3] = 50.0, 50.0, -np.inf
+    want = np.zeros((3, vocab), np.float32)
+    want[:, 7] = 1.0
+    want[1, [7, vocab - 2]] = 0.5
+    with Dev(gpu) as d:
+        for T in (1e-45, 1e-42, 1e-38, 1e-30):
+            out = d.zeros(3 * vocab * 4)
+            d.call("lv_probabilities", out, vocab, d.f32(x), vocab, vocab, 3, d.f32(np.full(3, T, np.float32)))
+            assert np.array_equal(d.get(out, (3, vocab)), want)
+
+
 # ---- verification -------------------------------------------------------------------------------------
 
 def run_verify(gpu, target, draft, drafted, starts, accept, pick, lens=None, gap=0):
