@@ -83,7 +83,7 @@ __device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t* u) {
 }
 __device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// the largest of three, NaN if one is
+// the largest of three; a NaN among them shows in the sum of the weights
 __device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
 
 // V: rows are keys (the K of the product), 64 columns per 128-byte row; groups of eight keys 1024 bytes apart, blocks of 64 columns `block` bytes apart
@@ -239,18 +239,19 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn
             const uint32_t turns = 32 * ((min(tile_rows(0), 128u) + 31) / 32 + (min(tile_rows(1), 128u) + 31) / 32);
             auto begin_turn = [&]() { asm volatile("bar.sync %0, %1;" ::"r"(2 + mine), "r"(turns) : "memory"); };
             auto end_turn = [&]() { asm volatile("bar.arrive %0, %1;" ::"r"(3 - mine), "r"(turns) : "memory"); };
+            auto pass_turn = [&](uint32_t w) { if (w + 1 < units) end_turn(); };          // (behind the last one nobody waits)
             if (mine == 1) end_turn();
             for (uint32_t w = mine; w < units; w += 2) {
                 const uint32_t turn = w >> 1, j = two ? turn : w, st = j % kPtStages;
                 // (after a lost wait the warp goes through the remaining steps without work: the other unit's wait for it)
                 ok = ok && mbar_wait_all(&sh.v_full[st], (j / kPtStages) & 1u, p.err);
-                if (!ok) { begin_turn(); end_turn(); continue; }
+                if (!ok) { begin_turn(); pass_turn(w); continue; }
                 const TcMeta& m = sh.meta[st];
                 const int j0 = int(j * kPtKeys);
                 const uint4 there = *reinterpret_cast<const uint4*>(m.there);
                 const bool open = __all_sync(0xffffffffu, (there.x & there.y & there.z & there.w) == 0xffffffffu && j0 + kPtKeys - 1 <= warp_hi && j0 >= warp_lo);
                 ok = mbar_wait_all(&sh.s_full[mine], turn & 1u, p.err);
-                if (!ok) { begin_turn(); end_turn(); continue; }
+                if (!ok) { begin_turn(); pass_turn(w); continue; }
                 tc_fence_after_sync();
                 float2 s[kPtKeys / 2];
                 float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -344,7 +345,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sh.p_full[mine][half]);
                 }
-                end_turn();
+                pass_turn(w);
                 l += (sums[0].x + sums[1].x) + (sums[0].y + sums[1].y);
             }
             if (mine < units) ok = ok && mbar_wait_warp_tc(&sh.o_full[mine], 0, p.err);

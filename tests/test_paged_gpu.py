@@ -237,6 +237,103 @@ def test_a_step_in_which_nobody_has_new_tokens(gpu):
         st.launch().check()
 
 
+@pytest.mark.parametrize("kind", KINDS, ids=pp.NAMES.get)
+@pytest.mark.parametrize("page,dim,heads,H,lens,new", [(8, 16, 3, 1, [90], [31]), (24, 48, 2, 2, [200, 1, 60], [40, 1, 35]), (40, 112, 4, 1, [700], [33]), (128, 128, 1, 1, [129, 128], [129, 128]),
+                                                       (256, 64, 5, 1, [600, 34], [60, 7]), (8, 128, 8, 2, [1, 300, 0, 257], [1, 64, 0, 65])])
+def test_many_rows_of_every_page(gpu, kind, page, dim, heads, H, lens, new):
+    """Boxes of 8 to 128 rows, head sizes that do not fill a block of columns, tiles of one row; windows that begin inside a box."""
+    rng = np.random.default_rng(page + dim)
+    c = pp.Cache(rng, lens, H, dim, kind, page).fill(rng)
+    with Dev(gpu) as d:
+        for window, out in ((0, BF16), (37, F16)):
+            Step(d, c, new, heads, out=out, window=window, sink=bool(window), pairs=dim // 2 if window else 0).launch().check()
+
+
+@pytest.mark.parametrize("new", [3, 100])
+@pytest.mark.parametrize("kind", KINDS, ids=pp.NAMES.get)
+def test_pages_that_are_not_there_to_16_bits(gpu, kind, new):
+    """As above through the kernels of 16-bit outputs: a masked key is one with a score of -infinity."""
+    rng = np.random.default_rng(new + 1)
+    c = pp.Cache(rng, [320], 1, 64, kind, 16).fill(rng)
+    with Dev(gpu) as d:
+        st = Step(d, c, [new], 2, out=F16)
+        table = c.table.copy()
+        table[0, [0, 3, 4, 9]] = [c.pages, c.pages, 0xFFFFFFFF, c.pages + 5]
+        st.a.cache.table = d.u32(table).value
+        st.launch()
+        error_word(gpu)
+        got = st.result()
+        gone = np.concatenate([np.arange(16), np.arange(48, 80), np.arange(144, 160)])
+        k, v = c.read(0, np.arange(320), 0)[:, 0], c.read(0, np.arange(320), 1)[:, 0]
+        z = st.scale * np.einsum("thd,jd->thj", st.q[:new].reshape(new, 2, 64).astype(np.float64), k)
+        z[..., gone] = -np.inf
+        z = np.where(np.arange(320) <= (320 - new + np.arange(new))[:, None, None], z, -np.inf)
+        p = np.exp(z - z.max(-1, keepdims=True))
+        # operands in 16 bits: scores off by 2^-8 (bf16) or 2^-11 times the largest sum |q| |k|, a weight by twice that and its rounding, results by f16's
+        u = pp.HALF_STEP[BF16 if kind == BF16 else F16]
+        most = st.scale * np.einsum("thd,jd->thj", np.abs(st.q[:new]).reshape(new, 2, 64).astype(np.float64), np.abs(k)).max()
+        off = (np.expm1(2 * u * most) + 2 * u + 2.0 ** -15) * (p @ np.abs(v) / p.sum(-1, keepdims=True))
+        want = p @ v / p.sum(-1, keepdims=True)
+        assert (np.abs(got - want) <= off + 2.0 ** -11 * (np.abs(want) + off) + 2.0 ** -25 + 320 * 2.0 ** -35 * np.abs(v).max()).all()
+        st.a.cache.table = d.u32(np.full_like(table, c.pages)).value
+        st.launch()
+        error_word(gpu)
+        assert (st.result() == 0.0).all()
+
+
+@pytest.mark.parametrize("new", [1, 60])
+@pytest.mark.parametrize("kind", [BF16, I8], ids=pp.NAMES.get)
+def test_a_query_that_is_no_number_keeps_to_its_row(gpu, kind, new):
+    rng = np.random.default_rng(3)
+    c = pp.Cache(rng, [300, 200], 1, 64, kind, 16).fill(rng)
+    with Dev(gpu) as d:
+        for out in (F32, BF16):
+            st = Step(d, c, [new, new], 2, out=out)
+            good = st.launch().check()
+            q = padded(st.q, st.ld, F32, 0.0)
+            q[new // 2, :64] = np.nan
+            st.a.q = d.up(q).value
+            got = st.launch().result()
+            bad = np.zeros(got.shape, bool)
+            bad[new // 2, 0] = True
+            assert np.isnan(got[bad]).all() and np.array_equal(got[~bad], good[~bad])
+
+
+def test_two_contexts_at_once(gpu):
+    """Two streams, each with its own scratch, many rows and few, split and whole."""
+    rng = np.random.default_rng(12)
+    c = pp.Cache(rng, [3000, 700], 2, 128, BF16, 64).fill(rng)
+    other = pkg.Context(0)
+    try:
+        with Dev(gpu) as d, Dev(other) as e:
+            steps = [Step(x, c, new, 8, out=BF16, seed=i) for x in (d, e) for i, new in enumerate(([60, 33], [1, 2]))]
+            gpu.sync()
+            other.sync()
+            for _ in range(8):
+                for st in steps:
+                    st.launch()
+            for st in steps:
+                st.check()
+    finally:
+        other.close()
+
+
+def test_many_rows_in_a_recorded_step(gpu):
+    rng = np.random.default_rng(13)
+    c = pp.Cache(rng, [900, 260], 1, 128, E4M3, 32).fill(rng)
+    with Dev(gpu) as d:
+        st = Step(d, c, [70, 40], 4, out=BF16, window=500, sink=True)
+        first = st.launch().check()
+        pkg.check(gpu.lib.lv_graph_begin_capture(gpu.handle))
+        st.launch()
+        g = C.c_void_p()
+        pkg.check(gpu.lib.lv_graph_end_capture(gpu.handle, C.byref(g)))
+        for _ in range(3):
+            pkg.check(gpu.lib.lv_graph_launch(gpu.handle, g))
+            assert np.array_equal(st.result(), first)
+        gpu.lib.lv_graph_destroy(g)
+
+
 def test_two_sequences_share_a_page(gpu):
     rng = np.random.default_rng(5)
     c = pp.Cache(rng, [40, 45], 2, 64, F16, 16).fill(rng)
