@@ -351,24 +351,32 @@ __global__ void __launch_bounds__(32 * kPrWarps, D == 256 ? 1 : NT == 1 ? 4 : NT
             }
             down = __uint_as_float((254u - unit) << 23);
         }
+        // (a row's reference is the same in all lanes: a vote tells whether one has to move, and only then its lanes compare their maxima)
+        float tops[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                float top = -INFINITY;
+                tops[nt][e] = -INFINITY;
 #pragma unroll
-                for (int m = 0; m < kMk; ++m) top = fmaxf(top, fmaxf(s[m][nt][e], s[m][nt][2 + e]));
-#pragma unroll
-                for (int d = 4; d < 32; d *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-                if (top > ref[nt][e] + (kPaLift + kPaStep)) {            // (-inf before the first visible key)
-                    const float next = top - kPaLift, f = exp2_fast(ref[nt][e] - next);
-                    l[nt][e] *= f;
-                    keep[nt][e] *= f;
-                    ref[nt][e] = next;
-                    moved = true;
-                }
+                for (int m = 0; m < kMk; ++m) tops[nt][e] = fmaxf(tops[nt][e], fmaxf(s[m][nt][e], s[m][nt][2 + e]));
+                moved = moved || tops[nt][e] > ref[nt][e] + (kPaLift + kPaStep);           // (-inf before the first visible key)
             }
         if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float top = tops[nt][e];
+#pragma unroll
+                    for (int d = 4; d < 32; d *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                    if (top > ref[nt][e] + (kPaLift + kPaStep)) {
+                        const float next = top - kPaLift, f = exp2_fast(ref[nt][e] - next);
+                        l[nt][e] *= f;
+                        keep[nt][e] *= f;
+                        ref[nt][e] = next;
+                    }
+                }
 #pragma unroll
             for (int j = 0; j < kMo; ++j)
 #pragma unroll
