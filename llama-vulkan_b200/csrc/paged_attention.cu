@@ -16,16 +16,29 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedAttn p, uint
     const uint64_t job = uint64_t(blockIdx.x) * 4 + threadIdx.x / 32;
     const uint32_t t = uint32_t(job / a.heads), h = uint32_t(job - uint64_t(t) * a.heads);
     if (t >= a.tokens) return;
+    // the first parts are asked for before it is known how many there are (all places lie in the scratch)
+    const size_t part = (size_t(t) * a.heads + h) * p.splits;
+    const float2 first = lane < p.splits ? p.part_rl[part + lane] : make_float2(-INFINITY, 0.f);
+    float4 x[4][2];
+    auto ask = [&](uint32_t i0, uint32_t end) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const uint32_t d = 4 * (lane + 32 * k);
+                x[e][k] = i0 + e < end && d < c.dim ? *reinterpret_cast<const float4*>(p.part_o + (part + i0 + e) * c.dim + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+    };
+    ask(0, p.splits);
     const uint32_t s = paged_owner(c, t);
     PagedSeq q;
     if (s == c.seqs || !paged_seq(c, s, a.tokens, &q) || q.n > a.max_new || q.len > a.max_len) return;       // (reported)
     const uint32_t r = (t - q.row0) * p.group + h % p.group, r0 = r / block_rows * block_rows;
     const PagedRange all = paged_range(p, q, r0, min(r0 + block_rows, q.n * p.group) - 1);
     const uint32_t n = (all.hi - (all.lo & ~p.align) + p.chunk - 1) / p.chunk;
-    const size_t part = (size_t(t) * a.heads + h) * p.splits;
     const float sink = paged_sink(p, h);
     float top = sink - kPaLift;
-    float2 mine = lane < n ? p.part_rl[part + lane] : make_float2(-INFINITY, 0.f);
+    float2 mine = lane < n ? first : make_float2(-INFINITY, 0.f);
     top = fmaxf(top, mine.x);
     for (uint32_t i = lane + 32; i < n; i += 32) top = fmaxf(top, p.part_rl[part + i].x);
     top = warp_max(top);
@@ -38,14 +51,7 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedAttn p, uint
         if (!(mine.x == -INFINITY && mine.y == 0.f)) total = fmaf(mine.y, mine_f, total);
         const uint32_t end = min(32u, n - b);
         for (uint32_t i = 0; i < end; i += 4) {
-            float4 x[4][2];
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const uint32_t d = 4 * (lane + 32 * k);
-                    x[e][k] = i + e < end && d < c.dim ? *reinterpret_cast<const float4*>(p.part_o + (part + b + i + e) * c.dim + d) : make_float4(0.f, 0.f, 0.f, 0.f);
-                }
+            if (b + i != 0) ask(b + i, n);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const float f = __shfl_sync(0xffffffffu, mine_f, int(min(i + e, 31u)));

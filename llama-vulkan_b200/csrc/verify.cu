@@ -1,5 +1,6 @@
 // Probabilities from logits, and drafted tokens against them.
 #include <float.h>
+#include <type_traits>
 
 #include "attention_gqa.cuh"
 #include "paged.cuh"
@@ -103,9 +104,10 @@ __global__ void __launch_bounds__(kProbThreads, 3) probabilities_kernel(const Pr
         for (uint32_t i = mine0; i < hi; i += kStep) look(load4(i), i);
     } else {
         // a running maximum of each thread; the exponentials of the values held are taken again below the CTA's
-        for (uint32_t i0 = mine0; i0 < hi; i0 += kStep * kProbGroups) {
+        auto take = [&](auto is_whole, uint32_t i0) {                    // whole: no value of the thread's groups is behind the end
+            constexpr bool whole = decltype(is_whole)::value;
 #pragma unroll
-            for (int k = 0; k < kProbGroups; ++k) v[k] = load4(i0 + k * kStep);
+            for (int k = 0; k < kProbGroups; ++k) v[k] = whole ? *reinterpret_cast<const float4*>(x + i0 + k * kStep) : load4(i0 + k * kStep);
             float most = top;
 #pragma unroll
             for (int k = 0; k < kProbGroups; ++k) most = fmaxf(fmaxf(most, fmaxf(v[k].x, v[k].y)), fmaxf(v[k].z, v[k].w));
@@ -114,12 +116,16 @@ __global__ void __launch_bounds__(kProbThreads, 3) probabilities_kernel(const Pr
                 sum *= exp2_fast((top - base) * f);                      // (0 while there is no maximum)
 #pragma unroll
                 for (int k = 0; k < kProbGroups; ++k) {
-                    if (i0 + k * kStep >= hi) continue;
+                    if (!whole && i0 + k * kStep >= hi) continue;
                     const float4 w = raise4(v[k]);
                     sum += (w.x + w.y) + (w.z + w.w);
                 }
             }
             top = most;
+        };
+        for (uint32_t i0 = mine0; i0 < hi; i0 += kStep * kProbGroups) {
+            if (VEC && i0 + (kProbGroups - 1) * kStep < whole_hi) take(std::true_type{}, i0);
+            else take(std::false_type{}, i0);
         }
     }
     const float own = top;
@@ -169,15 +175,24 @@ __global__ void __launch_bounds__(kProbThreads, 3) probabilities_kernel(const Pr
         return;
     }
     const float g = total == 0.f ? 0.f : (top == -INFINITY ? 1.f : exp2_fast((top - whole) * f)) / total;
-    for (uint32_t i0 = mine0; i0 < hi; i0 += kStep * kProbGroups) {
+    auto give = [&](auto is_whole, uint32_t i0) {
+        constexpr bool whole = decltype(is_whole)::value;
         if constexpr (!HELD) {
 #pragma unroll
-            for (int k = 0; k < kProbGroups; ++k) v[k] = load4(i0 + k * kStep);
+            for (int k = 0; k < kProbGroups; ++k) v[k] = whole ? *reinterpret_cast<const float4*>(x + i0 + k * kStep) : load4(i0 + k * kStep);
 #pragma unroll
             for (int k = 0; k < kProbGroups; ++k) v[k] = raise4(v[k]);
         }
 #pragma unroll
-        for (int k = 0; k < kProbGroups; ++k) store4(i0 + k * kStep, make_float4(v[k].x * g, v[k].y * g, v[k].z * g, v[k].w * g));
+        for (int k = 0; k < kProbGroups; ++k) {
+            const float4 w = make_float4(v[k].x * g, v[k].y * g, v[k].z * g, v[k].w * g);
+            if (whole) *reinterpret_cast<float4*>(y + i0 + k * kStep) = w;
+            else store4(i0 + k * kStep, w);
+        }
+    };
+    for (uint32_t i0 = mine0; i0 < hi; i0 += kStep * kProbGroups) {
+        if (VEC && i0 + (kProbGroups - 1) * kStep < whole_hi) give(std::true_type{}, i0);
+        else give(std::false_type{}, i0);
     }
 }
 
