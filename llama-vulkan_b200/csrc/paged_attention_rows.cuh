@@ -13,9 +13,10 @@
 // (each the rounding of what the ones before left): for f32 outputs with 22 or 24 bits together, for 16-bit outputs with 11 (f16) or 16 (bf16).
 // f16 operands: a query row is divided by a power of two (its largest value is near 1), and the scales of the values by the power of two of the largest so
 // far, so that neither overflows nor loses bits.
-// 64 sequences of one token, 500 to 8192 keys, int8, 32/8 heads of 128: 127 us, 4.7 TB/s of 593 MB; bound by the loads that are on their way (rows as the operand of 16
-// instead: 150 us).  One token of one sequence, 521 keys, 32 heads, f16: 9.0 us, two launches and a chain of loads.  16 sequences with up to 6 drafts over e4m3, blocks of 24 rows:
-// 55 us, bound by the instructions that take codes apart and split weights, not by memory (15 us); the tcgen05 kernel, with tiles four fifths empty: 160 us.
+// 64 sequences of one token, 500 to 8192 keys, int8, 32/8 heads of 128: 126 us, 4.7 TB/s of 593 MB.  Counters: integer pipe 63 %, issue 64 %, memory 62 % of its peak, few waits for loads:
+// the instructions that take codes apart share the time with memory (rows as the operand of 16 instead: 150 us; slices of 16 keys, so that a fourth CTA fits: 134).  One token of one sequence,
+// 521 keys, 32 heads, f16: 8.8 us, two launches and a chain of loads.  16 sequences with 6 drafts over e4m3, blocks of 24 rows: 54 us where memory takes 15: 250 registers leave eight warps per SM, which issue
+// in 44 % of the clocks and wait for their own results (three CTAs per SM, with spilled registers: 61); the tcgen05 kernel, with tiles four fifths empty: 160.
 #pragma once
 
 #include "paged_attention.cuh"

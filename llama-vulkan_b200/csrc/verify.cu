@@ -30,9 +30,9 @@ __device__ __forceinline__ void cluster_all_here() { asm volatile("barrier.clust
 
 // ---- probabilities --------------------------------------------------------------------------------
 
-// out = e^((x - m) / T) / sum: a cluster of up to 16 CTAs takes a row, so that all of it lies in registers between the read and the write; the CTAs tell one another
-// their maximum and sum once.  A value is read, raised and written once; longer rows than 16 x 16384 are read and raised a second time.
-// 512 rows of 128000: 127 us, 4.1 TB/s of 524 MB (one CTA per row: 418 us; all of a row held in registers, eight groups a thread: 165).  5 rows of 32000: 4.5 us, a launch and two meetings.
+// out = e^((x - m) / T) / sum: a cluster of up to 16 CTAs takes a row and its CTAs tell one another their maximum and sum once.  Where a CTA's share fits its
+// registers (HELD: 8192 values) a value is read, raised and written once; else every thread keeps a running maximum and sum, and values are read (from the L2) and raised a second time.
+// 512 rows of 128000: 121 us, 4.3 TB/s of 524 MB (one CTA per row: 418 us; all of a row held in registers, eight groups a thread: 165; every load with its bounds: 125).  5 rows of 32000: 4.5 us, a launch and two meetings.
 constexpr int kProbThreads = 512, kProbGroups = 4;                       // groups of four values that a thread holds, or has on their way at a time
 constexpr uint32_t kProbHeld = kProbThreads * 4 * kProbGroups;           // of a CTA: 8192
 constexpr int kProbCluster = 16;
@@ -202,7 +202,8 @@ __global__ void __launch_bounds__(kProbThreads, 3) probabilities_kernel(const Pr
 // a token is drawn from, each an eighth of it and every warp a run of neighbours, and tell one another their sums.  The bounds between runs are the same numbers
 // for both neighbours, so that exactly one run holds the target; its warp looks through it again.  Sums are f64: the first index whose cumulative weight is above
 // the target does not depend on the order of the sums but where the two agree to 2^-52.
-// 64 sequences with up to 7 drafts, vocabulary 128000: 22 us, 3.0 TB/s of 65 MB, a part of the clusters in a second attempt at the same row (one CTA per sequence: 110 us).  One
+// 64 sequences with up to 7 drafts, vocabulary 128000: 22 us, 3.0 TB/s of 65 MB: two CTAs per SM by their registers, so 1.7 rounds that each wait for look-ups and loads (one CTA per
+// sequence: 110 us; 256 threads: 20.7, but 4.65 for one sequence; clusters of four: 21.1 and 4.9).  One
 // sequence with 4 drafts: 4.1 us, a launch and its meetings (72 us).
 constexpr int kVerifyThreads = 512, kVerifyWarps = kVerifyThreads / 32, kVerifyCluster = 8;
 constexpr uint32_t kNobody = 0xffffffffu;
