@@ -695,7 +695,7 @@ int lv_paged_read(lv_ctx* ctx, const lv_paged_cache* cache, void* k_out, void* v
  * A row that sees nothing gets zeros.  q [tokens][q_ld] and out [tokens][out_ld]: heads * dim values a row, rows 16-byte aligned; q is rotated like the
  * keys of lv_paged_append.  max_new and max_len: upper bounds of the new tokens and of the length of a sequence; they size the launch.
  * Sums, maxima and the softmax are f32.  Output in 16 bits: queries and probabilities enter the matrix products in 16 bits (bf16 for a bf16 cache, else f16).
- * Output in f32: as the sums of two 16-bit numbers each (bf16 caches: three).  Results in 16 bits of more than 32 rows (new tokens times heads / kv_heads) are fastest with page_rows
+ * Output in f32: as the sums of two 16-bit numbers each (bf16 caches: three).  Up to 32 rows over a bf16 cache, or over an f16 cache with f16 results, take two numbers as well.  Results in 16 bits of more than 32 rows (new tokens times heads / kv_heads) are fastest with page_rows
  * a multiple of 8.  out does not overlap q.  Places that no new token sees are not looked at, whatever they hold; a value that is not finite reaches the
  * tokens that see it, and may reach others of the same sequence and step.
  * scratch: 16-byte aligned, lv_paged_attention_scratch_bytes; calls that run at the same time need their own. */

@@ -10,7 +10,7 @@
 // The products are mma.sync m16n8k16, transposed: S^T = K Q^T and O^T = V^T P^T, keys and values the operand of 16 rows, queries and weights the one of 8 columns, so that
 // 8 rows of queries (24, ..) are whole instructions; a tcgen05 tile of 128 would be mostly empty.  Weights change sides by movmatrix.  Operands: bf16 for bf16
 // caches, else f16; 8-bit codes are exact in f16, their scales multiply the finished scores and the weights.  Queries and weights enter as one or more 16-bit numbers
-// (each the rounding of what the ones before left): for f32 outputs with 22 or 24 bits together, for 16-bit outputs with 11 (f16) or 16 (bf16).
+// (each the rounding of what the ones before left): for f32 outputs with 22 or 24 bits together (f16 outputs over f16 caches: 22), for other 16-bit outputs with 11 (f16 operands) or 16 (bf16).
 // f16 operands: a query row is divided by a power of two (its largest value is near 1), and the scales of the values by the power of two of the largest so
 // far, so that neither overflows nor loses bits.
 // 64 sequences of one token, 500 to 8192 keys, int8, 32/8 heads of 128: 126 us, 4.7 TB/s of 593 MB.  Counters: integer pipe 63 %, issue 64 %, memory 62 % of its peak, few waits for loads:
@@ -57,7 +57,7 @@ __device__ __forceinline__ uint32_t take16(float& lo, float& hi) {
     return u;
 }
 
-// KIND: type of the cache; D: head size rounded up to 64, 128 or 256; EXACT: f32 outputs; NT: blocks of 8 rows
+// KIND: type of the cache; D: head size rounded up to 64, 128 or 256; EXACT: f32 outputs (f16 caches: f16 ones too); NT: blocks of 8 rows
 template <int KIND, int D, bool EXACT, int NT>
 struct RowsShape {
     static constexpr bool kEight = KIND == LV_TYPE_I8 || KIND == LV_TYPE_E4M3, kBf16 = KIND == LV_TYPE_BF16;
@@ -563,7 +563,10 @@ static int rows_launch_size(lv_ctx* ctx, const PagedAttn& p, uint32_t rows, uint
 
 template <int KIND>
 static int rows_launch_kind(lv_ctx* ctx, const PagedAttn& p, uint32_t rows, uint32_t blocks) {
-    return p.a.out_type == LV_TYPE_F32 ? rows_launch_size<KIND, true>(ctx, p, rows, blocks) : rows_launch_size<KIND, false>(ctx, p, rows, blocks);
+    // f16 caches take two numbers for f16 results too: with one they are off by 4.9e-4 relative to the result instead of its own rounding's 2.0e-4, and two cost 3 to 5 % (one token, 521 keys: 8.75 us
+    // against 8.49; 64 sequences: 189 against 181).  8-bit caches, whose codes are off by far more, do not: 142 us against 125 (64 sequences), 65 against 54 (drafts).
+    const bool exact = p.a.out_type == LV_TYPE_F32 || (KIND == LV_TYPE_F16 && p.a.out_type == LV_TYPE_F16);
+    return exact ? rows_launch_size<KIND, true>(ctx, p, rows, blocks) : rows_launch_size<KIND, false>(ctx, p, rows, blocks);
 }
 
 }  // namespace lv
