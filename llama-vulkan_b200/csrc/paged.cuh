@@ -58,7 +58,8 @@ __device__ __forceinline__ bool paged_seq(const lv_paged_cache& c, uint32_t s, u
     return a <= b && b <= tokens && b - a <= len && len <= uint64_t(c.table_ld) * c.page_rows;
 }
 
-// The sequence of row t: the last s with starts[s] <= t (seqs: t belongs to nobody); for a whole warp, 32 places at a time.  Ends for any contents of starts.
+// The sequence of row t: the last s with starts[s] <= t (seqs: t belongs to nobody); for a whole warp, 32 places at a time.  Ends for any contents of starts, but where
+// they decrease its answer need not hold t: paged_holds tells.
 __device__ __forceinline__ uint32_t paged_owner(const lv_paged_cache& c, uint32_t t) {
     const uint32_t lane = threadIdx.x & 31u, end = c.starts[c.seqs];
     uint32_t lo = 0, n = c.seqs;                 // of the places lo .. lo + n - 1
@@ -73,6 +74,8 @@ __device__ __forceinline__ uint32_t paged_owner(const lv_paged_cache& c, uint32_
     }
     return t < end ? lo : c.seqs;
 }
+
+__device__ __forceinline__ bool paged_holds(const PagedSeq& q, uint32_t t) { return t - q.row0 < q.n; }
 
 __host__ __device__ __forceinline__ bool paged_is8(int type) { return type == LV_TYPE_I8 || type == LV_TYPE_E4M3; }
 __host__ __device__ __forceinline__ uint32_t paged_bytes(int type) { return type == LV_TYPE_F32 ? 4u : paged_is8(type) ? 1u : 2u; }

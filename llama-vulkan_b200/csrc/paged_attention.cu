@@ -32,10 +32,10 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedAttn p, uint
     ask(0, p.splits);
     const uint32_t s = paged_owner(c, t);
     PagedSeq q;
-    if (s == c.seqs || !paged_seq(c, s, a.tokens, &q) || q.n > a.max_new || q.len > a.max_len) return;       // (reported)
+    if (s == c.seqs || !paged_seq(c, s, a.tokens, &q) || !paged_holds(q, t) || q.n > a.max_new || q.len > a.max_len) return;       // (reported)
     const uint32_t r = (t - q.row0) * p.group + h % p.group, r0 = r / block_rows * block_rows;
     const PagedRange all = paged_range(p, q, r0, min(r0 + block_rows, q.n * p.group) - 1);
-    const uint32_t n = (all.hi - (all.lo & ~p.align) + p.chunk - 1) / p.chunk;
+    const uint32_t n = min((all.hi - (all.lo & ~p.align) + p.chunk - 1) / p.chunk, p.splits);
     const float sink = paged_sink(p, h);
     float top = sink - kPaLift;
     float2 mine = lane < n ? first : make_float2(-INFINITY, 0.f);

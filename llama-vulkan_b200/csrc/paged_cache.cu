@@ -46,7 +46,7 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const PagedAppend p) 
     PagedSeq q;
     if (s == c.seqs) return;
     uint32_t row0;                                                       // of head 0
-    if (!paged_seq(c, s, p.tokens, &q) || !paged_row(c, c.table + size_t(s) * c.table_ld, q.len - q.n + (t - q.row0), 0, &row0)) {
+    if (!paged_seq(c, s, p.tokens, &q) || !paged_holds(q, t) || !paged_row(c, c.table + size_t(s) * c.table_ld, q.len - q.n + (t - q.row0), 0, &row0)) {
         if (lane == 0) atomicOr(p.err, ERR_BAD_INDEX);
         return;
     }

@@ -1,0 +1,68 @@
+"""The cache in pages, the attention over it, probabilities and verification where their inputs contradict themselves or reach the ends of their ranges."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import paged_plain as pp
+from conftest import load_pkg
+from device_data import Dev
+from paged_plain import BF16, E4M3, F16, F32, I8
+from test_paged_gpu import Step, error_word
+
+pytestmark = pytest.mark.gpu
+pkg = load_pkg()
+
+BACKWARDS = [([10, 12, 0, 5], [100, 30, 40]), ([0, 3, 50, 60, 20, 100], [9, 60, 70, 30, 300]), ([0, 40, 8, 9], [41, 3, 200])]
+
+
+# ---- starts that decrease ---------------------------------------------------------------------
+
+@pytest.mark.parametrize("kind", [BF16, I8], ids=pp.NAMES.get)
+@pytest.mark.parametrize("starts,lens", BACKWARDS)
+def test_an_append_whose_starts_decrease_leaves_old_rows_alone(gpu, kind, starts, lens):
+    """A row is looked up by its number among the starts: where they decrease it must not be taken for a row of a sequence that does not hold it."""
+    rng = np.random.default_rng(len(starts))
+    c = pp.Cache(rng, lens, 2, 64, kind, 16).fill(rng)
+    tokens = max(starts)
+    before = [x.copy() for x in c.data + c.scales]
+    with Dev(gpu) as d:
+        a = c.upload(d, starts)
+        x = rng.standard_normal((tokens, 128)).astype(np.float32) * 9
+        pkg.check(gpu.lib.lv_paged_append(gpu.handle, C.byref(a), d.f32(x), d.f32(-x), F32, 128, None, 0, 0, tokens))
+        error_word(gpu)
+        data, scales = c.download(gpu)
+    for s, n in enumerate(lens):                                         # (the new places of the sequences that are in order may be written)
+        m = starts[s + 1] - starts[s]
+        if 0 < m <= n:
+            p, r = c.place(s, np.arange(n - m, n))
+            for old, got in zip(before, data + scales):
+                old[p, :, r] = got[p, :, r]
+    for old, got in zip(before, data + scales):
+        assert np.array_equal(old, got, equal_nan=old.dtype == np.float32)
+
+
+@pytest.mark.parametrize("out", [F32, BF16], ids=["to-f32", "to-bf16"])
+@pytest.mark.parametrize("window", [0, 64])
+@pytest.mark.parametrize("starts,lens", BACKWARDS)
+def test_an_attention_whose_starts_decrease_stays_inside_its_scratch(gpu, starts, lens, window, out):
+    """The parts of a row are joined by its number of parts, which a sequence that does not hold the row does not know."""
+    rng = np.random.default_rng(len(starts))
+    lens = [n + 3000 for n in lens]                                      # (several parts)
+    c = pp.Cache(rng, lens, 1, 64, BF16, 16).fill(rng)
+    tokens = max(starts)
+    with Dev(gpu) as d:
+        st = Step(d, c, [tokens], 4, out=out, window=window, behind=0, max_new=tokens, max_len=max(lens))
+        st.a.cache = c.upload(d, starts)
+        st.bytes = gpu.lib.lv_paged_attention_scratch_bytes(gpu.handle, C.byref(st.a))
+        guard = 4096
+        st.scratch = d.up(np.full(st.bytes + guard, 0xFF, np.uint8))
+        st.launch()
+        error_word(gpu)
+        got = pp.values(gpu.download(st.dout, st.blank.dtype, st.blank.size), out).reshape(tokens, st.ld)
+        assert (gpu.download(st.scratch, np.uint8, st.bytes + guard)[st.bytes:] == 0xFF).all()
+    held = np.zeros(tokens, bool)
+    for a, b in zip(starts, starts[1:]):
+        if a < b:
+            held[a:b] = True
+    assert (got[~held] == -7.0).all() and (got[:, 4 * 64:] == -7.0).all()
