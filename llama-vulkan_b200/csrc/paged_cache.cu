@@ -4,6 +4,8 @@
 // lv_paged_read      value = code * scale
 //
 // Both move bytes: a value is read once and written once, with a handful of operations in between.
+#include <algorithm>
+
 #include "paged.cuh"
 
 namespace lv {
@@ -31,6 +33,11 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const PagedAppend p) 
     const uint32_t lane = threadIdx.x & 31u, H = c.kv_heads, groups = (H + kHeads - 1) / kHeads;
     const uint64_t job = uint64_t(blockIdx.x) * (blockDim.x / 32) + threadIdx.x / 32;
     const uint32_t t = uint32_t(job / (2 * groups)), in_t = uint32_t(job - uint64_t(t) * 2 * groups), which = in_t / groups, h0 = (in_t - which * groups) * kHeads + lane / L;
+    // every sequence is looked at by one thread: one whose rows all lie behind the step's has no warp that would find out
+    for (uint64_t s = uint64_t(blockIdx.x) * blockDim.x + threadIdx.x; s < c.seqs; s += uint64_t(gridDim.x) * blockDim.x) {
+        PagedSeq q;
+        if (!paged_seq(c, uint32_t(s), p.tokens, &q)) atomicOr(p.err, ERR_BAD_INDEX);
+    }
     if (t >= p.tokens) return;
     const uint32_t at0 = 4 * (lane % L);
     float4 v[kAppendRows][PARTS];
@@ -269,7 +276,6 @@ extern "C" int lv_paged_append(lv_ctx* ctx, const lv_paged_cache* cache, const v
     const uint64_t warps = uint64_t(tokens) * 2 * ((cache->kv_heads + heads - 1) / heads);
     LV_REQUIRE(warps < (uint64_t(1) << 31), "paged append: too many tokens");
     LV_ENTER(ctx);
-    if (!tokens) return LV_OK;
     PagedAppend p{};
     p.c = paged_cache(*cache);
     p.in[0] = k;
@@ -280,7 +286,7 @@ extern "C" int lv_paged_append(lv_ctx* ctx, const lv_paged_cache* cache, const v
     p.angle_pairs = angle_pairs;
     p.tokens = tokens;
     p.err = ctx->d_err;
-    const dim3 grid(uint32_t((warps + 7) / 8));
+    const dim3 grid(std::max(1u, uint32_t((warps + 7) / 8)));            // (without rows the sequences are looked at all the same)
     switch (in_type) {
         case LV_TYPE_F32: return append_launch_from<LV_TYPE_F32>(ctx, p, grid);
         case LV_TYPE_F16: return append_launch_from<LV_TYPE_F16>(ctx, p, grid);

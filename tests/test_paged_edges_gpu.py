@@ -19,7 +19,7 @@ BACKWARDS = [([10, 12, 0, 5], [100, 30, 40]), ([0, 3, 50, 60, 20, 100], [9, 60, 
 # ---- starts that decrease ---------------------------------------------------------------------
 
 @pytest.mark.parametrize("kind", [BF16, I8], ids=pp.NAMES.get)
-@pytest.mark.parametrize("starts,lens", BACKWARDS)
+@pytest.mark.parametrize("starts,lens", BACKWARDS + [([5, 0], [64])])
 def test_an_append_whose_starts_decrease_leaves_old_rows_alone(gpu, kind, starts, lens):
     """A row is looked up by its number among the starts: where they decrease it must not be taken for a row of a sequence that does not hold it."""
     rng = np.random.default_rng(len(starts))
@@ -66,3 +66,41 @@ def test_an_attention_whose_starts_decrease_stays_inside_its_scratch(gpu, starts
         if a < b:
             held[a:b] = True
     assert (got[~held] == -7.0).all() and (got[:, 4 * 64:] == -7.0).all()
+
+
+# ---- what an append is told ---------------------------------------------------------------------
+
+@pytest.mark.parametrize("seqs", [3, 700])
+@pytest.mark.parametrize("change", ["beyond the rows", "too long", "before the beginning", "behind all rows"])
+def test_an_append_reports_every_sequence_that_contradicts_itself(gpu, seqs, change):
+    """One of them; the others are written, also where no row of the step is the bad one's."""
+    rng = np.random.default_rng(seqs)
+    lens, new = rng.integers(1, 40, seqs), rng.integers(0, 2, seqs)
+    new[-1] = 1
+    lens[-1] = 20
+    c = pp.Cache(rng, lens, 1, 64, E4M3, 8).fill(rng)
+    starts = np.cumsum([0] + list(new))
+    tokens, told, bad = int(starts[-1]), lens.copy(), seqs - 1
+    if change == "beyond the rows":                                      # the last sequence's only row
+        tokens -= 1
+    elif change == "too long":
+        bad = int(np.argmin(new))                                        # (no new token: nothing else looks at it)
+        told[bad] = c.width * 8 + 1
+        assert new[bad] == 0
+    elif change == "before the beginning":
+        told[bad] = 0
+    else:
+        starts[-1] = 0xFFFFFFF0
+        told[bad] = 5
+    x = rng.standard_normal((max(tokens, 1), 64)).astype(np.float32)
+    with Dev(gpu) as d:
+        a = c.upload(d, starts, told)
+        pkg.check(gpu.lib.lv_paged_append(gpu.handle, C.byref(a), d.f32(x), d.f32(-x), F32, 64, None, 0, 0, tokens))
+        error_word(gpu)
+        data, scales = c.download(gpu)
+    for s in range(seqs):
+        if s != bad and new[s]:
+            c.write(s, [lens[s] - 1], 0, x[starts[s]].reshape(1, 1, 64))
+            c.write(s, [lens[s] - 1], 1, -x[starts[s]].reshape(1, 1, 64))
+    for want, got in zip(c.data + c.scales, data + scales):
+        assert np.array_equal(want, got, equal_nan=want.dtype == np.float32)
