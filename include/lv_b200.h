@@ -650,8 +650,9 @@ int lv_ssm(lv_ctx* ctx, const lv_ssm_args* a, void* scratch, size_t scratch_byte
  * are.  Position i lies in row i mod page_rows of page table[s * table_ld + i / page_rows].  Two sequences may share a page that neither appends to.
  * lens, starts and the table are device memory, so that a recorded step serves every token.  What they say is checked on the device: a length beyond
  * table_ld * page_rows, new tokens beyond the step's rows, beyond the stated upper bounds or before position 0, and pages beyond `pages` set the error word
- * (lv_stream_sync); such a sequence is left out, and positions of a page that is not there count as masked.  Where starts decrease, rows of the step
- * whose sequence cannot be told are left out too.  An attention without rows (tokens or max_new 0) launches nothing and checks nothing of these.
+ * (lv_stream_sync; unlike other errors they end no wait of later calls); such a sequence is left out, and positions of a page that is not there count as
+ * masked.  Where starts decrease, rows of the step whose sequence cannot be told are left out too.  An attention without rows (tokens or max_new 0)
+ * launches nothing and checks nothing of these.
  *
  * 8-bit types hold one f32 scale per row and head: value = code * scale, scale = a / top and code = round(x * (top / a)) to the nearest (ties to
  * even), a = max |x| of the row, top = 127 (LV_TYPE_I8) or 448 (LV_TYPE_E4M3).  A row with a < 2^-100 is stored as zeros, one that is not finite with

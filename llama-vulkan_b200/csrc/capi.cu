@@ -58,13 +58,13 @@ extern "C" int lv_ctx_create(int device, lv_ctx** out) {
     cudaError_t e = cudaStreamCreateWithFlags(&ctx->stream, cudaStreamNonBlocking);
     if (e == cudaSuccess) e = cudaMalloc(&ctx->d_err, 256);
     if (e == cudaSuccess) e = cudaMemset(ctx->d_err, 0, 256);
-    if (e == cudaSuccess) e = cudaMallocHost(&ctx->h_err, sizeof(uint32_t));
+    if (e == cudaSuccess) e = cudaMallocHost(&ctx->h_err, 2 * sizeof(uint32_t));
     if (e == cudaSuccess) e = cudaMallocHost(&ctx->h_bounce, kBounceBytes);
     if (e != cudaSuccess) {
         lv_ctx_destroy(ctx);
         return cuda_fail(e, "lv_ctx_create");
     }
-    *ctx->h_err = 0;
+    ctx->h_err[0] = ctx->h_err[1] = 0;
     int rc = gemv_configure(ctx);
     if (rc == LV_OK) rc = attention_configure(ctx);
     if (rc == LV_OK) rc = attention_prompt_configure(ctx);
@@ -257,12 +257,12 @@ extern "C" int lv_stream_sync(lv_ctx* ctx, int timeout_ms) {
             std::this_thread::yield();
         }
     }
-    LV_CUDA(cudaMemcpyAsync(ctx->h_err, ctx->d_err, sizeof(uint32_t), cudaMemcpyDeviceToHost, ctx->stream));
+    LV_CUDA(cudaMemcpyAsync(ctx->h_err, ctx->d_err, 2 * sizeof(uint32_t), cudaMemcpyDeviceToHost, ctx->stream));
     LV_CUDA(cudaStreamSynchronize(ctx->stream));
-    if (*ctx->h_err != 0) {
-        const uint32_t word = *ctx->h_err;
-        cudaMemsetAsync(ctx->d_err, 0, sizeof(uint32_t), ctx->stream);
-        gemm_tc_reset(ctx);
+    if (ctx->h_err[0] != 0 || ctx->h_err[1] != 0) {
+        const uint32_t word = ctx->h_err[0] | ctx->h_err[1];
+        cudaMemsetAsync(ctx->d_err, 0, 2 * sizeof(uint32_t), ctx->stream);
+        if (ctx->h_err[0] != 0) gemm_tc_reset(ctx);
         return fail(LV_ERR_DEVICE_WAIT, "device error word " + std::to_string(word) +
                                             " (1 = copy wait lost, 2 = grid barrier lost, 4 = peer wait lost, 8 = index out of range)");
     }

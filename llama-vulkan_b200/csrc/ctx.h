@@ -13,8 +13,10 @@ struct lv_ctx {
     int sm_count = 0;
     int max_smem_optin = 0;
     cudaStream_t stream = nullptr;
-    uint32_t* d_err = nullptr;        // device error word, see lv::ERR_* in common.cuh
-    uint32_t* h_err = nullptr;        // pinned mirror used by lv_ctx_check
+    uint32_t* d_err = nullptr;        // device error word, see lv::ERR_* in common.cuh; behind it data_err's
+    uint32_t* h_err = nullptr;        // pinned mirror of both
+    // What paged calls find wrong in a sequence's data: reported like the rest, but no wait looks at it, so that it is the sequence's trouble alone.
+    uint32_t* data_err() const { return d_err + 1; }
     void* h_bounce = nullptr;         // pinned, kBounceBytes: lv_download's way to ordinary memory (used under api_mutex)
     cudaGraph_t capture_graph = nullptr;
     bool capturing = false;

@@ -162,6 +162,7 @@ extern "C" int lv_paged_attention(lv_ctx* ctx, const lv_paged_attention_args* a,
     p.part_rl = static_cast<float2*>(scratch);
     p.part_o = static_cast<float*>(scratch) + (size_t(a->tokens) * a->heads * plan.splits * 2 + 3) / 4 * 4;
     p.err = ctx->d_err;
+    p.data_err = ctx->data_err();
     int rc = LV_OK;
     if (plan.many) rc = paged_tc_launch(ctx, p, plan.blocks);
     else switch (a->cache.type) {

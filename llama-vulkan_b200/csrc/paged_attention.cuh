@@ -23,7 +23,7 @@ struct PagedAttn {
     uint32_t box;                // rows of a TMA box (the kernel for many rows)
     float* part_o;               // [token][head][split][dim]: sums of the splits
     float2* part_rl;             // [token][head][split]: reference and sum of weights
-    uint32_t* err;
+    uint32_t *err, *data_err;    // of waits; of what sequences contain
 };
 
 // The keys that rows r0 .. r1 (of a sequence's n * group; row r is query head r mod group of new token r / group) see: lo .. hi - 1
@@ -39,7 +39,7 @@ __device__ __forceinline__ PagedRange paged_range(const PagedAttn& p, const Page
 // A sequence of the launch; false (reported): it contradicts itself or the stated bounds
 __device__ __forceinline__ bool paged_attention_seq(const PagedAttn& p, uint32_t s, PagedSeq* q) {
     if (paged_seq(p.c, s, p.a.tokens, q) && q->n <= p.a.max_new && q->len <= p.a.max_len) return true;
-    if (threadIdx.x == 0) atomicOr(p.err, ERR_BAD_INDEX);
+    if (threadIdx.x == 0) atomicOr(p.data_err, ERR_BAD_INDEX);
     return false;
 }
 

@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(32 * kPrWarps, D == 256 ? 1 : NT == 1 ? 4 : NT
         const uint64_t j = uint64_t(lo) + uint64_t(slice) * S::kKeys + lane;
         next_there = lane < S::kKeys && j < hi;
         if (next_there && !paged_row(c, table, uint32_t(j), kv, &next_row)) {
-            atomicOr(p.err, ERR_BAD_INDEX);
+            atomicOr(p.data_err, ERR_BAD_INDEX);
             next_there = false;
         }
         if (!next_there) next_row = 0;

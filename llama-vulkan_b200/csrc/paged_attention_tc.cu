@@ -157,7 +157,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn
     const uint32_t units = two ? 2 * steps : steps;
     auto tile_rows = [&](uint32_t unit) { return two ? (unit ? rows - 128 : 128u) : rows; };
     if (threadIdx.x == 0) {
-        if (smem_u32(smem) & 1023u) atomicOr(p.err, ERR_BAD_INDEX);      // (the swizzle's rows begin at 1024 bytes; never seen)
+        if (smem_u32(smem) & 1023u) atomicOr(p.data_err, ERR_BAD_INDEX);      // (the swizzle's rows begin at 1024 bytes; never seen)
         mbar_init(&sh.q_full, kPtSoftmax);
         for (int i = 0; i < kPtStages; ++i) {
             mbar_init(&sh.k_full[i], S::kEight ? kPtHelpers : 1);
@@ -430,7 +430,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn
         };
         auto take = [&]() {
             next_there = asked && page < c.pages;
-            if (asked && !next_there) atomicOr(p.err, ERR_BAD_INDEX);
+            if (asked && !next_there) atomicOr(p.data_err, ERR_BAD_INDEX);
             next_row = next_there ? (page * c.kv_heads + kv) * c.page_rows + in_page : 0;
         };
         auto publish = [&](uint64_t* bar) {

@@ -285,7 +285,7 @@ extern "C" int lv_paged_append(lv_ctx* ctx, const lv_paged_cache* cache, const v
     p.angle_ld = angle_ld;
     p.angle_pairs = angle_pairs;
     p.tokens = tokens;
-    p.err = ctx->d_err;
+    p.err = ctx->data_err();
     const dim3 grid(std::max(1u, uint32_t((warps + 7) / 8)));            // (without rows the sequences are looked at all the same)
     switch (in_type) {
         case LV_TYPE_F32: return append_launch_from<LV_TYPE_F32>(ctx, p, grid);
@@ -315,7 +315,7 @@ extern "C" int lv_paged_read(lv_ctx* ctx, const lv_paged_cache* cache, void* k_o
     p.row_stride = row_stride;
     p.first = first;
     p.rows = rows;
-    p.err = ctx->d_err;
+    p.err = ctx->data_err();
     const dim3 grid(uint32_t(blocks), 2 * cache->kv_heads, cache->seqs);
     switch (cache->type) {
         case LV_TYPE_F16: return read_launch_from<LV_TYPE_F16>(ctx, p, grid);

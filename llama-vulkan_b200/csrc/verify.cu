@@ -410,6 +410,6 @@ extern "C" int lv_verify_drafts(lv_ctx* ctx, const lv_verify_args* a) {
     LV_REQUIRE(a->seqs && a->seqs < (1u << 28) && a->rows < (1u << 31), "verification of drafts: too many rows");
     LV_ENTER(ctx);
     const bool vec = aligned16(a->target) && a->target_ld % 4 == 0 && aligned16(a->draft) && (!a->draft || a->draft_ld % 4 == 0);
-    LV_CUDA(launch_pdl_cluster(ctx, vec ? verify_kernel<true> : verify_kernel<false>, dim3(a->seqs * kVerifyCluster), dim3(kVerifyThreads), dim3(kVerifyCluster), 0, *a, ctx->d_err));
+    LV_CUDA(launch_pdl_cluster(ctx, vec ? verify_kernel<true> : verify_kernel<false>, dim3(a->seqs * kVerifyCluster), dim3(kVerifyThreads), dim3(kVerifyCluster), 0, *a, ctx->data_err()));
     return LV_OK;
 }

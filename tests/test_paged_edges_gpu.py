@@ -5,6 +5,7 @@ import numpy as np
 import pytest
 
 import paged_plain as pp
+import quant_np as qn
 from conftest import load_pkg
 from device_data import Dev
 from paged_plain import BF16, E4M3, F16, F32, I8
@@ -104,3 +105,44 @@ def test_an_append_reports_every_sequence_that_contradicts_itself(gpu, seqs, cha
             c.write(s, [lens[s] - 1], 1, -x[starts[s]].reshape(1, 1, 64))
     for want, got in zip(c.data + c.scales, data + scales):
         assert np.array_equal(want, got, equal_nan=want.dtype == np.float32)
+
+
+# ---- what is behind a contradiction -----------------------------------------------------------------
+
+def contradictions(d):
+    """The paged calls that find their data at odds, by name: each reports and is otherwise in order."""
+    rng = np.random.default_rng(1)
+    c = pp.Cache(rng, [20, 30], 1, 64, BF16, 16).fill(rng)
+    a = c.upload(d, [0, 1, 2], [c.width * 16 + 1, 30])
+    x, out = d.f32(rng.standard_normal((2, 64))), d.zeros(2 * 30 * 64 * 4)
+    lib, h = d.gpu.lib, d.gpu.handle
+    few, many = Step(d, c, [1, 1], 1, behind=0), Step(d, c, [20, 30], 2, behind=0)
+    for st in (few, many):
+        st.a.cache.lens = a.lens
+    v = pkg.VerifyArgs(target=d.f32(np.full((1, 8), 0.125)).value, target_ld=8, vocab=8, drafted=d.u32([0]).value, starts=d.u32([0, 1]).value, seqs=1, rows=1, accept=d.f32([0.5]).value,
+                       pick=d.f32([2.0]).value, tokens=d.u32([0]).value, accepted=d.u32([0]).value)
+    return {"append": lambda: lib.lv_paged_append(h, C.byref(a), x, x, F32, 64, None, 0, 0, 2), "read": lambda: lib.lv_paged_read(h, C.byref(a), out, out, F32, 30 * 64, 0, 64, 0, 30),
+            "attention of few rows": lambda: few.launch() and 0, "attention of many": lambda: many.launch() and 0, "verification": lambda: lib.lv_verify_drafts(h, C.byref(v))}
+
+
+@pytest.mark.parametrize("call", ["append", "read", "attention of few rows", "attention of many", "verification"])
+def test_a_contradiction_does_not_end_the_waits_of_what_follows(gpu, call):
+    """A product whose activations come behind a long launch: all of its rows are there, although a sequence of the step was left out."""
+    rows, cols, batch, lib, h = 23680, 1024, 40, gpu.lib, gpu.handle
+    rng = np.random.default_rng(70)
+    W = np.tile(qn.quantize((rng.standard_normal((32, cols)) * 0.02).astype(np.float32), qn.Q8_0).reshape(32, -1), (rows // 32, 1))
+    x, n = rng.standard_normal((batch, cols)).astype(np.float32), 1 << 23
+    with Dev(gpu) as d:
+        dW, dx, xh, long_row, norm, out = d.up(W), d.f32(x), d.zeros(lib.lv_act_split_bytes(cols, batch)), d.zeros(n * 4), d.zeros(n * 4), d.zeros(batch * rows * 4)
+        pkg.check(lib.lv_act_split_f16(h, xh, dx, None, cols, batch))
+        pkg.check(lib.lv_gemm_tc(h, out, dW, qn.Q8_0, xh, rows, cols, batch, 0))
+        gpu.sync()
+        want = d.get(out, (batch, rows))
+        bad = contradictions(d)[call]
+        gpu.sync()
+        pkg.check(lib.lv_memset(h, out, 255, batch * rows * 4))
+        pkg.check(bad())
+        pkg.check(lib.lv_norm_f32(h, norm, long_row, long_row, n, 1))    # one thread block
+        pkg.check(lib.lv_gemm_tc(h, out, dW, qn.Q8_0, xh, rows, cols, batch, 0))
+        error_word(gpu)
+        assert np.array_equal(d.get(out, (batch, rows)), want)
