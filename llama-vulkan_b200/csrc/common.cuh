@@ -78,14 +78,14 @@ __device__ __forceinline__ bool mbar_poll(uint64_t* bar, uint32_t parity) {
 
 // Waits for the phase with the given parity.  Gives up after kWaitCycleLimit cycles
 // (or at once if another wait already failed), records the failure in *err and
-// returns false; the caller must then stop touching the guarded data.
-__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, uint32_t* err) {
+// returns false; the caller must then stop touching the guarded data.  `ends`: the errors that end the wait at once.
+__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, uint32_t* err, uint32_t ends = 0xffffffffu) {
     if (mbar_test(bar, parity)) return true;
     const long long t0 = clock64();
     for (uint32_t spin = 1;; ++spin) {
         if (mbar_test(bar, parity)) return true;
         if ((spin & 0xffu) == 0) {
-            if (*reinterpret_cast<volatile uint32_t*>(err) != 0) return false;
+            if ((*reinterpret_cast<volatile uint32_t*>(err) & ends) != 0) return false;
             if (clock64() - t0 > kWaitCycleLimit) break;
         }
     }
@@ -95,9 +95,9 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, uint32
 
 // The same for a whole warp: one lane polls (32 lanes that poll one barrier take turns at it, about half a microsecond for
 // the eight warps of a softmax).
-__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, uint32_t* err) {
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, uint32_t* err, uint32_t ends = 0xffffffffu) {
     uint32_t ok = 1;
-    if ((threadIdx.x & 31u) == 0) ok = mbar_wait(bar, parity, err) ? 1u : 0u;
+    if ((threadIdx.x & 31u) == 0) ok = mbar_wait(bar, parity, err, ends) ? 1u : 0u;
     __syncwarp();                                        // what the lane has seen to be there is there for all (a shuffle orders no memory)
     return __shfl_sync(0xffffffffu, ok, 0) != 0;
 }
@@ -112,8 +112,8 @@ __device__ __forceinline__ void mbar_drain(uint64_t* bar, uint32_t parity) {
 // For a whole warp, every lane of which looks at the barrier itself: what it guards is ordered for all without a lane that tells the others.  Whether
 // the wait was lost is put to the vote, since each lane finds out on its own and what follows (elections, shuffles, tcgen05 .sync) needs the whole
 // warp: lanes that went on alone would wait for the others without a limit.
-__device__ __forceinline__ bool mbar_wait_all(uint64_t* bar, uint32_t parity, uint32_t* err) {
-    return __all_sync(0xffffffffu, mbar_wait(bar, parity, err));
+__device__ __forceinline__ bool mbar_wait_all(uint64_t* bar, uint32_t parity, uint32_t* err, uint32_t ends = 0xffffffffu) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, ends));
 }
 
 // 1-D bulk copy global -> shared, completion counted in bytes on `bar`.

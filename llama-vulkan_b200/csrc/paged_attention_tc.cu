@@ -31,6 +31,8 @@ namespace lv {
 // Warps: eight of the softmax, four that convert or mend what was copied, four of which two issue the products and one the copies.  Registers move from the latter eight to the former: a row's 128 scores are held at a
 // time.  512 threads are launched with 128 registers each: (8 x 200 + 8 x 56) x 32 = 512 x 128.
 constexpr int kPtSoftmax = 8, kPtHelpers = 4, kPtThreads = 512, kPtStages = 2, kPtRing = 3, kPtManyRegs = 200, kPtFewRegs = 56;
+// A wait ends at once where another one has been lost, but not for an index that some earlier kernel found out of range: that was reported, and these sequences are in order.
+constexpr uint32_t kPtEnds = ~uint32_t(ERR_BAD_INDEX);
 
 template <int N>
 __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
@@ -244,13 +246,13 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn
             for (uint32_t w = mine; w < units; w += 2) {
                 const uint32_t turn = w >> 1, j = two ? turn : w, st = j % kPtStages;
                 // (after a lost wait the warp goes through the remaining steps without work: the other unit's wait for it)
-                ok = ok && mbar_wait_all(&sh.v_full[st], (j / kPtStages) & 1u, p.err);
+                ok = ok && mbar_wait_all(&sh.v_full[st], (j / kPtStages) & 1u, p.err, kPtEnds);
                 if (!ok) { begin_turn(); pass_turn(w); continue; }
                 const TcMeta& m = sh.meta[st];
                 const int j0 = int(j * kPtKeys);
                 const uint4 there = *reinterpret_cast<const uint4*>(m.there);
                 const bool open = __all_sync(0xffffffffu, (there.x & there.y & there.z & there.w) == 0xffffffffu && j0 + kPtKeys - 1 <= warp_hi && j0 >= warp_lo);
-                ok = mbar_wait_all(&sh.s_full[mine], turn & 1u, p.err);
+                ok = mbar_wait_all(&sh.s_full[mine], turn & 1u, p.err, kPtEnds);
                 if (!ok) { begin_turn(); pass_turn(w); continue; }
                 tc_fence_after_sync();
                 float2 s[kPtKeys / 2];
@@ -348,7 +350,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn
                 pass_turn(w);
                 l += (sums[0].x + sums[1].x) + (sums[0].y + sums[1].y);
             }
-            if (mine < units) ok = ok && mbar_wait_warp_tc(&sh.o_full[mine], 0, p.err);
+            if (mine < units) ok = ok && mbar_wait_warp_tc(&sh.o_full[mine], 0, p.err, kPtEnds);
         }
         float2 part1 = make_float2(-INFINITY, 0.f);                      // reference and sum of the other unit of the same rows
         uint32_t unit1 = 0;
@@ -364,6 +366,8 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn
                 unit1 = sh.unit;
             }
         }
+        if (!ok && p.splits != 1 && row < rows && (two || mine == 0))    // (a lost wait: the join finds that this part saw nothing)
+            p.part_rl[(size_t(q.row0 + (r0 + row) / p.group) * a.heads + kv * p.group + (r0 + row) % p.group) * p.splits + split] = make_float2(-INFINITY, 0.f);
         if (ok && base_row + 32 * quarter < rows && (two || mine == 0)) {
             tc_fence_after_sync();
             const uint32_t t = q.row0 + (r0 + row) / p.group, h = kv * p.group + (r0 + row) % p.group;
@@ -457,7 +461,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn
             ask(step + 2);
             TcMeta& m = sh.meta[st];
             if constexpr (!S::kEight) {
-                ok = mbar_wait_warp(&sh.v_raw[st], (step / kPtStages) & 1u, p.err);
+                ok = mbar_wait_warp(&sh.v_raw[st], (step / kPtStages) & 1u, p.err, kPtEnds);
                 if (!ok) break;
                 if (there != 0xffffffffu)
                     for (uint32_t r = 0; r < 32; ++r)
@@ -468,8 +472,8 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn
 #pragma unroll
                 for (uint32_t values = 0; values < 2; ++values) {
                     const uint32_t item = 2 * step + values, slot = item % kPtRing, stages = values ? kPtStages : S::kKeyStages, to_st = step % stages;
-                    ok = ok && mbar_wait_warp(&sh.raw_full[slot], (item / kPtRing) & 1u, p.err);
-                    if (step >= stages) ok = ok && mbar_wait_warp(values ? &sh.v_empty[to_st] : &sh.k_empty[(step - stages) & 1u], ((step - stages) >> 1) & 1u, p.err);
+                    ok = ok && mbar_wait_warp(&sh.raw_full[slot], (item / kPtRing) & 1u, p.err, kPtEnds);
+                    if (step >= stages) ok = ok && mbar_wait_warp(values ? &sh.v_empty[to_st] : &sh.k_empty[(step - stages) & 1u], ((step - stages) >> 1) & 1u, p.err, kPtEnds);
                     if (!ok) break;
                     const uint8_t* from = s_raw + slot * S::kRaw + my_unit * 16;
                     uint8_t* to = (values ? s_v : s_k) + to_st * S::kTile;
@@ -525,9 +529,9 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn
                 }
                 uint64_t* bar = S::kEight ? &sh.raw_full[slot] : values ? &sh.v_raw[st] : &sh.k_full[st];
                 if constexpr (S::kEight) {
-                    if (item >= kPtRing && !mbar_wait_warp(&sh.raw_empty[slot], (item / kPtRing - 1) & 1u, p.err)) break;
+                    if (item >= kPtRing && !mbar_wait_warp(&sh.raw_empty[slot], (item / kPtRing - 1) & 1u, p.err, kPtEnds)) break;
                 } else {
-                    if (step >= kPtStages && !mbar_wait_warp(values ? &sh.v_empty[st] : &sh.k_empty[st], (step / kPtStages - 1) & 1u, p.err)) break;
+                    if (step >= kPtStages && !mbar_wait_warp(values ? &sh.v_empty[st] : &sh.k_empty[st], (step / kPtStages - 1) & 1u, p.err, kPtEnds)) break;
                 }
                 const uint32_t n = uint32_t(__popc(__ballot_sync(0xffffffffu, here)));
                 if (lane == 0) mbar_expect_tx(bar, n * bytes);
@@ -567,7 +571,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn
         auto step_of = [&](uint32_t w) { return both ? w >> 1 : w; };
         auto wait_keys = [&](uint32_t w) {
             const uint32_t j = step_of(w);
-            return mbar_wait_all(&sh.k_full[j & 1u], (j >> 1) & 1u, p.err);
+            return mbar_wait_all(&sh.k_full[j & 1u], (j >> 1) & 1u, p.err, kPtEnds);
         };
         auto keys = [&](uint32_t w) { return k_desc + (((step_of(w) % S::kKeyStages) * S::kTile) >> 4); };
         // (one lane)
@@ -580,7 +584,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn
             tc_commit(&sh.s_full[mine]);
             tc_commit(&sh.k_empty[step_of(w) & 1u]);
         };
-        bool ok = mine < n && mbar_wait_all(&sh.q_full, 0, p.err) && wait_keys(mine);
+        bool ok = mine < n && mbar_wait_all(&sh.q_full, 0, p.err, kPtEnds) && wait_keys(mine);
         if (ok) {
             tc_fence_after_sync();
             const uint64_t kd = keys(mine);
@@ -591,9 +595,9 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn
             const uint32_t turn = w >> 1, st = step_of(w) % kPtStages;
             const bool more = w + 2 < n;
             // what the products of this turn need beside the weights is waited for first
-            ok = mbar_wait_all(&sh.v_full[st], (step_of(w) / kPtStages) & 1u, p.err) && (!more || wait_keys(w + 2));
+            ok = mbar_wait_all(&sh.v_full[st], (step_of(w) / kPtStages) & 1u, p.err, kPtEnds) && (!more || wait_keys(w + 2));
             const uint64_t vd = v_desc + ((st * S::kTile) >> 4), kd = keys(w + 2);
-            ok = ok && mbar_wait_all(&sh.p_full[mine][0], turn & 1u, p.err);
+            ok = ok && mbar_wait_all(&sh.p_full[mine][0], turn & 1u, p.err, kPtEnds);
             if (!ok) break;
             tc_fence_after_sync();
             if (tc_elect()) {
@@ -602,7 +606,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn
                     tc_mma_f16_ta(o_at, s_at + 8 * k, vd + 128u * k, o_desc, k != 0 ? 1u : uint32_t(turn != 0));
             }
             __syncwarp();
-            ok = mbar_wait_all(&sh.p_full[mine][1], turn & 1u, p.err);
+            ok = mbar_wait_all(&sh.p_full[mine][1], turn & 1u, p.err, kPtEnds);
             if (!ok) break;
             tc_fence_after_sync();
             if (tc_elect()) {

@@ -55,9 +55,9 @@ __device__ __forceinline__ bool tc_elect() {
 
 // mbar_wait_warp for a warp whose next step is tc_load16, an instruction of the whole warp that the fence in front of it orders: without the
 // ordering of ordinary loads by other lanes (0.1 us for each of the ends of a segment in gemm_tc_stream.cu).
-__device__ __forceinline__ bool mbar_wait_warp_tc(uint64_t* bar, uint32_t parity, uint32_t* err) {
+__device__ __forceinline__ bool mbar_wait_warp_tc(uint64_t* bar, uint32_t parity, uint32_t* err, uint32_t ends = 0xffffffffu) {
     uint32_t ok = 1;
-    if ((threadIdx.x & 31u) == 0) ok = mbar_wait(bar, parity, err) ? 1u : 0u;
+    if ((threadIdx.x & 31u) == 0) ok = mbar_wait(bar, parity, err, ends) ? 1u : 0u;
     return __shfl_sync(0xffffffffu, ok, 0) != 0;
 }
 

@@ -146,3 +146,17 @@ def test_a_contradiction_does_not_end_the_waits_of_what_follows(gpu, call):
         pkg.check(lib.lv_gemm_tc(h, out, dW, qn.Q8_0, xh, rows, cols, batch, 0))
         error_word(gpu)
         assert np.array_equal(d.get(out, (batch, rows)), want)
+
+
+@pytest.mark.parametrize("kind", [BF16, E4M3], ids=pp.NAMES.get)
+@pytest.mark.parametrize("lens,new", [([9000, 40, 12001], [70, 40, 33]), ([2500], [900])], ids=["split", "whole"])
+def test_an_earlier_index_out_of_range_does_not_end_the_waits_of_many_rows(gpu, kind, lens, new):
+    rng = np.random.default_rng(len(lens))
+    c = pp.Cache(rng, lens, 1, 64, kind, 64).fill(rng)
+    with Dev(gpu) as d:
+        st = Step(d, c, new, 2, out=F16)
+        cache, row = d.zeros(128), d.f32(np.zeros(64))
+        pkg.check(gpu.lib.lv_kv_append_f16(gpu.handle, cache, row, d.u32([8]), 64, 1, 1))        # row 8 of a cache of one row
+        st.launch()
+        error_word(gpu)
+        st.check()
