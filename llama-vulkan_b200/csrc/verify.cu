@@ -200,7 +200,8 @@ __global__ void __launch_bounds__(kProbThreads, 3) probabilities_kernel(const Pr
 
 // A cluster of eight CTAs takes a sequence.  Every CTA finds the first rejected draft by itself (two values a draft), then they sum the weights of the one row that
 // a token is drawn from, each an eighth of it and every warp a run of neighbours, and tell one another their sums.  The bounds between runs are the same numbers
-// for both neighbours, so that exactly one run holds the target; its warp looks through it again.  Sums are f64: the first index whose cumulative weight is above
+// for both neighbours and never decrease, and the target is below the last one (pick is at most 1 - 2^-24), so that exactly one run holds it, one with weight; its warp looks through it
+// again.  Sums are f64: the first index whose cumulative weight is above
 // the target does not depend on the order of the sums but where the two agree to 2^-52.
 // 64 sequences with up to 7 drafts, vocabulary 128000: 22 us, 3.0 TB/s of 65 MB: two CTAs per SM by their registers, so 1.7 rounds that each wait for look-ups and loads (one CTA per
 // sequence: 110 us; 256 threads: 20.7, but 4.65 for one sequence; clusters of four: 21.1 and 4.9).  One
@@ -307,12 +308,10 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const lv_verify_
         if (lane == 0) s_before[warp + 1] = mine;
         __syncthreads();
         if (warp == 0) {
-            double run = lane < kVerifyWarps ? s_before[lane + 1] : 0.0;
+            // one after the other: every bound is the one before plus what lies between, so that bounds rise, and stay where a run has no weight
+            double run = 0.0;
 #pragma unroll
-            for (int o = 1; o < kVerifyWarps; o <<= 1) {
-                const double up = __shfl_up_sync(0xffffffffu, run, o);
-                if (lane >= uint32_t(o)) run += up;
-            }
+            for (uint32_t w = 0; w < kVerifyWarps; ++w) run += w <= lane ? s_before[w + 1] : 0.0;
             __syncwarp();
             if (lane < kVerifyWarps) s_before[lane + 1] = run;
             if (lane == 0) s_before[0] = 0.0;
@@ -344,11 +343,10 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const lv_verify_
             }
         }
     }
-    // the run that holds the target: bounds are sums in a fixed order, the last one of a CTA is the first one of the next
+    // the run that holds the target: the last bound of a CTA is the first one of the next (its warps' sums and the CTAs' are added up in order)
     const double target = double(pick) * total;
     const double from = cta0 + s_before[warp], to = warp + 1 == kVerifyWarps ? cta1 : cta0 + s_before[warp + 1];
-    const bool last = rank + 1 == kVerifyCluster && warp + 1 == kVerifyWarps;
-    if (!drawn || !(from <= target) || !(target < to || last)) return;
+    if (!drawn || !(from <= target && target < to)) return;
     double run = from;
     uint32_t found = kNobody, fallback = kNobody;
     for (uint32_t k = 0; k < each && found == kNobody; ++k) {

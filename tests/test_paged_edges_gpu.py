@@ -1,5 +1,6 @@
 """The cache in pages, the attention over it, probabilities and verification where their inputs contradict themselves or reach the ends of their ranges."""
 import ctypes as C
+from fractions import Fraction
 
 import numpy as np
 import pytest
@@ -9,7 +10,7 @@ import quant_np as qn
 from conftest import load_pkg
 from device_data import Dev
 from paged_plain import BF16, E4M3, F16, F32, I8
-from test_paged_gpu import Step, error_word
+from test_paged_gpu import Step, error_word, run_verify
 
 pytestmark = pytest.mark.gpu
 pkg = load_pkg()
@@ -160,3 +161,56 @@ def test_an_earlier_index_out_of_range_does_not_end_the_waits_of_many_rows(gpu, 
         st.launch()
         error_word(gpu)
         st.check()
+
+
+# ---- verification: the bounds between runs --------------------------------------------------------
+
+def sums_by_halves(s):
+    """Running sums in float64 that add up in pairs of runs, so that each has brackets of its own."""
+    run, o = [float(x) for x in s], 1
+    while o < len(run):
+        run = [run[i] + run[i - o] if i >= o else run[i] for i in range(len(run))]
+        o *= 2
+    return run
+
+
+def rows_with_a_gap():
+    """(weights of 16 runs, weights behind them, run): half of the whole weight is the running sum behind `run`, where the next one, without any weight, has a larger one by halves."""
+    cases = []
+    for seed in range(400):
+        rng = np.random.default_rng(seed)
+        s = (rng.random(16) * 2.0 ** rng.integers(-40, 0, 16)).astype(np.float32)
+        s[rng.integers(8, 15):] = 0
+        p = sums_by_halves(s)
+        for i in range(15):
+            if s[i + 1] == 0 and p[i + 1] > p[i]:
+                rest, left = [], 2 * p[i] - p[15]
+                for _ in range(3):
+                    h = np.float32(left)
+                    h = np.nextafter(h, np.float32(0)) if float(h) > left else h
+                    rest.append(h)
+                    left -= float(h)
+                if left == 0 and p[15] + (2 * p[i] - p[15]) == 2 * p[i]:
+                    cases.append((s, rest, i))
+                break
+    return cases
+
+
+def test_a_pick_between_two_runs_draws_a_token(gpu):
+    """Each warp sums a run of 128 values (a vocabulary of 16384 is 8 x 16 of them) and asks whether the target lies in its run: between the bounds of one and the next there
+    must be no gap, and none at all around a run without weight."""
+    cases = rows_with_a_gap()
+    assert len(cases) > 30
+    target = np.zeros((len(cases), 16384), np.float32)
+    for row, (s, rest, _) in zip(target, cases):
+        row[np.arange(16) * 128] = s
+        row[np.arange(16, 16 + len(rest)) * 128] = rest
+    n = len(cases)
+    accepted, tokens, _, failed = run_verify(gpu, target, None, np.zeros(n, np.uint32), np.arange(n + 1), np.zeros(n, np.float32), np.full(n, 0.5, np.float32))
+    assert failed is None and (accepted == 0).all()
+    for row, token in zip(target, tokens):
+        assert token < 16384 and row[token] > 0                          # (77 where nothing was written)
+        before = sum((Fraction(float(x)) for x in row[:token]), Fraction(0))
+        whole = sum((Fraction(float(x)) for x in row), Fraction(0))
+        slack = whole / 2 ** 50                                          # (19 additions of 2^-53 each)
+        assert before <= whole / 2 + slack and before + Fraction(float(row[token])) > whole / 2 - slack
