@@ -719,10 +719,11 @@ typedef struct lv_paged_attention_args {
 size_t lv_paged_attention_scratch_bytes(lv_ctx* ctx, const lv_paged_attention_args* a);
 int lv_paged_attention(lv_ctx* ctx, const lv_paged_attention_args* a, void* scratch, size_t scratch_bytes);
 
-/* out[r] = softmax(logits[r] / temperature[r]) over vocab values, f32 [rows][out_ld] and [rows][ld]; temperature f32 [rows] (device), not negative, null: 1
- * everywhere.  Temperature 0: one at the first index of the maximum, zero elsewhere (NaN never is the maximum; a row of nothing else: index 0).  A row of
- * nothing but -infinity gets zeros at any other temperature.
- * out may be logits (with the same stride). */
+/* out[r] = softmax(logits[r] / temperature[r]) over vocab values, f32 [rows][out_ld] and [rows][ld]; temperature f32 [rows] (device), null: 1 everywhere.
+ * Temperature 0: one at the first index of the maximum, zero elsewhere (NaN never is the maximum; a row of nothing else: index 0).  A row of nothing but
+ * -infinity gets zeros at any other temperature.  Infinite temperature: the same for all values but -infinity, which get zero.  A temperature that is
+ * negative or NaN gives NaN.
+ * out may be logits (with the same stride); otherwise they do not overlap. */
 int lv_probabilities(lv_ctx* ctx, float* out, uint32_t out_ld, const float* logits, uint32_t ld, uint32_t vocab, uint32_t rows, const float* temperature);
 
 /* Drafted tokens against the target's probabilities, from given random numbers (speculative sampling: what comes out is distributed as if drawn from the

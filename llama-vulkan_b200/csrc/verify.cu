@@ -63,7 +63,8 @@ __global__ void __launch_bounds__(kProbThreads, 3) probabilities_kernel(const Pr
     const float* x = p.logits + size_t(row) * p.ld;
     float* y = p.out + size_t(row) * p.out_ld;
     const float T = p.temperature ? p.temperature[row] : 1.f;
-    const float f = T == 0.f ? 1.f : fminf(1.4426950408889634f / T, FLT_MAX);        // e^(z / T) as a power of two (finite: zero times infinity is NaN)
+    // e^(z / T) as a power of two.  Finite and above zero: zero times infinity is NaN, for equal values as well as for what lies behind the end
+    const float f = T == 0.f ? 1.f : T > 0.f ? fmaxf(fminf(1.4426950408889634f / T, FLT_MAX), __uint_as_float(1u)) : NAN;
     const uint32_t lo = min(p.vocab, rank * p.each), hi = min(p.vocab, lo + p.each);
     // values i .. i + 3; those behind the end count as -inf.  (Vectors first, the few values behind the last whole one in a branch of their own: the loads of
     // several calls are on their way together.)

@@ -214,3 +214,40 @@ def test_a_pick_between_two_runs_draws_a_token(gpu):
         whole = sum((Fraction(float(x)) for x in row), Fraction(0))
         slack = whole / 2 ** 50                                          # (19 additions of 2^-53 each)
         assert before <= whole / 2 + slack and before + Fraction(float(row[token])) > whole / 2 - slack
+
+
+# ---- probabilities: temperatures at the ends --------------------------------------------------------
+
+@pytest.mark.parametrize("vocab", [1, 50, 32000, 40001, 300002])
+@pytest.mark.parametrize("rows", [1, 60])
+def test_probabilities_at_the_largest_temperatures(gpu, vocab, rows):
+    """A temperature without end leaves no differences but that -infinity has no weight; 3e38 next to none."""
+    x = (np.random.default_rng(vocab).standard_normal((rows, vocab)) * 5).astype(np.float32)
+    if vocab > 1:
+        x[:, ::3] = -np.inf
+        x[:, 1] = 1e30
+    there = np.isfinite(x)
+    want = there / there.sum(1, keepdims=True)
+    with Dev(gpu) as d:
+        dx = d.f32(x)
+        for T in (np.inf, 3e38, 1.5e38):
+            out = d.zeros(x.nbytes)
+            d.call("lv_probabilities", out, vocab, dx, vocab, vocab, rows, d.f32(np.full(rows, T)))
+            got = d.get(out, x.shape)
+            # exponents are at most 1e30 / 1.5e38 < 2^-26; equal values sum to whole numbers of up to 2^24 in any order, the quotient is rounded twice
+            assert (got[~there] == 0).all() and (np.abs(got - want) <= 2.0 ** -22 * want).all()
+
+
+def test_temperatures_that_are_none(gpu):
+    """Negative or not a number: not a number, beside rows that are in order; minus zero is zero."""
+    for vocab in (700, 200001):
+        x = np.random.default_rng(vocab).standard_normal((5, vocab)).astype(np.float32)
+        x[1, 3] = -np.inf
+        with Dev(gpu) as d:
+            out = d.zeros(x.nbytes)
+            d.call("lv_probabilities", out, vocab, d.f32(x), vocab, vocab, 5, d.f32([np.nan, -1.0, -np.inf, -0.0, 1.0]))
+            got = d.get(out, x.shape)
+        assert np.isnan(got[:3]).all()
+        assert got[3, x[3].argmax()] == 1.0 and got[3].sum() == 1.0
+        e = np.exp(x[4].astype(np.float64) - x[4].max())
+        assert np.abs(got[4] - e / e.sum()).max() <= 1e-6
