@@ -251,3 +251,19 @@ def test_temperatures_that_are_none(gpu):
         assert got[3, x[3].argmax()] == 1.0 and got[3].sum() == 1.0
         e = np.exp(x[4].astype(np.float64) - x[4].max())
         assert np.abs(got[4] - e / e.sum()).max() <= 1e-6
+
+
+@pytest.mark.parametrize("vocab", [1, 3, 700, 32000, 40001, 300002])
+def test_the_first_minus_infinity_of_a_row_without_numbers(gpu, vocab):
+    """At temperature 0 it is the maximum of a row of -infinity and NaN, wherever it lies, also where the values of a thread end behind it."""
+    places = sorted({0, vocab // 3, vocab // 2, vocab - 2, vocab - 1} & set(range(vocab)))
+    x = np.full((len(places) + 1, vocab), np.nan, np.float32)
+    for r, at in enumerate(places):
+        x[r, at:] = np.where(np.arange(vocab - at) % 2 == 0, -np.inf, np.nan)
+    with Dev(gpu) as d:
+        out = d.zeros(x.nbytes)
+        d.call("lv_probabilities", out, vocab, d.f32(x), vocab, vocab, len(x), d.f32(np.zeros(len(x))))
+        got = d.get(out, x.shape)
+    want = np.zeros(x.shape)
+    want[np.arange(len(x)), places + [0]] = 1.0
+    assert np.array_equal(got, want)
