@@ -735,7 +735,8 @@ int lv_probabilities(lv_ctx* ctx, float* out, uint32_t out_ld, const float* logi
  *   nothing), from target behind the last one: the first index whose cumulative weight is above pick[s] * the whole weight
  * accepted[s]: number of drafts accepted; tokens[starts[s] ..]: the accepted drafts, the drawn token, then 0xFFFFFFFF.  A sequence without rows accepts 0 and draws nothing;
  * a draft >= vocab is reported through the error word and rejected; a row without weight or of infinite weight, and a pick outside [0, 1), are reported, the token 0xFFFFFFFF.
- * lens (may be null): lens[s] -= number of rejected drafts, whose rows in a paged cache are overwritten by the next step.
+ * lens (may be null): lens[s] -= number of rejected drafts, whose rows in a paged cache are overwritten by the next step (a smaller length is reported and
+ * stays).
  * accept, pick: in [0, 1).  Weights are summed in f64. */
 typedef struct lv_verify_args {
     const float* target;

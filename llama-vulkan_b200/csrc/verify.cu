@@ -340,7 +340,11 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const lv_verify_
             if (i != accepted) a.tokens[row0 + i] = i < accepted ? a.drafted[row0 + i] : kNobody;
         if (threadIdx.x == 0) {
             a.accepted[s] = accepted;
-            if (a.lens) a.lens[s] -= n - accepted;
+            if (a.lens) {
+                const uint32_t len = a.lens[s], gone = n - accepted;
+                if (len >= gone) a.lens[s] = len - gone;
+                else atomicOr(err, ERR_BAD_INDEX);
+            }
             if (!drawn) {
                 a.tokens[r] = kNobody;
                 atomicOr(err, ERR_BAD_INDEX);

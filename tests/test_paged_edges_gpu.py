@@ -267,3 +267,16 @@ def test_the_first_minus_infinity_of_a_row_without_numbers(gpu, vocab):
     want = np.zeros(x.shape)
     want[np.arange(len(x)), places + [0]] = 1.0
     assert np.array_equal(got, want)
+
+
+# ---- verification: lengths ----------------------------------------------------------------------------
+
+def test_lengths_shorter_than_what_is_rejected(gpu):
+    """They stay as they are and are reported; the tokens are drawn all the same, and other sequences' lengths shortened."""
+    target, draft = np.full((9, 16), 1 / 16, np.float32), np.full((9, 16), 1 / 16, np.float32)
+    draft[:, 3] = 1.0
+    starts, drafted, accept = [0, 4, 8, 9], np.full(9, 3, np.uint32), np.full(9, 0.9, np.float32)        # (0.9 is above 1 / 16: all rejected)
+    for lens, want, wrong in (([2, 10, 0], [2, 7, 0], True), ([3, 3, 0], [0, 0, 0], False)):
+        n, t, left, failed = run_verify(gpu, target, draft, drafted, starts, accept, np.full(3, 0.5, np.float32), lens)
+        assert list(n) == [0, 0, 0] and list(left) == want and failed == (pkg.LV_ERR_DEVICE_WAIT if wrong else None)
+        assert (t[[0, 4, 8]] < 16).all() and (t[[1, 2, 3, 5, 6, 7]] == 0xFFFFFFFF).all()
