@@ -210,12 +210,12 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn
             for (int k = 0; k < kBatch; ++k) {
                 float4 x = unpack_raw4(raw[k], a.q_type);
                 if (a.angles != nullptr) x = rotate4(x, turn[k][0], turn[k][1]);
-                float f = a.scale * kPaLog2e;
+                // (the scale is the scores' factor, in f32: bf16 queries that are not rotated enter as they are)
+                float f = 1.f;
                 if constexpr (!S::kBf16) {
                     const float top = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
-                    const float u = paged_row_unit(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top))));
-                    if (lane == 0) sh.factor[i0 + k] = f / u;
-                    f = u;
+                    f = paged_row_unit(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top))));
+                    if (lane == 0) sh.factor[i0 + k] = a.scale * kPaLog2e / f;
                 }
                 if (d < D) *reinterpret_cast<uint2*>(s_q + ((i0 + k) >> 7) * S::kTile + tile_at((i0 + k) & 127u, d >> 3) + (d & 4u) * 2) =
                     make_uint2(pack16<S::kBf16>(x.x * f, x.y * f), pack16<S::kBf16>(x.z * f, x.w * f));
@@ -231,7 +231,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn
         uint32_t unit = 0;
         bool ok = true;
         if (base_row + 32 * quarter < rows) {
-            const float row_factor = S::kBf16 ? 1.f : sh.factor[row];
+            const float row_factor = S::kBf16 ? a.scale * kPaLog2e : sh.factor[row];
             const uint32_t pos = before + (r0 + min(row, rows - 1)) / p.group;
             const int key_hi = row < rows ? int(pos) - int(lo) : -1, key_lo = int(paged_first_key(pos, a.window)) - int(lo);
             // keys that every row of the warp sees
@@ -288,7 +288,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn
                     for (int i = 32 * half; i < 32 * half + 32; ++i) tops[i & 3] = max3(tops[i & 3], s[i].x, s[i].y);
                 }
                 float top = max3(max3(tops[0], tops[1], tops[2]), tops[3], tops[3]);
-                if constexpr (!S::kBf16) top *= row_factor;              // (the scale over a power of two: positive)
+                top *= row_factor;                                       // (the scale, over a power of two: positive)
                 float keep = 1.f;
                 bool moved = false;
                 if constexpr (S::kEight) {
@@ -328,7 +328,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn
                     uint32_t u[32];
 #pragma unroll
                     for (int i = 0; i < 32; ++i) {
-                        const float2 z = s[32 * half + i], x = S::kBf16 ? add2(z, minus) : fma2(z, factor, minus);
+                        const float2 z = s[32 * half + i], x = fma2(z, factor, minus);
                         float2 e = make_float2(exp2_fast(x.x), exp2_fast(x.y));
                         sums[i & 1] = add2(sums[i & 1], e);
                         if constexpr (S::kEight) {

@@ -280,3 +280,51 @@ def test_lengths_shorter_than_what_is_rejected(gpu):
         n, t, left, failed = run_verify(gpu, target, draft, drafted, starts, accept, np.full(3, 0.5, np.float32), lens)
         assert list(n) == [0, 0, 0] and list(left) == want and failed == (pkg.LV_ERR_DEVICE_WAIT if wrong else None)
         assert (t[[0, 4, 8]] < 16).all() and (t[[1, 2, 3, 5, 6, 7]] == 0xFFFFFFFF).all()
+
+
+# ---- attention: as many bits as the header says --------------------------------------------------------
+
+def attend_tight(c, starts, q, heads, scale, out_kind, uq, up, terms, angles=None):
+    """(out, bound) like paged_plain.attend, for queries and weights whose relative errors are at most uq and up, and queries with `terms` values that are not zero.
+
+    A product of |q| |k| is exact in f32 where one number has 8 or 11 bits and within 2^-24 elsewhere, `terms` products and planes add up with one rounding of the running sum each, the
+    factors take four more: a score is off by d = (uq + (3 terms + 8) 2^-24) scale sum |q| |k|; f16 queries also by 2^-25 of the row's largest value per key value (they are
+    whole multiples of that).  A quotient of weights is off by 2 d, by 2^-22 |s| + 2^-19 for the exponentials, and n 2^-24 for the sums; the numerator's weights by up, f16 weights also by 2^-35 of the
+    largest one each (see paged_plain).  Together times sum p |v|, and the rounding of the result."""
+    x = pp.rotate(q, angles).astype(np.float64)
+    G, dim = heads // c.H, c.dim
+    out, bound = np.zeros((2,) + x.shape)
+    for s, n in enumerate(c.lens):
+        m = int(starts[s + 1]) - int(starts[s])
+        k, v = (c.read(s, np.arange(n), w) for w in range(2))
+        for i in range(m):
+            t, at = int(starts[s]) + i, n - m + i
+            for h in range(heads):
+                kk, vv = k[:at + 1, h // G], v[:at + 1, h // G]
+                z = scale * (kk @ x[t, h])
+                p = np.exp(z - z.max())
+                p /= p.sum()
+                size = scale * (np.abs(kk) @ np.abs(x[t, h])).max()
+                d = (uq + (3 * terms + 8) * 2.0 ** -24) * size
+                floor = 0.0
+                if c.kind != BF16:
+                    d += 2.0 ** -25 * scale * np.abs(x[t, h]).max() * np.abs(kk).sum(1).max()
+                    floor = len(z) * 2.0 ** -35 * np.abs(vv).max()
+                out[t, h] = p @ vv
+                bound[t, h] = floor + (np.expm1(2 * d) + up + 2.0 ** -19 + 2.0 ** -22 * size + len(z) * 2.0 ** -24) * (p @ np.abs(vv))
+    bound += pp.HALF_STEP[out_kind] * (np.abs(out) + bound) + 1e-30 + (2.0 ** -25 if out_kind == F16 else 0)
+    return out, bound
+
+
+@pytest.mark.parametrize("out", [BF16, F16], ids=["to-bf16", "to-f16"])
+@pytest.mark.parametrize("scale", [None, 0.1, 0.9])
+def test_queries_that_fit_enter_many_rows_unrounded(gpu, out, scale):
+    """bf16 queries without a rotation over a bf16 cache: the scale is applied to the scores, so that large ones are off by the sums' roundings alone."""
+    rng = np.random.default_rng(9)
+    c = pp.Cache(rng, [160, 90], 1, 64, BF16, 16).fill(rng)
+    with Dev(gpu) as d:
+        st = Step(d, c, [50, 40], 2, out=out, given=BF16, size=30.0 * 0.125 / (scale or 0.125), scale=scale, behind=0)
+        got = st.launch().result()
+        want, bound = attend_tight(c, st.starts, st.q.reshape(90, 2, 64), 2, st.scale, out, 0.0, pp.HALF_STEP[BF16], 64)
+        worst = (np.abs(got - want) / bound).max()
+        assert worst <= 1.0, worst
