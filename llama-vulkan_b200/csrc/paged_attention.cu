@@ -155,6 +155,7 @@ extern "C" int lv_paged_attention(lv_ctx* ctx, const lv_paged_attention_args* a,
     p.a = *a;
     p.c = paged_cache(a->cache);
     p.group = a->heads / a->cache.kv_heads;
+    p.factor = paged_factor(a->scale * kPaLog2e, 1.f);
     p.chunk = plan.chunk;
     p.splits = plan.splits;
     p.align = plan.many ? kPtKeys - 1 : 0;

@@ -1,6 +1,8 @@
 // Pieces of the two kernels of the attention over pages: what they are given, the rows that a sequence's new tokens are, and partial results.
 #pragma once
 
+#include <float.h>
+
 #include "paged.cuh"
 
 namespace lv {
@@ -21,6 +23,7 @@ struct PagedAttn {
     uint32_t chunk, splits;      // keys of a split (from the first key that a block of rows sees on), upper bound of the splits
     uint32_t align;              // splits begin at the block's first key with these bits cleared
     uint32_t box;                // rows of a TMA box (the kernel for many rows)
+    float factor;                // the scale in log2 units
     float* part_o;               // [token][head][split][dim]: sums of the splits
     float2* part_rl;             // [token][head][split]: reference and sum of weights
     uint32_t *err, *data_err;    // of waits; of what sequences contain
@@ -42,6 +45,10 @@ __device__ __forceinline__ bool paged_attention_seq(const PagedAttn& p, uint32_t
     if (threadIdx.x == 0) atomicOr(p.data_err, ERR_BAD_INDEX);
     return false;
 }
+
+// What a row's products are multiplied by: the scale in log2 units, over the power of two of the row's queries.  Above zero and finite, so that it times zero is zero and times
+// -infinity is that
+__host__ __device__ __forceinline__ float paged_factor(float scale, float unit) { return fminf(fmaxf(scale / unit, 0x1p-149f), FLT_MAX); }
 
 // the weight of a head's sink, and the least reference that it fits under
 __device__ __forceinline__ float paged_sink(const PagedAttn& p, uint32_t head) { return p.a.sink ? p.a.sink[head] * kPaLog2e : -INFINITY; }

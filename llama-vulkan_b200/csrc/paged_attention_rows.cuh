@@ -187,7 +187,7 @@ __global__ void __launch_bounds__(32 * kPrWarps, D == 256 ? 1 : NT == 1 ? 4 : NT
             }
             float f = 1.f;                                               // 2^-e of the largest value (f16 operands)
             if constexpr (!S::kBf16) f = paged_row_unit(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top))));
-            if (lane == 0) s_factor[r] = a.scale * kPaLog2e / f;
+            if (lane == 0) s_factor[r] = paged_factor(p.factor, f);
 #pragma unroll
             for (int i = 0; i < kParts; ++i) {
                 const uint32_t d = 4 * (lane + 32 * i);

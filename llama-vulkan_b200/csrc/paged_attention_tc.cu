@@ -215,7 +215,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn
                 if constexpr (!S::kBf16) {
                     const float top = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
                     f = paged_row_unit(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top))));
-                    if (lane == 0) sh.factor[i0 + k] = a.scale * kPaLog2e / f;
+                    if (lane == 0) sh.factor[i0 + k] = paged_factor(p.factor, f);
                 }
                 if (d < D) *reinterpret_cast<uint2*>(s_q + ((i0 + k) >> 7) * S::kTile + tile_at((i0 + k) & 127u, d >> 3) + (d & 4u) * 2) =
                     make_uint2(pack16<S::kBf16>(x.x * f, x.y * f), pack16<S::kBf16>(x.z * f, x.w * f));
@@ -231,7 +231,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const PagedAttn
         uint32_t unit = 0;
         bool ok = true;
         if (base_row + 32 * quarter < rows) {
-            const float row_factor = S::kBf16 ? a.scale * kPaLog2e : sh.factor[row];
+            const float row_factor = S::kBf16 ? p.factor : sh.factor[row];
             const uint32_t pos = before + (r0 + min(row, rows - 1)) / p.group;
             const int key_hi = row < rows ? int(pos) - int(lo) : -1, key_lo = int(paged_first_key(pos, a.window)) - int(lo);
             // keys that every row of the warp sees

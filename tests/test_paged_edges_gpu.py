@@ -328,3 +328,18 @@ def test_queries_that_fit_enter_many_rows_unrounded(gpu, out, scale):
         want, bound = attend_tight(c, st.starts, st.q.reshape(90, 2, 64), 2, st.scale, out, 0.0, pp.HALF_STEP[BF16], 64)
         worst = (np.abs(got - want) / bound).max()
         assert worst <= 1.0, worst
+
+
+@pytest.mark.parametrize("kind", [F16, BF16, I8], ids=pp.NAMES.get)
+@pytest.mark.parametrize("new", [2, 50])
+@pytest.mark.parametrize("out", [F32, BF16], ids=["to-f32", "to-bf16"])
+@pytest.mark.parametrize("scale", [1e-45, 1e-30, 3e38])
+def test_rows_of_zeros_at_any_scale(gpu, kind, new, out, scale):
+    """All scores are zero: the mean of the values, whatever the scale."""
+    rng = np.random.default_rng(new)
+    c = pp.Cache(rng, [140], 1, 64, kind, 16).fill(rng)
+    with Dev(gpu) as d:
+        st = Step(d, c, [new], 2, out=out, scale=scale, size=0.0, behind=0)
+        got = st.launch().result()
+        want, bound = attend_tight(c, st.starts, st.q.reshape(new, 2, 64), 2, st.scale, out, 0.0, pp.HALF_STEP[BF16 if kind == BF16 else F16], 64)
+        assert (np.abs(got - want) <= bound).all()
