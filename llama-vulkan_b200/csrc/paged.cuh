@@ -81,6 +81,8 @@ __host__ __device__ __forceinline__ bool paged_is8(int type) { return type == LV
 __host__ __device__ __forceinline__ uint32_t paged_bytes(int type) { return type == LV_TYPE_F32 ? 4u : paged_is8(type) ? 1u : 2u; }
 inline bool paged_value_type(int type) { return type == LV_TYPE_F32 || type == LV_TYPE_F16 || type == LV_TYPE_BF16; }
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+template <typename... P>
+inline bool words_aligned(const P*... p) { return ((... | reinterpret_cast<uintptr_t>(p)) & 3u) == 0; }
 
 // Four consecutive values of type f32, f16 or bf16 (the type is the same for a whole launch)
 __device__ __forceinline__ float4 unpack_values4(uint2 u, int type) {
@@ -170,6 +172,7 @@ inline int paged_check(const lv_paged_cache* c) {
     LV_REQUIRE(uint64_t(c->table_ld) * c->page_rows <= 0x7fffffffull, "paged cache: positions of a sequence are below 2^31");
     LV_REQUIRE(uint64_t(c->pages) * c->page_rows <= 0xffffffffull && uint64_t(c->pages) * c->page_rows * c->kv_heads <= 0xffffffffull, "paged cache: rows are below 2^32");
     LV_REQUIRE(aligned16(c->k) && aligned16(c->v), "paged cache: k and v are 16-byte aligned");
+    LV_REQUIRE(words_aligned(c->table, c->lens, c->starts) && (!paged_is8(c->type) || words_aligned(c->k_scale, c->v_scale)), "paged cache: 32-bit values are 4-byte aligned");
     return LV_OK;
 }
 inline int paged_check_rotation(const float* angles, uint32_t angle_ld, uint32_t angle_pairs, uint32_t dim) {

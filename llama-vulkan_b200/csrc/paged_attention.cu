@@ -132,6 +132,7 @@ static int paged_attention_check(const lv_paged_attention_args* a) {
     LV_REQUIRE(a->max_new <= a->tokens && a->max_new <= a->max_len && a->max_len <= uint64_t(a->cache.table_ld) * a->cache.page_rows, "paged attention: bad upper bounds");
     LV_REQUIRE(uint64_t(a->tokens) * a->heads < (uint64_t(1) << 31), "paged attention: too many tokens");
     LV_REQUIRE(a->scale > 0.f && isfinite(a->scale), "paged attention: scale");
+    LV_REQUIRE(words_aligned(a->sink), "paged attention: 32-bit values are 4-byte aligned");
     return paged_check_rotation(a->angles, a->angle_ld, a->angle_pairs, a->cache.dim);
 }
 

@@ -395,6 +395,7 @@ extern "C" int lv_probabilities(lv_ctx* ctx, float* out, uint32_t out_ld, const 
     LV_REQUIRE(out && logits && vocab && out_ld >= vocab && ld >= vocab, "probabilities: bad arguments");
     LV_REQUIRE(vocab <= (1u << 24) && rows < (1u << 27), "probabilities: vocabulary larger than 16777216 or too many rows");
     LV_REQUIRE(out != logits || out_ld == ld, "probabilities: in place, the strides are the same");
+    LV_REQUIRE(words_aligned(out, logits, temperature), "probabilities: 32-bit values are 4-byte aligned");
     LV_ENTER(ctx);
     if (!rows) return LV_OK;
     Probabilities p{out, logits, temperature, out_ld, ld, vocab, 0};
@@ -414,6 +415,7 @@ extern "C" int lv_verify_drafts(lv_ctx* ctx, const lv_verify_args* a) {
     LV_REQUIRE(a && a->target && a->drafted && a->starts && a->accept && a->pick && a->tokens && a->accepted, "verification of drafts: null argument");
     LV_REQUIRE(a->vocab && a->vocab <= (1u << 24) && a->target_ld >= a->vocab && (!a->draft || a->draft_ld >= a->vocab), "verification of drafts: bad sizes");
     LV_REQUIRE(a->seqs && a->seqs < (1u << 28) && a->rows < (1u << 31), "verification of drafts: too many rows");
+    LV_REQUIRE(words_aligned(a->target, a->draft, a->drafted, a->starts, a->accept, a->pick, a->tokens, a->accepted, a->lens), "verification of drafts: 32-bit values are 4-byte aligned");
     LV_ENTER(ctx);
     const bool vec = aligned16(a->target) && a->target_ld % 4 == 0 && aligned16(a->draft) && (!a->draft || a->draft_ld % 4 == 0);
     LV_CUDA(launch_pdl_cluster(ctx, vec ? verify_kernel<true> : verify_kernel<false>, dim3(a->seqs * kVerifyCluster), dim3(kVerifyThreads), dim3(kVerifyCluster), 0, *a, ctx->data_err()));
