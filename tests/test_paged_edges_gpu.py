@@ -10,7 +10,7 @@ import quant_np as qn
 from conftest import load_pkg
 from device_data import Dev
 from paged_plain import BF16, E4M3, F16, F32, I8
-from test_paged_gpu import Step, error_word, run_verify
+from test_paged_gpu import Step, error_word, padded, run_verify
 
 pytestmark = pytest.mark.gpu
 pkg = load_pkg()
@@ -343,3 +343,42 @@ def test_rows_of_zeros_at_any_scale(gpu, kind, new, out, scale):
         got = st.launch().result()
         want, bound = attend_tight(c, st.starts, st.q.reshape(new, 2, 64), 2, st.scale, out, 0.0, pp.HALF_STEP[BF16 if kind == BF16 else F16], 64)
         assert (np.abs(got - want) <= bound).all()
+
+
+# relative error of what enters the products for up to 32 rows: the numbers that a value enters as leave 2^-11 (f16) or 2^-8 (bf16) of it each
+FEW = {(BF16, F32): 2.0 ** -24, (BF16, BF16): 2.0 ** -16, (BF16, F16): 2.0 ** -16, (F16, F32): 2.0 ** -22, (F16, F16): 2.0 ** -22, (F16, BF16): 2.0 ** -11, (I8, F32): 2.0 ** -22,
+       (I8, F16): 2.0 ** -11, (I8, BF16): 2.0 ** -11, (E4M3, F32): 2.0 ** -22, (E4M3, F16): 2.0 ** -11, (E4M3, BF16): 2.0 ** -11}
+
+
+@pytest.mark.parametrize("kind,out", FEW, ids=[f"{pp.NAMES[k]}-to-{pp.NAMES[o]}" for k, o in FEW])
+@pytest.mark.parametrize("size", [0.3, 150.0])
+def test_few_rows_have_the_bits_that_the_header_states(gpu, kind, out, size):
+    """Queries of two values, so that sums hide nothing: with large scores a number that is missing from the queries shows, with small ones and few keys one that is
+    missing from the weights."""
+    rng = np.random.default_rng(31)
+    lens = [2, 3, 4, 3, 2, 4, 5, 7] * 3
+    c = pp.Cache(rng, lens, 1, 64, kind, 16).fill(rng)
+    u = FEW[kind, out]
+    with Dev(gpu) as d:
+        st = Step(d, c, [1] * len(lens), 4, out=out, size=size, behind=0)
+        q = st.q.reshape(len(lens), 4, 64)
+        q[..., [i for i in range(64) if i not in (3, 40)]] = 0
+        st.a.q = d.up(padded(q.reshape(len(lens), -1), st.ld, F32, 0.0)).value
+        got = st.launch().result()
+        want, bound = attend_tight(c, st.starts, q, 4, st.scale, out, u, u, 2)
+        worst = (np.abs(got - want) / bound).max()
+        assert worst <= 1.0, worst
+
+
+def test_f32_results_of_many_rows_have_them_too(gpu):
+    rng = np.random.default_rng(32)
+    for kind in (F16, BF16, I8, E4M3):
+        c = pp.Cache(rng, [60, 9], 1, 64, kind, 16).fill(rng)
+        with Dev(gpu) as d:
+            st = Step(d, c, [40, 9], 4, out=F32, size=20.0, behind=0)
+            q = st.q.reshape(49, 4, 64)
+            q[..., 2:] = 0
+            st.a.q = d.up(padded(q.reshape(49, -1), st.ld, F32, 0.0)).value
+            got = st.launch().result()
+            want, bound = attend_tight(c, st.starts, q, 4, st.scale, F32, FEW[kind, F32], FEW[kind, F32], 2)
+            assert (np.abs(got - want) <= bound).all()
