@@ -680,8 +680,9 @@ int lv_paged_locate(const lv_paged_cache* cache, const uint32_t* table_row, uint
 
 /* Keys and values of the new tokens (k, v: [tokens][ld] of in_type f32, f16 or bf16, kv_heads * dim values a row, rows 16-byte aligned) to their
  * places.  Keys are rotated on the way: the pair (2 i, 2 i + 1) of every head turns by angles[t * angle_ld + 2 i] = {cos, sin} for
- * i < angle_pairs, t the token's row (lv_rotary_table makes such rows); products and sums of the rotation are rounded to f32 one by one.  angles null:
- * none.  tokens: rows of k and v. */
+ * i < angle_pairs, t the token's row: the angles of its position, which the caller lays out by row (lv_rotary_table makes the rows of consecutive positions,
+ * one call per sequence of a step).  Other pairings, of value i with value i + dim / 2 for one, are the caller's to permute (weights once, or rows).
+ * Products and sums of the rotation are rounded to f32 one by one.  angles null: none.  tokens: rows of k and v. */
 int lv_paged_append(lv_ctx* ctx, const lv_paged_cache* cache, const void* k, const void* v, int in_type, uint32_t ld, const float* angles, uint32_t angle_ld,
                     uint32_t angle_pairs, uint32_t tokens);
 
@@ -696,10 +697,15 @@ int lv_paged_read(lv_ctx* ctx, const lv_paged_cache* cache, void* k_out, void* v
  *   s_j = scale * (q . k_j) (scale > 0),   out = sum_j e^(s_j) v_j / (e^(sink_h) + sum_j e^(s_j)).
  * A row that sees nothing gets zeros.  q [tokens][q_ld] and out [tokens][out_ld]: heads * dim values a row, rows 16-byte aligned; q is rotated like the
  * keys of lv_paged_append.  max_new and max_len: upper bounds of the new tokens and of the length of a sequence; they size the launch.
- * Sums, maxima and the softmax are f32.  Output in 16 bits: queries and probabilities enter the matrix products in 16 bits (bf16 for a bf16 cache, else f16).
- * Output in f32: as the sums of two 16-bit numbers each (bf16 caches: three).  Up to 32 rows over a bf16 cache, or over an f16 cache with f16 results, take two numbers as well.  Results in 16 bits of more than 32 rows (new tokens times heads / kv_heads) are fastest with page_rows
- * a multiple of 8.  out does not overlap q.  Places that no new token sees are not looked at, whatever they hold; a value that is not finite reaches the
- * tokens that see it, and may reach others of the same sequence and step.
+ * Sums, maxima and the softmax are f32.  Queries (after their rotation) and probabilities enter the matrix products as 16-bit numbers, bf16 for a bf16 cache, else f16:
+ *   results in f32                                                         two of them (bf16 caches: three)
+ *   results in 16 bits, up to 32 rows of a sequence that share keys        two over a bf16 cache, and over an f16 cache for f16 results; else one
+ *   results in 16 bits, more rows (8-bit caches: any)                      one at least
+ * Rows that share keys are new tokens times heads / kv_heads; which line holds goes by max_new, so that a sequence's results may differ in their last bits
+ * with the company that it is in.  Probabilities over an 8-bit cache enter times the scales of the values, in f16 and in units of the largest scale that the
+ * tokens of a step see in their sequence: a position counts with fewer bits where its scale is below 2^-20 of that.
+ * Results in 16 bits of more than 32 rows (8-bit caches: 96) are fastest with page_rows a multiple of 8.  out does not overlap q.  Places that no new token
+ * sees are not looked at, whatever they hold; a value that is not finite reaches the tokens that see it, and may reach others of the same sequence and step.
  * scratch: 16-byte aligned, lv_paged_attention_scratch_bytes; calls that run at the same time need their own. */
 typedef struct lv_paged_attention_args {
     lv_paged_cache cache;
@@ -733,8 +739,9 @@ int lv_probabilities(lv_ctx* ctx, float* out, uint32_t out_ld, const float* logi
  *   draft i of s is accepted while all before it were and accept[r] * draft[r][d] < target[r][d],  r = starts[s] + i, d = drafted[r]
  *   then one token is drawn from row starts[s] + (number accepted): from max(target - draft, 0) behind a rejected draft (from target where that leaves
  *   nothing), from target behind the last one: the first index whose cumulative weight is above pick[s] * the whole weight
- * accepted[s]: number of drafts accepted; tokens[starts[s] ..]: the accepted drafts, the drawn token, then 0xFFFFFFFF.  A sequence without rows accepts 0 and draws nothing;
- * a draft >= vocab is reported through the error word and rejected; a row without weight or of infinite weight, and a pick outside [0, 1), are reported, the token 0xFFFFFFFF.
+ * accepted[s]: number of drafts accepted; tokens[starts[s] ..]: the accepted drafts, the drawn token, then 0xFFFFFFFF.  A sequence without rows accepts 0
+ * and draws nothing; a draft >= vocab is reported through the error word and rejected; a row without weight or of infinite weight, and a pick outside
+ * [0, 1), are reported, the token 0xFFFFFFFF.
  * lens (may be null): lens[s] -= number of rejected drafts, whose rows in a paged cache are overwritten by the next step (a smaller length is reported and
  * stays).
  * accept, pick: in [0, 1).  Weights are summed in f64. */

@@ -87,9 +87,16 @@ static PagedPlan paged_plan(const lv_ctx* ctx, const lv_paged_attention_args& a)
         return plan;
     }
     const uint32_t group = a.heads / a.cache.kv_heads, rows = a.max_new * group;
-    // 16-bit outputs of more than 32 rows that share their keys: a tile of the tensor cores, whose copies take eight rows of a page at least
+    // 16-bit outputs of more than 32 rows that share their keys (8-bit caches: of more than 96): tiles of the tensor cores, whose copies take eight rows of a page at least.  Both sides,
+    // us in blocks of 32 rows against tiles, 8 key/value heads, rows of the longest sequence:
+    //   16 sequences of 200 to 6000 keys, bf16   40 rows  99, 114    48  110, 114    64  121, 116     96  156, 120
+    //   64 of 500 to 8192, bf16                  40      373, 369                    64  523, 379    128  835, 405        one of 4096   48  31.7, 17.0
+    //   16, e4m3                                 40       83, 213    64  102, 216    96  131, 228    128  165, 240       192  232, 277       320  338, 309
+    //   64, int8                                 40      303, 720    64  430, 739                    128  685, 784       320  1506, 1261
+    //   one of 12000, int8                       40       43, 42     64   47, 44                     128   64, 47         one of 2000, e4m3   96  26.5, 23.4
+    // (a tile's codes are taken apart by four warps, whatever its rows)
     plan.box = std::min(a.cache.page_rows & (0u - a.cache.page_rows), uint32_t(kPtKeys));
-    plan.many = a.out_type != LV_TYPE_F32 && a.cache.dim <= 128 && rows > 32 && plan.box >= 8 && uint64_t(a.cache.pages) * a.cache.kv_heads * a.cache.page_rows < (uint64_t(1) << 31);
+    plan.many = a.out_type != LV_TYPE_F32 && a.cache.dim <= 128 && rows > (paged_is8(a.cache.type) ? 96 : 32) && plan.box >= 8 && uint64_t(a.cache.pages) * a.cache.kv_heads * a.cache.page_rows < (uint64_t(1) << 31);
     plan.rows = plan.many ? kPtRows : std::min((rows + 7) / 8 * 8, a.cache.dim > 128 ? 16u : 32u);
     plan.blocks = (rows + plan.rows - 1) / plan.rows;
     const uint64_t seen = a.window ? std::min<uint64_t>(a.max_len, uint64_t(a.window) + std::min(a.max_new, plan.rows)) : a.max_len;

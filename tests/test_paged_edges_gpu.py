@@ -382,3 +382,28 @@ def test_f32_results_of_many_rows_have_them_too(gpu):
             got = st.launch().result()
             want, bound = attend_tight(c, st.starts, q, 4, st.scale, F32, FEW[kind, F32], FEW[kind, F32], 2)
             assert (np.abs(got - want) <= bound).all()
+
+
+# ---- where the kernels of few rows and of many meet -------------------------------------------------
+
+@pytest.mark.parametrize("kind", [BF16, F16, I8, E4M3], ids=pp.NAMES.get)
+@pytest.mark.parametrize("rows", [24, 32, 33, 40, 95, 96, 97, 98, 128, 129])
+def test_rows_on_both_sides_of_the_kernels_border(gpu, kind, rows):
+    """One query head, so that rows are tokens; a second sequence has a row of its own, a third none."""
+    rng = np.random.default_rng(rows)
+    c = pp.Cache(rng, [rows + 70, 40, 9], 1, 128, kind, 16).fill(rng)
+    with Dev(gpu) as d:
+        for out in (BF16, F16):
+            Step(d, c, [rows, 1, 0], 1, out=out, pairs=32, sink=out == F16).launch().check()
+
+
+@pytest.mark.parametrize("kind", [I8, E4M3], ids=pp.NAMES.get)
+@pytest.mark.parametrize("page,dim,heads,H,lens,new", [(8, 16, 4, 1, [90, 40], [31, 25]), (24, 48, 4, 2, [200, 1, 60], [70, 1, 35]), (40, 112, 4, 1, [700], [33]), (128, 128, 1, 1, [129, 128], [129, 128]),
+                                                       (256, 64, 5, 1, [600, 34], [60, 7]), (8, 128, 8, 2, [1, 300, 0, 257], [1, 64, 0, 65]), (16, 80, 1, 1, [1300], [100])])
+def test_many_rows_of_8_bit_pages(gpu, kind, page, dim, heads, H, lens, new):
+    """More than 96 rows of the longest: boxes of 8 to 128 rows, head sizes that do not fill a block of columns, windows that begin inside a box."""
+    rng = np.random.default_rng(page + dim)
+    c = pp.Cache(rng, lens, H, dim, kind, page).fill(rng)
+    with Dev(gpu) as d:
+        for window, out in ((0, BF16), (37, F16)):
+            Step(d, c, new, heads, out=out, window=window, sink=bool(window), pairs=dim // 2 if window else 0).launch().check()
