@@ -115,8 +115,14 @@ static PagedPlan paged_plan(const lv_ctx* ctx, const lv_paged_attention_args& a)
             if (cost < best) { best = cost; splits = n; }
         }
     } else {
-        // three CTAs per SM hold blocks of up to 16 rows, two the larger ones; sequences of different lengths share the GPU evenly when there are several rounds of CTAs (16 sequences of up to 6000 keys, blocks of 24 rows: 54.7 us with 6 CTAs per SM, 59.2 with 12; 64 of up to 8192, blocks of 8: 127 with 12, 136 with 6)
-        const uint64_t want = uint64_t(ctx->sm_count) * (a.cache.seqs == 1 ? 3 : plan.rows <= 16 ? 12 : 6);
+        // Three CTAs per SM hold blocks of up to 16 rows, two the larger ones.  Where there are fewer blocks than SMs (larger ones: than half of the SMs), splits fill the GPU once: more would be short
+        // ones, each with its start and a part to join.  Where there are more blocks, sequences of different lengths share the GPU evenly when there are several rounds of CTAs.  us with 3, 6 and 12
+        // CTAs per SM, 8 key/value heads, one token (blocks of 8 rows):
+        //   int8  2 sequences of 4096 keys  12.8, 14.6, 14.5    8  21.2, 22.8, 22.3    16 of 500 to 2000  18.8, 21.4, 20.7    24 of 500 to 8192  60, 60, 56    64  145, 134, 125
+        //   bf16  2                         13.6, 15.9, 21.6    8  24.8, 27.9, 29.1    16                 22.0, 25.9, 25.7    24                 80, 91, 84    64  208, 208, 188
+        // six drafts of sequences of 200 to 6000 keys (blocks of 24), e4m3:  2  25.5, 32.5, 32.5    8  30.8, 38.6, 50.7    16  53.5, 52.2, 57.8    32  92, 86, 92    64  163, 148, 145    (bf16  4  40.3, 35.6, 50.6)
+        const bool free_sms = a.cache.seqs == 1 || ctas * (plan.rows <= 16 ? 1 : 2) <= uint64_t(ctx->sm_count);
+        const uint64_t want = uint64_t(ctx->sm_count) * (free_sms ? 3 : plan.rows <= 16 ? 12 : 6);
         splits = std::max<uint64_t>(1, std::min<uint64_t>((want + ctas - 1) / ctas, most));
     }
     uint64_t chunk = ((seen + splits - 1) / splits + unit - 1) / unit * unit;
