@@ -399,8 +399,12 @@ extern "C" int lv_probabilities(lv_ctx* ctx, float* out, uint32_t out_ld, const 
     LV_ENTER(ctx);
     if (!rows) return LV_OK;
     Probabilities p{out, logits, temperature, out_ld, ld, vocab, 0};
-    // few rows: as many CTAs as hold the row, down to 2048 values each; many: eight, which read it a second time from the L2 (5 rows of 32000: 4.5 us held, 5.2 read again; 512 rows of 128000: 127 us with eight, 131 with four and four CTAs per SM)
-    const bool few = uint64_t(rows) * 8 <= 2 * uint64_t(ctx->sm_count);
+    // few rows: as many CTAs as hold the row, down to 2048 values each; many: eight, which read a larger one a second time from the L2.  us with 16 and with 8:
+    //   128000 values  5 rows 5.5, 6.5    18  8.7, 12.4    24  12.5, 13.4    30  15.0, 13.2    37  18.7, 13.8
+    //    70000         5      5.0, 6.1    16  8.2, 10.6    24  11.3, 10.8    30  12.4, 10.9
+    //   200000         5      7.7, 8.7    16 12.7, 17.6    24  19.4, 18.5    30  21.6, 18.8
+    // (512 rows of 128000: 127 with eight, 131 with four and four CTAs per SM, on an earlier state)
+    const bool few = uint64_t(rows) * 6 <= uint64_t(ctx->sm_count);
     uint32_t n = 1;
     while (n < (few && vocab > 8 * kProbHeld ? uint32_t(kProbCluster) : 8u) && vocab / (2 * n) >= 2048) n *= 2;
     p.each = ((vocab + n - 1) / n + 3) / 4 * 4;

@@ -407,3 +407,20 @@ def test_many_rows_of_8_bit_pages(gpu, kind, page, dim, heads, H, lens, new):
     with Dev(gpu) as d:
         for window, out in ((0, BF16), (37, F16)):
             Step(d, c, new, heads, out=out, window=window, sink=bool(window), pairs=dim // 2 if window else 0).launch().check()
+
+
+@pytest.mark.parametrize("rows", [24, 25, 37, 38])
+@pytest.mark.parametrize("vocab", [65536, 65540, 70001, 131072, 200000])
+def test_probabilities_on_both_sides_of_the_clusters_border(gpu, rows, vocab):
+    rng = np.random.default_rng(rows)
+    x = (rng.standard_normal((rows, vocab)) * 4).astype(np.float32)
+    with Dev(gpu) as d:
+        out = d.zeros(x.nbytes)
+        d.call("lv_probabilities", out, vocab, d.f32(x), vocab, vocab, rows, None)
+        got = d.get(out, x.shape)
+    z = x.astype(np.float64) - x.max(1, keepdims=True).astype(np.float64)
+    e = np.exp(z)
+    e /= e.sum(1, keepdims=True)
+    # an exponential's argument is off by 2^-22 of itself, the exponential by 2^-22, the sum by the mean of both and its longest chain of additions
+    tol = np.abs(z) * 2.0 ** -22 + 2.0 ** -22 + (np.abs(z) * e).sum(1, keepdims=True) * 2.0 ** -22 + (128 + vocab / 1024) * 2.0 ** -24
+    assert (np.abs(got - e) <= tol * e).all()
