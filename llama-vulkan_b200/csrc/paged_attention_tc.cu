@@ -14,9 +14,9 @@
 // pattern): 16-bit rows straight into the operands' swizzle, 8-bit codes into a ring, from which four warps convert them to f16 (exact).  cp.async by the same four
 // warps was tried first and kept the load and store unit so busy that every other warp of the CTA waited for it (1142 us against 1084).  Places that no query sees are not
 // fetched, or zeroed behind the copy: their weights are zero, but zero times NaN is not.  References, f16 ranges and scales as in paged_attention_rows.cuh.
-// Two prompts of 2048 tokens behind 9001 to 16384 keys, bf16, 32/8 heads of 128: 947 us, 862 TFLOP/s of 1681 that a library's large product reaches.  Bound by the chain of a
-// unit, not by one pipe: with the softmax left out the copies and products take 775 us, with the products left out the softmax takes 744, and the two units hide
-// only a part of one behind the other.  Without turns at the exponentials: 1003 us.  A quarter of the exponentials by a polynomial on the multipliers: 1003 us with
+// Two prompts of 2048 tokens behind 9001 to 16384 keys, bf16, 32/8 heads of 128: 931 us, 876 TFLOP/s of 1681 that a library's large product reaches.  Bound by the chain of a
+// unit, not by one pipe: with the softmax left out the copies and products took 775 us, with the products left out the softmax took 744 (947 together then), and the two units hide
+// only a part of one behind the other.  Two of 512 behind 4096 to 8192: bf16 165 us, f16 175, int8 399, e4m3 371 (the four warps' conversions).  Without turns at the exponentials: 1003 us.  A quarter of the exponentials by a polynomial on the multipliers: 1003 us with
 // turns, for its instructions take the issue slots that the turns have freed.  Steps that one warp issued for both units: 1084 us.
 //
 // Every wait is bounded; one that gives up sets the error word, and the CTA drains and frees its tensor memory.

@@ -32,7 +32,7 @@ __device__ __forceinline__ void cluster_all_here() { asm volatile("barrier.clust
 
 // out = e^((x - m) / T) / sum: a cluster of up to 16 CTAs takes a row and its CTAs tell one another their maximum and sum once.  Where a CTA's share fits its
 // registers (HELD: 8192 values) a value is read, raised and written once; else every thread keeps a running maximum and sum, and values are read (from the L2) and raised a second time.
-// 512 rows of 128000: 121 us, 4.3 TB/s of 524 MB (one CTA per row: 418 us; all of a row held in registers, eight groups a thread: 165; every load with its bounds: 125).  5 rows of 32000: 4.5 us, a launch and two meetings.
+// 512 rows of 128000: 121 us, 4.3 TB/s of 524 MB; of 128001, off their 16 bytes: 203 (one CTA per row: 418 us; all of a row held in registers, eight groups a thread: 165; every load with its bounds: 125).  5 rows of 32000: 4.4 us, a launch and two meetings (read again: 5.2).
 constexpr int kProbThreads = 512, kProbGroups = 4;                       // groups of four values that a thread holds, or has on their way at a time
 constexpr uint32_t kProbHeld = kProbThreads * 4 * kProbGroups;           // of a CTA: 8192
 constexpr int kProbCluster = 16;
@@ -207,9 +207,9 @@ __global__ void __launch_bounds__(kProbThreads, 3) probabilities_kernel(const Pr
 // for both neighbours and never decrease, and the target is below the last one (pick is at most 1 - 2^-24), so that exactly one run holds it, one with weight; its warp looks through it
 // again.  Sums are f64: the first index whose cumulative weight is above
 // the target does not depend on the order of the sums but where the two agree to 2^-52.
-// 64 sequences with up to 7 drafts, vocabulary 128000: 22 us, 3.0 TB/s of 65 MB: two CTAs per SM by their registers, so 1.7 rounds that each wait for look-ups and loads (one CTA per
+// 64 sequences with up to 7 drafts, vocabulary 128000: 21.7 us, 3.0 TB/s of 65 MB: two CTAs per SM by their registers, so 1.7 rounds that each wait for look-ups and loads (one CTA per
 // sequence: 110 us; 256 threads: 20.7, but 4.65 for one sequence; clusters of four: 21.1 and 4.9).  One
-// sequence with 4 drafts: 4.1 us, a launch and its meetings (72 us).
+// sequence with 4 drafts: 4.3 us, a launch and its meetings (72 us).
 constexpr int kVerifyThreads = 512, kVerifyWarps = kVerifyThreads / 32, kVerifyCluster = 8;
 constexpr uint32_t kNobody = 0xffffffffu;
 
