@@ -424,3 +424,113 @@ def test_probabilities_on_both_sides_of_the_clusters_border(gpu, rows, vocab):
     # an exponential's argument is off by 2^-22 of itself, the exponential by 2^-22, the sum by the mean of both and its longest chain of additions
     tol = np.abs(z) * 2.0 ** -22 + 2.0 ** -22 + (np.abs(z) * e).sum(1, keepdims=True) * 2.0 ** -22 + (128 + vocab / 1024) * 2.0 ** -24
     assert (np.abs(got - e) <= tol * e).all()
+
+
+# ---- the largest and the most, and what is recorded ----------------------------------------------------
+
+def test_the_most_sequences(gpu):
+    """65535 of one position each: a result is the value itself."""
+    n, dim = 65535, 16
+    rng = np.random.default_rng(5)
+    k, v, q = (rng.standard_normal((n, dim)).astype(np.float32) for _ in range(3))
+    v = pp.rounded(v, F16)
+    with Dev(gpu) as d:
+        cache = pkg.PagedCache(k=d.zeros(n * dim * 2).value, v=d.zeros(n * dim * 2).value, type=F16, pages=n, page_rows=1, kv_heads=1, dim=dim, table=d.u32(rng.permutation(n)).value, table_ld=1,
+                               lens=d.u32(np.ones(n)).value, starts=d.u32(np.arange(n + 1)).value, seqs=n)
+        d.call("lv_paged_append", C.byref(cache), d.f32(k), d.f32(v), F32, dim, None, 0, 0, n)
+        out = d.zeros(n * dim * 4)
+        a = pkg.PagedAttentionArgs(cache=cache, q=d.f32(q).value, q_type=F32, q_ld=dim, heads=1, tokens=n, max_new=1, max_len=1, scale=0.25, out=out.value, out_type=F32, out_ld=dim)
+        nbytes = gpu.lib.lv_paged_attention_scratch_bytes(gpu.handle, C.byref(a))
+        d.call("lv_paged_attention", C.byref(a), d.zeros(nbytes), nbytes)
+        # a weight of 2^10 is exact, the quotient is rounded twice
+        assert (np.abs(d.get(out, (n, dim)) - v) <= 2.0 ** -22 * np.abs(v)).all()
+
+
+@pytest.mark.parametrize("kind", [F16, I8], ids=pp.NAMES.get)
+@pytest.mark.parametrize("new", [1, 3, 200])
+def test_positions_near_the_largest(gpu, kind, new):
+    """One page of 2^20 rows that a table names 2047 times, and a window over the last positions below 2^31."""
+    page, dim, slots, window = 1 << 20, 16, 2047, 70
+    length = slots * page
+    rng = np.random.default_rng(new)
+    width = new + window - 1
+    x, v = (rng.standard_normal((width, 1, dim)).astype(np.float32) for _ in range(2))
+    eight = kind in pp.TOP
+    with Dev(gpu) as d:
+        bufs = [d.zeros(page * dim * (1 if eight else 2)) for _ in range(2)] + [d.zeros(page * 4) for _ in range(2)]
+        lens = d.u32([length])
+        cache = pkg.PagedCache(k=bufs[0].value, v=bufs[1].value, k_scale=bufs[2].value if eight else None, v_scale=bufs[3].value if eight else None, type=kind, pages=1, page_rows=page, kv_heads=1,
+                               dim=dim, table=d.u32(np.zeros(slots)).value, table_ld=slots, lens=lens.value, starts=d.u32([0, width]).value, seqs=1)
+        d.call("lv_paged_append", C.byref(cache), d.f32(x), d.f32(v), F32, dim, None, 0, 0, width)
+        c = pp.Cache(rng, [width], 1, dim, kind, 256)                    # the same rows as a short sequence
+        c.write(0, np.arange(width), 0, x)
+        c.write(0, np.arange(width), 1, v)
+        for out in (F32, BF16):
+            q = rng.standard_normal((new, 1, dim)).astype(np.float32)
+            to = d.zeros(new * dim * 4)
+            cache.starts = d.u32([0, new]).value
+            a = pkg.PagedAttentionArgs(cache=cache, q=d.f32(q).value, q_type=F32, q_ld=dim, heads=1, tokens=new, max_new=new, max_len=length, scale=0.25, window=window, out=to.value, out_type=out,
+                                       out_ld=dim)
+            nbytes = gpu.lib.lv_paged_attention_scratch_bytes(gpu.handle, C.byref(a))
+            d.call("lv_paged_attention", C.byref(a), d.zeros(nbytes), nbytes)
+            got = pp.values(gpu.download(to, np.float32 if out == F32 else np.uint16, new * dim), out).reshape(new, 1, dim)
+            want, bound = pp.attend(c, [0, new], q, 1, 0.25, window, out_kind=out)
+            assert (np.abs(got - want) <= bound).all()
+
+
+def test_the_largest_vocabulary(gpu):
+    n = 1 << 24
+    rng = np.random.default_rng(24)
+    x = rng.standard_normal((2, n)).astype(np.float32)
+    with Dev(gpu) as d:
+        p = d.zeros(2 * n * 4)
+        d.call("lv_probabilities", p, n, d.f32(x), n, n, 2, None)
+        got = d.get(p, (2, n))
+    e = np.exp(x.astype(np.float64))
+    e /= e.sum(1, keepdims=True)
+    assert np.abs(got / e - 1).max() <= 2.0 ** -18                      # (arguments of at most 11 in magnitude, sums of 2^20 terms in chains of 2^11)
+    drafted, accept, pick = np.array([n - 1, 0], np.uint32), np.array([0.999, 0.0], np.float32), np.array([0.73], np.float32)
+    draft = np.zeros((2, n), np.float32)
+    draft[0, n - 1] = 1.0
+    k, t, _, failed = run_verify(gpu, got, draft, drafted, [0, 2], accept, pick)
+    assert failed is None and list(k) == [0]
+    cum = np.cumsum(np.maximum(got[0].astype(np.float64) - draft[0], 0))
+    at = int(t[0])
+    assert cum[at] > 0.73 * cum[-1] * (1 - 1e-6) and (at == 0 or cum[at - 1] <= 0.73 * cum[-1] * (1 + 1e-6))
+    k, t, _, failed = run_verify(gpu, got, None, drafted, [0, 2], np.zeros(2, np.float32), pick)
+    assert failed is None and list(k) == [1] and t[0] == n - 1
+
+
+@pytest.mark.parametrize("rows,vocab", [(3, 200), (5, 70001), (20, 140000), (60, 33000)])
+def test_probabilities_and_verification_in_a_recorded_step(gpu, rows, vocab):
+    """Recorded once, replayed with other logits, drafts, random numbers and lengths."""
+    rng = np.random.default_rng(vocab)
+    starts = np.array([0, rows // 2, rows])
+    lib, h = gpu.lib, gpu.handle
+    with Dev(gpu) as d:
+        dx, dp, dt = d.zeros(rows * vocab * 4), d.zeros(rows * vocab * 4), d.f32(np.full(rows, 0.8))
+        drafted, accept, pick, tok, acc, lens = d.zeros(rows * 4), d.zeros(rows * 4), d.zeros(8), d.zeros(rows * 4), d.zeros(8), d.zeros(8)
+        a = pkg.VerifyArgs(target=dp.value, target_ld=vocab, vocab=vocab, drafted=drafted.value, starts=d.u32(starts).value, seqs=2, rows=rows, accept=accept.value, pick=pick.value,
+                           tokens=tok.value, accepted=acc.value, lens=lens.value)
+        pkg.check(lib.lv_graph_begin_capture(h))
+        pkg.check(lib.lv_probabilities(h, dp, vocab, dx, vocab, vocab, rows, dt))
+        pkg.check(lib.lv_verify_drafts(h, C.byref(a)))
+        g = C.c_void_p()
+        pkg.check(lib.lv_graph_end_capture(h, C.byref(g)))
+        for step in range(3):
+            x = (rng.standard_normal((rows, vocab)) * 3).astype(np.float32)
+            drafts, u, picks = x.argmax(1).astype(np.uint32), rng.random(rows).astype(np.float32) * np.float32(0.3), rng.random(2).astype(np.float32)
+            for b, host in ((dx, x), (drafted, drafts), (accept, u), (pick, picks), (lens, np.full(2, 100, np.uint32))):
+                pkg.check(lib.lv_upload(h, b, np.ascontiguousarray(host).ctypes.data_as(C.c_void_p), host.nbytes))
+            pkg.check(lib.lv_graph_launch(h, g))
+            gpu.sync()
+            p = d.get(dp, (rows, vocab))
+            z = x.astype(np.float64) / np.float64(np.float32(0.8))
+            e = np.exp(z - z.max(1, keepdims=True))
+            e /= e.sum(1, keepdims=True)
+            assert (np.abs(p - e) <= (40 * 2.0 ** -21 + (128 + vocab / 1024) * 2.0 ** -24) * e + 1e-37).all()          # (arguments of at most 40 in magnitude, see test_probabilities)
+            wn, wt = pp.verify(p, None, drafts, starts, u, picks)
+            n = gpu.download(acc, np.uint32, 2)
+            assert np.array_equal(n, wn) and np.array_equal(gpu.download(tok, np.uint32, rows), wt)
+            assert np.array_equal(gpu.download(lens, np.uint32, 2), 100 - (np.diff(starts) - 1 - wn))
+        lib.lv_graph_destroy(g)
