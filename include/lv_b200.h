@@ -703,7 +703,7 @@ int lv_paged_read(lv_ctx* ctx, const lv_paged_cache* cache, void* k_out, void* v
  *   results in 16 bits, more rows (8-bit caches: any)                      one at least
  * Rows that share keys are new tokens times heads / kv_heads; which line holds goes by max_new, so that a sequence's results may differ in their last bits
  * with the company that it is in.  Probabilities over an 8-bit cache enter times the scales of the values, in f16 and in units of the largest scale that the
- * tokens of a step see in their sequence: a position counts with fewer bits where its scale is below 2^-20 of that.
+ * tokens of a step see in their sequence: a position counts with fewer bits where its scale is below 2^-20 (results in f32: 2^-12) of that.
  * Results in 16 bits of more than 32 rows (8-bit caches: 96) are fastest with page_rows a multiple of 8.  out does not overlap q.  Places that no new token
  * sees are not looked at, whatever they hold; a value that is not finite reaches the tokens that see it, and may reach others of the same sequence and step.
  * scratch: 16-byte aligned, lv_paged_attention_scratch_bytes; calls that run at the same time need their own. */

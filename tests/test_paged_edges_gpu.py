@@ -534,3 +534,22 @@ def test_probabilities_and_verification_in_a_recorded_step(gpu, rows, vocab):
             assert np.array_equal(n, wn) and np.array_equal(gpu.download(tok, np.uint32, rows), wt)
             assert np.array_equal(gpu.download(lens, np.uint32, 2), 100 - (np.diff(starts) - 1 - wn))
         lib.lv_graph_destroy(g)
+
+
+@pytest.mark.parametrize("kind", [I8, E4M3], ids=pp.NAMES.get)
+@pytest.mark.parametrize("out", [F32, BF16], ids=["to-f32", "to-bf16"])
+@pytest.mark.parametrize("new", [3, 120])
+@pytest.mark.parametrize("times", [12, 20])
+def test_values_far_below_another_rows(gpu, kind, out, new, times):
+    """The last position's values are 2^12 or 2^20 times the others', which all tokens before it do not see: weights are whole multiples of 2^-35 of the largest in units of the largest scale,
+    which leaves 11 bits at 2^20 and 22 at 2^12."""
+    rng = np.random.default_rng(times)
+    c = pp.Cache(rng, [300], 1, 64, kind, 16).fill(rng)
+    c.write(0, [299], 1, np.float32(2.0 ** times) * rng.standard_normal((1, 1, 64)).astype(np.float32))
+    with Dev(gpu) as d:
+        st = Step(d, c, [new], 1, out=out, behind=0)
+        got = st.launch().result()
+        u = 2.0 ** -22 if out == F32 else 2.0 ** -11
+        want, bound = attend_tight(c, st.starts, st.q.reshape(new, 1, 64), 1, st.scale, out, u, u, 64)
+        largest = np.abs(c.read(0, np.arange(300), 1)).max()
+        assert (np.abs(got - want) <= bound + 300 * 2.0 ** -35 * largest).all()
