@@ -93,14 +93,17 @@ __global__ void __launch_bounds__(kProbThreads, 3) probabilities_kernel(const Pr
     float top = -INFINITY, sum = 0.f, base = 0.f;
     uint32_t at = 0xffffffffu;
     auto look = [&](const float4& w, uint32_t i) {
-        // (in the order of the indexes: a later value has to be larger, but for the first that is a number, which may be -inf; what lies behind the end is nobody's)
-        auto one = [&](float z, uint32_t j) {
-            if (z > top || (z == top && at == 0xffffffffu && j < hi)) { top = z; at = j; }
-        };
-        one(w.x, i);
-        one(w.y, i + 1);
-        one(w.z, i + 2);
-        one(w.w, i + 3);
+        // (in the order of the indexes: a later value has to be larger)
+        if (w.x > top) { top = w.x; at = i; }
+        if (w.y > top) { top = w.y; at = i + 1; }
+        if (w.z > top) { top = w.z; at = i + 2; }
+        if (w.w > top) { top = w.w; at = i + 3; }
+        if (at == 0xffffffffu) {                                         // nothing above -inf so far: the first -inf itself (what lies behind the end is nobody's)
+            if (w.w == top && i + 3 < hi) at = i + 3;
+            if (w.z == top && i + 2 < hi) at = i + 2;
+            if (w.y == top && i + 1 < hi) at = i + 1;
+            if (w.x == top && i < hi) at = i;
+        }
     };
     auto raise4 = [&](const float4& w) { return make_float4(exp2_fast((w.x - base) * f), exp2_fast((w.y - base) * f), exp2_fast((w.z - base) * f), exp2_fast((w.w - base) * f)); };
     const uint32_t mine0 = lo + 4 * threadIdx.x;
